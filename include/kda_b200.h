@@ -279,6 +279,62 @@ int kda_selftest_mma(const float *A, const float *B, float *D, int N, int K, int
  * The device stays usable; the tests use it to check that a given-up wait is reported. */
 int kda_selftest_wait(const float *src, float *dst, int poll_limit, int code, int *status, void *cuda_stream);
 
+/* ---- gated delta rule with one decay per value head -------------------------------------------------------------
+ * S~ = e^g S;  e = beta (v - S~^T k);  S' = S~ + k e^T;  o = scale S'^T q      per sequence and value head
+ *   q, k : [B, T, H, dk]      v, o : [B, T, HV, dv]      g, beta : [B, T, HV]      states : [N, HV, dk, dv] float
+ * HV is a multiple of H: value head h goes with key head h / (HV / H).  dk and dv are 64 or 128, each by itself.
+ * KDA_FLAG_QK_L2NORM, _GATE (g is the gate's input, the log decay is -exp(A_log[h]) softplus(g + dt_bias[h])), _BETA_SIGMOID and
+ * _STATE_V_FIRST ([N, HV, dv, dk] states) mean what they mean for kda_fwd.  Rows of q, k are divided by max(norm, 1e-6) in FP32.
+ * Log decays below -1000 count as -1000 (their exponential is 0 in FP32 either way).  Rows outside the sequences are not
+ * touched.  Every tensor starts on a 16-byte boundary; workspace and scratch on 256 bytes. */
+typedef struct KdaGdrParams {
+    int32_t B, T, H, HV, dk, dv;
+    int32_t N, NT;               /* sequences; 64-token chunks over all of them */
+    int32_t dtype, g_dtype;      /* of q, k, v, o, grad_o and their gradients; of g, beta and theirs */
+    int32_t flags;
+    float scale;
+    const void *q, *k, *v, *g, *beta;
+    const float *A_log, *dt_bias; /* [HV]; dt_bias may be NULL */
+    const float *h0;             /* may be NULL */
+    const int64_t *cu_seqlens;   /* device [N+1], may be NULL; B is 1 with it, and the three tables below are needed */
+    const int32_t *chunk_seq, *seq_chunk_off, *chunk_tab; /* as in KdaParams */
+    void *o;
+    float *ht;                   /* may be NULL */
+    void *workspace;             /* kda_gdr_workspace_bytes(); written by kda_gdr_fwd, read by kda_gdr_bwd unless KDA_FLAG_NO_SAVE */
+    size_t workspace_bytes;
+    const void *grad_o;
+    const float *grad_ht;        /* may be NULL */
+    void *grad_q, *grad_k, *grad_v, *grad_g, *grad_beta;
+    float *grad_A_log, *grad_dt_bias; /* needed with KDA_FLAG_GATE (grad_dt_bias only where dt_bias is given) */
+    float *grad_h0;              /* may be NULL */
+    void *bwd_scratch;
+    size_t bwd_scratch_bytes;
+} KdaGdrParams;
+int kda_gdr_workspace_bytes(const KdaGdrParams *p, size_t *fwd_bytes, size_t *bwd_bytes);
+int kda_gdr_fwd(const KdaGdrParams *p, void *cuda_stream);
+int kda_gdr_bwd(const KdaGdrParams *p, void *cuda_stream);
+
+/* The same recurrence token by token in one launch, the state on chip in between (decoding).  state_in NULL: zero initial state;
+ * state_out NULL: no final state; they may be equal. */
+int kda_gdr_recurrent_fwd(const void *q, const void *k, const void *v, const void *g, const void *beta, const float *A_log,
+                          const float *dt_bias, const float *state_in, float *state_out, void *o, int32_t N, int32_t T, int32_t H,
+                          int32_t HV, int32_t dk, int32_t dv, int32_t dtype, int32_t g_dtype, int32_t flags, float scale,
+                          void *cuda_stream);
+
+/* Group normalisation with an activation, channels last: x, y [N, S, channels], statistics over the S positions and
+ * channels / groups channels of every (sample, group); y = act((x - mean) / sqrt(var + eps) * weight + bias), act SiLU or none.
+ * weight, bias [channels] may be NULL (1, 0).  mean, rstd [N, groups] are written by the forward and read by the backward unless
+ * S == 1 with groups of at most 1024 channels, where they and the forward's scratch may be NULL.  dweight and dbias: both or
+ * neither. */
+int kda_group_norm_scratch_bytes(int64_t N, int64_t S, int32_t channels, int32_t groups, int32_t dtype, size_t *fwd_bytes,
+                                 size_t *bwd_bytes);
+int kda_group_norm_fwd(const void *x, const float *weight, const float *bias, void *y, float *mean, float *rstd, float *scratch,
+                       int64_t N, int64_t S, int32_t channels, int32_t groups, float eps, int32_t silu, int32_t dtype,
+                       void *cuda_stream);
+int kda_group_norm_bwd(const void *x, const float *weight, const float *bias, const float *mean, const float *rstd, const void *dy,
+                       void *dx, float *dweight, float *dbias, float *scratch, int64_t N, int64_t S, int32_t channels,
+                       int32_t groups, float eps, int32_t silu, int32_t dtype, void *cuda_stream);
+
 /* Launches a one-thread kernel on the given stream that copies a non-zero *status into *status_host
  * (pinned, device-mapped): for entry points that take a bare status pointer, such as kda_recurrent_step. */
 int kda_status_publish(const int32_t *status, int32_t *status_host, void *cuda_stream);

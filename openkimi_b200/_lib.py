@@ -46,6 +46,17 @@ class KdaParams(C.Structure):
     ]
 
 
+class KdaGdrParams(C.Structure):
+    """Field-for-field mirror of ``struct KdaGdrParams`` in include/kda_b200.h."""
+
+    _fields_ = (
+        [(n, C.c_int32) for n in ("B", "T", "H", "HV", "dk", "dv", "N", "NT", "dtype", "g_dtype", "flags")] + [("scale", C.c_float)]
+        + [(n, C.c_void_p) for n in ("q", "k", "v", "g", "beta", "A_log", "dt_bias", "h0", "cu_seqlens", "chunk_seq", "seq_chunk_off",
+                                     "chunk_tab", "o", "ht", "workspace")] + [("workspace_bytes", C.c_size_t)]
+        + [(n, C.c_void_p) for n in ("grad_o", "grad_ht", "grad_q", "grad_k", "grad_v", "grad_g", "grad_beta", "grad_A_log",
+                                     "grad_dt_bias", "grad_h0", "bwd_scratch")] + [("bwd_scratch_bytes", C.c_size_t)])
+
+
 EXPORTS = {
     "kda_abi_version": (C.c_int, []),
     "kda_guard_version": (C.c_int, []),
@@ -75,6 +86,13 @@ EXPORTS = {
     "kda_short_conv_bwd_static": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32,
                                             C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p, C.c_int32,
                                             C.c_void_p]),
+    "kda_gdr_workspace_bytes": (C.c_int, [C.POINTER(KdaGdrParams), C.POINTER(C.c_size_t), C.POINTER(C.c_size_t)]),
+    "kda_gdr_fwd": (C.c_int, [C.POINTER(KdaGdrParams), C.c_void_p]),
+    "kda_gdr_bwd": (C.c_int, [C.POINTER(KdaGdrParams), C.c_void_p]),
+    "kda_gdr_recurrent_fwd": (C.c_int, [C.c_void_p] * 10 + [C.c_int32] * 9 + [C.c_float, C.c_void_p]),
+    "kda_group_norm_scratch_bytes": (C.c_int, [C.c_int64] * 2 + [C.c_int32] * 3 + [C.POINTER(C.c_size_t)] * 2),
+    "kda_group_norm_fwd": (C.c_int, [C.c_void_p] * 7 + [C.c_int64] * 2 + [C.c_int32] * 2 + [C.c_float] + [C.c_int32] * 2 + [C.c_void_p]),
+    "kda_group_norm_bwd": (C.c_int, [C.c_void_p] * 10 + [C.c_int64] * 2 + [C.c_int32] * 2 + [C.c_float] + [C.c_int32] * 2 + [C.c_void_p]),
     "kda_norm_gate_fwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
                                     C.c_int32, C.c_float, C.c_int32, C.c_void_p]),
     "kda_norm_gate_bwd": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,

@@ -1,0 +1,205 @@
+// Gated delta rule with one decay per value head: shared definitions of its kernels.
+//
+// With one decay per head the pairwise decays of a chunk are numbers, not vectors: q k^T and k k^T are plain products of the
+// rows as they arrive, and decay, beta and the rows' 1 / norm multiply the results in FP32.  So in BF16 mode every product has
+// an operand that BF16 holds exactly (q, k, do) or two computed ones (T, V', S, ...).  Computed operands are BF16 in up to three
+// parts, x = p0 + p1 + p2 to 2^-24, and a product of parts i and j is taken where i + j < 3: FP32-class results (measured against
+// 64 bits: 2e-7 to 1e-6) from tensor cores with FP32 accumulators.  Where only a BF16 output can see the difference two parts do
+// (2^-17).  FP32 tensors go the same way with three parts for q, k, v, do as well.
+#pragma once
+
+#include "kda_common.cuh"
+#include "kda_tc.cuh"
+
+namespace kda {
+namespace gdr {
+
+using namespace tc;
+using bf16 = __nv_bfloat16;
+
+constexpr int NBLK = 10;           // 16 x 16 blocks of a lower triangular 64 x 64 matrix
+constexpr int BLK = 256;           // elements of one
+constexpr int TRI = NBLK * BLK;    // elements of one part of such a matrix
+constexpr int AUX = 8 * C;         // floats of a unit's per-row numbers
+enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST };  // e^G, e^(G_last - G), beta, 1/|q|, 1/|k|, G in two floats; [A_LAST][0] = e^G_last
+constexpr float G_MIN = -1000.f;   // log decays below count as this: e^-1000 is 0 in FP32, and sums of 64 stay finite
+
+__host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I * (I + 1) / 2 + J; }
+
+// per (chunk, value head) unit, byte offsets
+struct Layout {
+    size_t aux, T, A, total_nosave, S0, Vn, total;        // workspace
+    size_t dS, Y, part, dqk, bwd_total;                   // backward scratch
+};
+__host__ __device__ inline Layout layout(const KdaGdrParams& p) {
+    const size_t n = (size_t)p.NT * p.HV;
+    Layout l;
+    size_t off = 0;
+    l.aux = off; off = align256(off + n * AUX * 4);
+    l.T = off;   off = align256(off + n * 3 * TRI * 2);   // (I + diag(beta) L)^-1 and scale (q k^T) D as three BF16 parts, blocks of
+    l.A = off;   off = align256(off + n * 3 * TRI * 2);   // the lower triangle in blk() order, rows swizzled as tri_frag reads them
+    l.total_nosave = off;
+    l.S0 = off;  off = align256(off + n * p.dk * p.dv * 4);  // state at the chunk's start [dk][dv]
+    l.Vn = off;  off = align256(off + n * C * p.dv * 4);     // V' [64][dv]
+    l.total = off;
+    off = 0;
+    l.dS = off;   off = align256(off + n * p.dk * p.dv * 4); // gradient of the state at the chunk's end
+    l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV'
+    l.part = off; off = align256(off + n * 2 * 4);           // this unit's share of dA_log and ddt_bias
+    l.dqk = off;  if (p.HV != p.H) off = align256(off + n * 2 * C * p.dk * 4);  // shared key heads: this value head's share of dq, dk
+    l.bwd_total = off;
+    return l;
+}
+
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldsm(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm_t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+
+// Fragments of a row-major tile X with rows of LD elements (LD = 8 mod 16 keeps the eight rows of a matrix in different banks).
+// a_frag: the 16 x 16 block of X at (r, c) as A.   a_frag_t: the block at (r, c) of X^T as A (X holds it at (c, r)).
+// b_frag: X holds B^T, rows n: 16 columns n.. of B, k..k+16.   b_frag_t: X holds B, rows k.   Both give two column tiles (b[0..1], b[2..3]).
+template <int LD>
+__device__ __forceinline__ void a_frag(uint32_t (&f)[4], uint32_t x, int r, int c, int lane) {
+    ldsm(f, x + 2 * ((r + (lane & 15)) * LD + c + (lane >> 4) * 8));
+}
+template <int LD>
+__device__ __forceinline__ void a_frag_t(uint32_t (&f)[4], uint32_t x, int r, int c, int lane) {
+    ldsm_t(f, x + 2 * ((c + (lane & 7) + (lane >> 4) * 8) * LD + r + ((lane >> 3) & 1) * 8));
+}
+template <int LD>
+__device__ __forceinline__ void b_frag(uint32_t (&f)[4], uint32_t x, int n, int k, int lane) {
+    ldsm(f, x + 2 * ((n + (lane & 7) + (lane >> 4) * 8) * LD + k + ((lane >> 3) & 1) * 8));
+}
+template <int LD>
+__device__ __forceinline__ void b_frag_t(uint32_t (&f)[4], uint32_t x, int n, int k, int lane) {
+    ldsm_t(f, x + 2 * ((k + (lane & 7) + ((lane >> 3) & 1) * 8) * LD + n + (lane >> 4) * 8));
+}
+// 16 x 16 blocks of a lower triangular matrix as the workspace holds them: rows of 32 bytes whose halves change places in rows
+// 4..7 and 12..15, so that eight rows of a matrix lie in different banks
+__device__ __forceinline__ int tri_idx(int r, int c) { return r * 16 + ((((c >> 3) ^ (r >> 2)) & 1) << 3) + (c & 7); }
+__device__ __forceinline__ void tri_frag(uint32_t (&f)[4], uint32_t x, int b, int lane) {
+    ldsm(f, x + 2 * (b * BLK + tri_idx(lane & 15, (lane >> 4) * 8)));
+}
+__device__ __forceinline__ void tri_frag_t(uint32_t (&f)[4], uint32_t x, int b, int lane) {
+    ldsm_t(f, x + 2 * (b * BLK + tri_idx((lane & 7) + (lane >> 4) * 8, ((lane >> 3) & 1) * 8)));
+}
+
+// products of the parts of one A block and two column tiles of B
+template <int PA, int PB, int ORD, int NT>
+__device__ __forceinline__ void mma_parts(float (&acc)[NT][4], int pair, const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][4]) {
+#pragma unroll
+    for (int j = PB - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = PA - 1; i >= 0; --i)
+            if (i + j < ORD) {
+                mma(acc[2 * pair], a[i], b[j][0], b[j][1]);
+                mma(acc[2 * pair + 1], a[i], b[j][2], b[j][3]);
+            }
+}
+
+template <int P>
+__device__ __forceinline__ void split(float x0, float x1, uint32_t (&w)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+        x0 -= __uint_as_float(w[i] << 16);
+        x1 -= __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+// two neighbouring elements into the P part tiles at element offset idx
+template <int P>
+__device__ __forceinline__ void put(bf16* tile, int part, int idx, float x0, float x1) {
+    uint32_t w[P];
+    split(x0, x1, w);
+#pragma unroll
+    for (int i = 0; i < P; ++i) *reinterpret_cast<uint32_t*>(tile + i * part + idx) = w[i];
+}
+template <int P>
+__device__ __forceinline__ void put4(bf16* tile, int part, int idx, const float4& x) {
+    uint32_t a[P], b[P];
+    split(x.x, x.y, a);
+    split(x.z, x.w, b);
+#pragma unroll
+    for (int i = 0; i < P; ++i) *reinterpret_cast<uint2*>(tile + i * part + idx) = make_uint2(a[i], b[i]);
+}
+// two neighbouring elements of a tile in P parts
+template <int P>
+__device__ __forceinline__ float2 get2(const bf16* tile, int part, int idx) {
+    float2 x = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = P - 1; i >= 0; --i) {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + i * part + idx);
+        x.x += __uint_as_float(w << 16);
+        x.y += __uint_as_float(w & 0xffff0000u);
+    }
+    return x;
+}
+
+template <typename T> struct In;
+template <> struct In<bf16> { static constexpr int P = 1, PO = 2; };   // parts of inputs; of computed operands behind a 16-bit output
+template <> struct In<float> { static constexpr int P = 3, PO = 3; };
+
+// rows of COLS elements, `stride` apart in memory, into row-major part tiles; rows from `rows` on are zero
+template <int COLS, int LD, int NTHR>
+__device__ __forceinline__ void load_tile(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
+    constexpr int W = COLS / 8;
+#pragma unroll
+    for (int i = tid; i < C * W; i += NTHR) {
+        const int r = i / W, c = i % W * 8;
+        const bool in = r < rows;
+        cp_async16_z(dst + r * LD + c, src + (in ? r * stride + c : 0), in);
+    }
+}
+template <int COLS, int LD, int NTHR>
+__device__ __forceinline__ void load_tile(bf16* dst, const float* src, size_t stride, int rows, int tid) {
+    constexpr int W = COLS / 4;
+#pragma unroll 4
+    for (int i = tid; i < C * W; i += NTHR) {
+        const int r = i / W, c = i % W * 4;
+        const float4 x = r < rows ? *reinterpret_cast<const float4*>(src + r * stride + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        put4<3>(dst, C * LD, r * LD + c, x);
+    }
+}
+// `count` 16-byte words
+template <int NTHR>
+__device__ __forceinline__ void load_words(bf16* dst, const bf16* src, int count, int tid) {
+    for (int i = tid; i < count; i += NTHR) cp_async16_z(dst + 8 * i, src + 8 * i, true);
+}
+
+__device__ __forceinline__ float2 load2(const float* p) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 load2(const bf16* p) {
+    const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ void store2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
+__device__ __forceinline__ void store2(bf16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
+
+__device__ __forceinline__ float load_g(const KdaGdrParams& p, const void* x, size_t i) {
+    return p.g_dtype == KDA_DTYPE_F32 ? static_cast<const float*>(x)[i] : __bfloat162float(static_cast<const bf16*>(x)[i]);
+}
+__device__ __forceinline__ void store_g(const KdaGdrParams& p, void* x, size_t i, float v) {
+    if (p.g_dtype == KDA_DTYPE_F32) static_cast<float*>(x)[i] = v;
+    else static_cast<bf16*>(x)[i] = __float2bfloat16_rn(v);
+}
+// log decay of a token (a NaN stays one)
+__device__ __forceinline__ float log_decay(const KdaGdrParams& p, size_t i, int h) {
+    float g = load_g(p, p.g, i);
+    if (p.flags & KDA_FLAG_GATE) g = -expf(p.A_log[h]) * softplus_f(g + (p.dt_bias ? p.dt_bias[h] : 0.f));
+    return g < G_MIN ? G_MIN : g;
+}
+// the three index tables take the same fields as KdaParams
+__device__ __forceinline__ size_t state_at(const KdaGdrParams& p, int d, int e) {
+    return (p.flags & KDA_FLAG_STATE_V_FIRST) ? (size_t)e * p.dk + d : (size_t)d * p.dv + e;
+}
+
+}  // namespace gdr
+}  // namespace kda

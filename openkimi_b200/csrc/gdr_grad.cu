@@ -1,0 +1,477 @@
+// Gated delta rule, backward: the gradients of a chunk once the state S0 at its start and the gradient dS at its end are known.
+//
+//   F = do S0^T, E = Y S0^T, H = V' dS^T;   dA = do V'^T (i >= j),  dL = -Y V'^T (i > j)
+//   Z = scale dA D / (|q_i| |k_j|),  X = dL beta_i D / (|k_i| |k_j|)
+//   dq = scale e^G / |q| F + Z k          dk = -e^G beta / |k| E + e^(G_last - G) / |k| H + X k + X^T k + Z^T q
+// and, with L2 norm, dq -= q (q . dq) / |q|^2, the same for k.  (Everything is in units of the rows as they arrive.)
+//   dbeta = Y . v - e^G k^ . E + rows of dL KKD
+//   dG = rows - columns of N + q^ . (scale e^G F) - e^G beta k^ . E - e^(G_last-G) k^ . H,   N = dA A + dL beta KKD below the diagonal
+//   dG_last += e^G_last <S0, dS> + sum e^(G_last-G) k^ . H,    dg = reverse cumulative sum of dG
+// The diagonal of A does not depend on G: left out of N, where its share of rows and columns would cancel (kept, it costs a factor
+// 20 of dg's precision at decays of e^-4 a token).
+//
+// One CTA of eight warps per (chunk, value head): warp w has rows 16 (w mod 4).. and half w / 4 of the columns of every product.
+// The value columns come in panels of 32, as three BF16 parts each of S0, dS, Y, V'.
+#include "gdr.cuh"
+
+namespace kda {
+namespace gdr {
+
+namespace gr {
+constexpr int NTHR = 256, EP = 32, LDE = EP + 8, PAN = C * LDE, LDZ = C + 8;
+}
+
+template <typename T, int K>
+struct GradMap {
+    static constexpr int P = In<T>::P, PO = In<T>::PO, LDK = K + 8, ROWS = C * LDK;
+    static constexpr int Q = 0, KK = P * ROWS, DO = 2 * P * ROWS, Y = DO + P * gr::PAN, V = Y + 3 * gr::PAN, S0 = V + 3 * gr::PAN,
+                         DS = S0 + 3 * K * gr::LDE, END = DS + 3 * K * gr::LDE;
+    static constexpr int Z = DO, X = Z + PO * C * gr::LDZ;  // over the panels, once they have been used
+    static_assert(X + PO * C * gr::LDZ <= END, "Z and X fit");
+    static constexpr int FLOATS = 7 * C + 16 * C;            // rows' numbers; sums over rows and columns
+    static constexpr int BYTES = 2 * END + FLOATS * 4;
+};
+
+template <typename T, int K>
+__global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, const Layout lay) {
+    using namespace gr;
+    using M = GradMap<T, K>;
+    constexpr int P = M::P, PO = M::PO, LDK = M::LDK, NK = K / 16;  // NK column tiles of a warp's half of K
+    extern __shared__ __align__(16) unsigned char smem[];
+    bf16* sm = reinterpret_cast<bf16*>(smem);
+    const uint32_t sa = smem_u32(sm);
+    float* sx = reinterpret_cast<float*>(smem + 2 * M::END);
+    float *gam = sx, *fall = sx + C, *be = sx + 2 * C, *rq = sx + 3 * C, *rk = sx + 4 * C, *ghi = sx + 5 * C, *glo = sx + 6 * C;
+    float* red = sx + 7 * C;   // [16][C]: row sums N (2 halves), dL KKD (2), q.F (2), k.E (2), k.H (2), Y.v (1), column sums (4), spare
+    enum { R_N = 0, R_B = 2, R_F = 4, R_E = 6, R_H = 8, R_Y = 10, R_COL = 11, R_X = 15 };
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3, rb = w & 3, half = w >> 2;
+    const int c = blockIdx.x / p.HV, h = blockIdx.x % p.HV, grp = p.HV / p.H, kh = h / grp;
+    const size_t unit = blockIdx.x;
+    pdl_wait();
+    const ChunkInfo ci = chunk_info(p, c);
+    const char* ws = static_cast<const char*>(p.workspace);
+    const char* sc = static_cast<const char*>(p.bwd_scratch);
+    const size_t qrow = (size_t)ci.tok0 * p.H + kh, vrow = (size_t)ci.tok0 * p.HV + h;
+    load_tile<K, LDK, NTHR>(sm + M::Q, static_cast<const T*>(p.q) + qrow * K, (size_t)p.H * K, ci.len, tid);
+    load_tile<K, LDK, NTHR>(sm + M::KK, static_cast<const T*>(p.k) + qrow * K, (size_t)p.H * K, ci.len, tid);
+    cp_async_commit();
+    const float* aux = reinterpret_cast<const float*>(ws + lay.aux) + unit * AUX;
+    for (int i = tid; i < 7 * C; i += NTHR) sx[i] = aux[i];
+    const float last = aux[A_LAST * C];
+
+    float F[NK][4], E[NK][4], H[NK][4], dA[4][4], dL[4][4];
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) F[j][i] = E[j][i] = H[j][i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dA[j][i] = dL[j][i] = 0.f;
+    float ss = 0.f, yv[2] = {0.f, 0.f};
+    const float* gY = reinterpret_cast<const float*>(sc + lay.Y) + unit * C * p.dv;
+    const float* gV = reinterpret_cast<const float*>(ws + lay.Vn) + unit * C * p.dv;
+    const float* gS = reinterpret_cast<const float*>(ws + lay.S0) + unit * K * p.dv;
+    const float* gD = reinterpret_cast<const float*>(sc + lay.dS) + unit * K * p.dv;
+    const int pr = tid >> 3, pc = (tid & 7) * 4;  // this thread's rows pr, pr + 32, .. and columns of a panel
+#pragma unroll 1
+    for (int e0 = 0; e0 < p.dv; e0 += EP) {
+        if (e0) __syncthreads();
+        load_tile<EP, LDE, NTHR>(sm + M::DO, static_cast<const T*>(p.grad_o) + vrow * p.dv + e0, (size_t)p.HV * p.dv, ci.len, tid);
+        cp_async_commit();
+        float4 ry[2], rv[2], rs[K / 32], rd[K / 32];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ry[i] = *reinterpret_cast<const float4*>(gY + (size_t)(pr + 32 * i) * p.dv + e0 + pc);
+            rv[i] = *reinterpret_cast<const float4*>(gV + (size_t)(pr + 32 * i) * p.dv + e0 + pc);
+        }
+#pragma unroll
+        for (int i = 0; i < K / 32; ++i) {
+            rs[i] = *reinterpret_cast<const float4*>(gS + (size_t)(pr + 32 * i) * p.dv + e0 + pc);
+            rd[i] = *reinterpret_cast<const float4*>(gD + (size_t)(pr + 32 * i) * p.dv + e0 + pc);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (pr + 32 * i < ci.len) {
+                const T* v = static_cast<const T*>(p.v) + (vrow + (size_t)(pr + 32 * i) * p.HV) * p.dv + e0 + pc;
+                const float2 a = load2(v), b = load2(v + 2);
+                yv[i] += ry[i].x * a.x + ry[i].y * a.y + ry[i].z * b.x + ry[i].w * b.y;
+            }
+            put4<3>(sm + M::Y, PAN, (pr + 32 * i) * LDE + pc, ry[i]);
+            put4<3>(sm + M::V, PAN, (pr + 32 * i) * LDE + pc, rv[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < K / 32; ++i) {
+            ss += rs[i].x * rd[i].x + rs[i].y * rd[i].y + rs[i].z * rd[i].z + rs[i].w * rd[i].w;
+            put4<3>(sm + M::S0, K * LDE, (pr + 32 * i) * LDE + pc, rs[i]);
+            put4<3>(sm + M::DS, K * LDE, (pr + 32 * i) * LDE + pc, rd[i]);
+        }
+        cp_async_wait<0>();
+        __syncthreads();
+#pragma unroll 1
+        for (int e = 0; e < EP; e += 16) {
+            uint32_t fo[P][4], fy[3][4], fv[3][4];
+#pragma unroll
+            for (int i = 0; i < P; ++i) a_frag<LDE>(fo[i], sa + 2 * (M::DO + i * PAN), 16 * rb, e, lane);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) {
+                a_frag<LDE>(fy[i], sa + 2 * (M::Y + i * PAN), 16 * rb, e, lane);
+                a_frag<LDE>(fv[i], sa + 2 * (M::V + i * PAN), 16 * rb, e, lane);
+            }
+#pragma unroll
+            for (int j = 0; j < NK / 2; ++j) {
+                uint32_t b[3][4];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) b_frag<LDE>(b[i], sa + 2 * (M::S0 + i * K * LDE), half * (K / 2) + 16 * j, e, lane);
+                mma_parts<P, 3, 3>(F, j, fo, b);
+                mma_parts<3, 3, 3>(E, j, fy, b);
+#pragma unroll
+                for (int i = 0; i < 3; ++i) b_frag<LDE>(b[i], sa + 2 * (M::DS + i * K * LDE), half * (K / 2) + 16 * j, e, lane);
+                mma_parts<3, 3, 3>(H, j, fv, b);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                if (2 * half + j > rb) break;
+                uint32_t b[3][4];
+#pragma unroll
+                for (int i = 0; i < 3; ++i) b_frag<LDE>(b[i], sa + 2 * (M::V + i * PAN), 32 * half + 16 * j, e, lane);
+                mma_parts<P, 3, 3>(dA, j, fo, b);
+                mma_parts<3, 3, 3>(dL, j, fy, b);
+            }
+        }
+    }
+    // q k^T, k k^T again
+    float qk[4][4], kk[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) qk[j][i] = kk[j][i] = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < K; d += 16) {
+        uint32_t fq[P][4], fk[P][4];
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            a_frag<LDK>(fq[i], sa + 2 * (M::Q + i * M::ROWS), 16 * rb, d, lane);
+            a_frag<LDK>(fk[i], sa + 2 * (M::KK + i * M::ROWS), 16 * rb, d, lane);
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            if (2 * half + j > rb) break;
+            uint32_t b[P][4];
+#pragma unroll
+            for (int i = 0; i < P; ++i) b_frag<LDK>(b[i], sa + 2 * (M::KK + i * M::ROWS), 32 * half + 16 * j, d, lane);
+            mma_parts<P, P, P>(qk, j, fq, b);
+            mma_parts<P, P, P>(kk, j, fk, b);
+        }
+    }
+    // Y . v: eight lanes have a row
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) yv[i] += __shfl_xor_sync(0xffffffffu, yv[i], o);
+        if ((tid & 7) == 0) red[R_Y * C + pr + 32 * i] = yv[i];
+    }
+    ss = warp_sum(ss);
+    if (lane == 0) red[R_X * C + w] = ss;
+    __syncthreads();  // the panels have been used
+    const int r0 = 16 * rb + g;
+    float rn[2] = {0.f, 0.f}, rbeta[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        if (2 * half + j / 2 > rb) break;
+        float col[2] = {0.f, 0.f};
+        const int j0 = 32 * half + 8 * j + 2 * t;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 8 * i;
+            float z[2], x[2];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int cc = j0 + y;
+                const float d = r >= cc ? expf(ghi[r] - ghi[cc] + (glo[r] - glo[cc])) : 0.f;
+                const float a = r >= cc ? dA[j][2 * i + y] * p.scale * d * rq[r] * rk[cc] : 0.f;
+                const float kkd = rk[r] * rk[cc] * d, l = r > cc ? -dL[j][2 * i + y] * kkd : 0.f;
+                z[y] = a;
+                x[y] = l * be[r];
+                const float lk = l * kk[j][2 * i + y];
+                const float nn = r > cc ? fmaf(a, qk[j][2 * i + y], be[r] * lk) : 0.f;
+                rn[i] += nn;
+                rbeta[i] += r > cc ? lk : 0.f;
+                col[y] += nn;
+            }
+            put<PO>(sm + M::Z, C * LDZ, r * LDZ + j0, z[0], z[1]);
+            put<PO>(sm + M::X, C * LDZ, r * LDZ + j0, x[0], x[1]);
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) col[y] += __shfl_xor_sync(0xffffffffu, col[y], o);
+            if (g == 0) red[(R_COL + rb) * C + j0 + y] = col[y];
+        }
+    }
+    // this half's share of the row sums; scale the products with the states to the rows' units
+    float rf[2] = {0.f, 0.f}, re[2] = {0.f, 0.f}, rh[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < NK; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 8 * i, d = half * (K / 2) + 8 * j + 2 * t;
+            const float2 q = get2<P>(sm + M::Q, M::ROWS, r * LDK + d), k = get2<P>(sm + M::KK, M::ROWS, r * LDK + d);
+            const float ff = p.scale * gam[r] * rq[r], fe = gam[r] * rk[r], fh = fall[r] * rk[r];
+            float &f0 = F[j][2 * i], &f1 = F[j][2 * i + 1];
+            f0 *= ff; f1 *= ff;
+            const float e0 = E[j][2 * i] * fe, e1 = E[j][2 * i + 1] * fe, h0 = H[j][2 * i] * fh, h1 = H[j][2 * i + 1] * fh;
+            rf[i] += q.x * f0 + q.y * f1;
+            re[i] += k.x * e0 + k.y * e1;
+            rh[i] += k.x * h0 + k.y * h1;
+            E[j][2 * i] = h0 - be[r] * e0;
+            E[j][2 * i + 1] = h1 - be[r] * e1;
+        }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            rn[i] += __shfl_xor_sync(0xffffffffu, rn[i], o);
+            rbeta[i] += __shfl_xor_sync(0xffffffffu, rbeta[i], o);
+            rf[i] += __shfl_xor_sync(0xffffffffu, rf[i], o);
+            re[i] += __shfl_xor_sync(0xffffffffu, re[i], o);
+            rh[i] += __shfl_xor_sync(0xffffffffu, rh[i], o);
+        }
+        if (t == 0) {
+            const int r = r0 + 8 * i;
+            red[(R_N + half) * C + r] = rn[i];
+            red[(R_B + half) * C + r] = rbeta[i];
+            red[(R_F + half) * C + r] = rf[i];
+            red[(R_E + half) * C + r] = re[i];
+            red[(R_H + half) * C + r] = rh[i];
+        }
+    }
+    __syncthreads();  // Z, X and the sums are there
+    // dq (in F) and dk (in E) of 16 rows and this half of the channels
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+        uint32_t fz[PO][4], fx[PO][4], zt[PO][4], xt[PO][4];
+#pragma unroll
+        for (int i = 0; i < PO; ++i) {
+            if (b <= rb) {
+                a_frag<LDZ>(fz[i], sa + 2 * (M::Z + i * C * LDZ), 16 * rb, 16 * b, lane);
+                a_frag<LDZ>(fx[i], sa + 2 * (M::X + i * C * LDZ), 16 * rb, 16 * b, lane);
+            }
+            if (b >= rb) {
+                a_frag_t<LDZ>(zt[i], sa + 2 * (M::Z + i * C * LDZ), 16 * rb, 16 * b, lane);
+                a_frag_t<LDZ>(xt[i], sa + 2 * (M::X + i * C * LDZ), 16 * rb, 16 * b, lane);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NK / 2; ++j) {
+            uint32_t bk[P][4], bq[P][4];
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                b_frag_t<LDK>(bk[i], sa + 2 * (M::KK + i * M::ROWS), half * (K / 2) + 16 * j, 16 * b, lane);
+                b_frag_t<LDK>(bq[i], sa + 2 * (M::Q + i * M::ROWS), half * (K / 2) + 16 * j, 16 * b, lane);
+            }
+            if (b <= rb) {
+                mma_parts<PO, P, PO>(F, j, fz, bk);
+                mma_parts<PO, P, PO>(E, j, fx, bk);
+            }
+            if (b >= rb) {
+                mma_parts<PO, P, PO>(E, j, xt, bk);
+                mma_parts<PO, P, PO>(E, j, zt, bq);
+            }
+        }
+    }
+    if (w == 0) {  // the gate's and beta's gradients, two neighbouring rows per lane
+        float total = 0.f;
+        for (int i = 0; i < 8; ++i) total += red[R_X * C + i];
+        double dG[2], hsum = 0.0;
+        float db[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * lane + i, I = r >> 4;
+            float colsum = 0.f;
+            for (int x = I; x < 4; ++x) colsum += red[(R_COL + x) * C + r];
+            const float n = red[R_N * C + r] + red[(R_N + 1) * C + r], bb = red[R_B * C + r] + red[(R_B + 1) * C + r];
+            const float f = red[R_F * C + r] + red[(R_F + 1) * C + r], e = red[R_E * C + r] + red[(R_E + 1) * C + r],
+                        hh = red[R_H * C + r] + red[(R_H + 1) * C + r];
+            dG[i] = (double)n - colsum + f - (double)be[r] * e - hh;
+            hsum += hh;
+            db[i] = red[R_Y * C + r] - e + bb;
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
+        double run = dG[0] + dG[1];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const double dn = __shfl_down_sync(0xffffffffu, run, o);
+            if (lane + o < 32) run += dn;
+        }
+        run += (double)last * total + hsum;
+        const double dg[2] = {run, run - dG[0]};
+        float dAl = 0.f, dbi = 0.f;
+        const float eA = (p.flags & KDA_FLAG_GATE) ? expf(p.A_log[h]) : 0.f, bias = (p.flags & KDA_FLAG_GATE) && p.dt_bias ? p.dt_bias[h] : 0.f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = 2 * lane + i;
+            if (r < ci.len) {
+                const size_t at = (size_t)(ci.tok0 + r) * p.HV + h;
+                float d = (float)dg[i], b = db[i];
+                if (p.flags & KDA_FLAG_GATE) {
+                    const float a = load_g(p, p.g, at) + bias, sp = softplus_f(a);
+                    dAl += d * fmaxf(-eA * sp, G_MIN);
+                    d *= -eA * (a > 20.f ? 1.f : sigmoid_f(a));
+                    dbi += d;
+                }
+                if (p.flags & KDA_FLAG_BETA_SIGMOID) b *= be[r] * (1.f - be[r]);
+                store_g(p, p.grad_g, at, d);
+                store_g(p, p.grad_beta, at, b);
+            }
+        }
+        if (p.flags & KDA_FLAG_GATE) {
+            dAl = warp_sum(dAl);
+            dbi = warp_sum(dbi);
+            if (lane == 0) *reinterpret_cast<float2*>(static_cast<char*>(p.bwd_scratch) + lay.part + unit * 8) = make_float2(dAl, dbi);
+        }
+    }
+    if (grp > 1) {  // the group's value heads are added up by gdr_heads_kernel
+        float* out = reinterpret_cast<float*>(static_cast<char*>(p.bwd_scratch) + lay.dqk) + unit * 2 * C * K;
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = (r0 + 8 * i) * K + half * (K / 2) + 8 * j + 2 * t;
+                store2(out + at, F[j][2 * i], F[j][2 * i + 1]);
+                store2(out + C * K + at, E[j][2 * i], E[j][2 * i + 1]);
+            }
+        return;
+    }
+    float dot[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+    if (p.flags & KDA_FLAG_QK_L2NORM) {
+#pragma unroll
+        for (int j = 0; j < NK; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int at = (r0 + 8 * i) * LDK + half * (K / 2) + 8 * j + 2 * t;
+                const float2 q = get2<P>(sm + M::Q, M::ROWS, at), k = get2<P>(sm + M::KK, M::ROWS, at);
+                dot[0][i] += q.x * F[j][2 * i] + q.y * F[j][2 * i + 1];
+                dot[1][i] += k.x * E[j][2 * i] + k.y * E[j][2 * i + 1];
+            }
+        __syncthreads();  // (the sums above have been read)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) dot[x][i] += __shfl_xor_sync(0xffffffffu, dot[x][i], o);
+                if (t == 0) red[(2 * x + half) * C + r0 + 8 * i] = dot[x][i];
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = r0 + 8 * i;
+            // a row shorter than 1e-6 is divided by that, whatever its length
+            dot[0][i] = rq[r] < 1e6f ? rq[r] * rq[r] * (red[r] + red[C + r]) : 0.f;
+            dot[1][i] = rk[r] < 1e6f ? rk[r] * rk[r] * (red[2 * C + r] + red[3 * C + r]) : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = r0 + 8 * i;
+        if (r >= ci.len) continue;
+#pragma unroll
+        for (int j = 0; j < NK; ++j) {
+            const int d = half * (K / 2) + 8 * j + 2 * t;
+            const float2 q = get2<P>(sm + M::Q, M::ROWS, r * LDK + d), k = get2<P>(sm + M::KK, M::ROWS, r * LDK + d);
+            const size_t at = (qrow + (size_t)r * p.H) * K + d;
+            store2(static_cast<T*>(p.grad_q) + at, F[j][2 * i] - q.x * dot[0][i], F[j][2 * i + 1] - q.y * dot[0][i]);
+            store2(static_cast<T*>(p.grad_k) + at, E[j][2 * i] - k.x * dot[1][i], E[j][2 * i + 1] - k.y * dot[1][i]);
+        }
+    }
+}
+
+// dq and dk of shared key heads: the shares of a group's value heads in their order, then the gradient of the L2 norm.  A warp per
+// (row, key head).
+template <typename T, int K>
+__global__ void __launch_bounds__(256) gdr_heads_kernel(const KdaGdrParams p, const Layout lay) {
+    constexpr int N = K / 32;
+    const int lane = threadIdx.x & 31, grp = p.HV / p.H;
+    const int c = blockIdx.x / p.H, kh = blockIdx.x % p.H;
+    pdl_wait();
+    const ChunkInfo ci = chunk_info(p, c);
+    const float* aux = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + lay.aux) + ((size_t)c * p.HV + kh * grp) * AUX;
+    const float* in = reinterpret_cast<const float*>(static_cast<const char*>(p.bwd_scratch) + lay.dqk) + ((size_t)c * p.HV + kh * grp) * 2 * C * K;
+    for (int x = threadIdx.x >> 5; x < 2 * ci.len; x += 8) {
+        const int r = x >> 1, which = x & 1;  // q, k
+        float s[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = 0.f;
+        for (int hg = 0; hg < grp; ++hg)
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float2 v = load2(in + ((size_t)hg * 2 + which) * C * K + r * K + N * lane + i);
+                s[i] += v.x; s[i + 1] += v.y;
+            }
+        const size_t at = (((size_t)ci.tok0 + r) * p.H + kh) * K + N * lane;
+        const T* row = static_cast<const T*>(which ? p.k : p.q) + at;
+        T* out = static_cast<T*>(which ? p.grad_k : p.grad_q) + at;
+        float xv[N], dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float2 v = load2(row + i);
+            xv[i] = v.x; xv[i + 1] = v.y;
+            dot += v.x * s[i] + v.y * s[i + 1];
+        }
+        float f = 0.f;
+        if (p.flags & KDA_FLAG_QK_L2NORM) {
+            const float inv = aux[(which ? A_RK : A_RQ) * C + r];
+            f = inv < 1e6f ? inv * inv * warp_sum(dot) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i += 2) store2(out + i, s[i] - xv[i] * f, s[i + 1] - xv[i + 1] * f);
+    }
+}
+
+// dA_log and ddt_bias: the units' shares of a value head, in a fixed order and in 64 bits
+__global__ void __launch_bounds__(256) gdr_param_kernel(const KdaGdrParams p, const Layout lay) {
+    __shared__ double s[2][256];
+    const int h = blockIdx.x;
+    pdl_wait();
+    const float2* part = reinterpret_cast<const float2*>(static_cast<const char*>(p.bwd_scratch) + lay.part);
+    double a = 0.0, b = 0.0;
+    for (int c = threadIdx.x; c < p.NT; c += 256) {
+        const float2 x = part[(size_t)c * p.HV + h];
+        a += x.x;
+        b += x.y;
+    }
+    s[0][threadIdx.x] = a;
+    s[1][threadIdx.x] = b;
+    for (int o = 128; o > 0; o >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < o) {
+            s[0][threadIdx.x] += s[0][threadIdx.x + o];
+            s[1][threadIdx.x] += s[1][threadIdx.x + o];
+        }
+    }
+    if (threadIdx.x == 0) {
+        p.grad_A_log[h] = (float)s[0][0];
+        if (p.grad_dt_bias) p.grad_dt_bias[h] = (float)s[1][0];
+    }
+}
+
+template <typename T, int K>
+static cudaError_t launch_grad(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    constexpr int bytes = GradMap<T, K>::BYTES;
+    static_assert(bytes <= 232448, "shared memory");
+    cudaError_t e = allow_smem(gdr_grad_kernel<T, K>, bytes);
+    if (e == cudaSuccess) e = launch_dependent(gdr_grad_kernel<T, K>, p.NT * p.HV, gr::NTHR, bytes, s, p, l);
+    if (e == cudaSuccess && p.HV != p.H) e = launch_dependent(gdr_heads_kernel<T, K>, p.NT * p.H, 256, 0, s, p, l);
+    if (e == cudaSuccess && (p.flags & KDA_FLAG_GATE)) e = launch_dependent(gdr_param_kernel, p.HV, 256, 0, s, p, l);
+    return e;
+}
+
+cudaError_t grad(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    if (p.dtype == KDA_DTYPE_F32) return p.dk == 64 ? launch_grad<float, 64>(p, l, s) : launch_grad<float, 128>(p, l, s);
+    return p.dk == 64 ? launch_grad<bf16, 64>(p, l, s) : launch_grad<bf16, 128>(p, l, s);
+}
+
+}  // namespace gdr
+}  // namespace kda

@@ -1,0 +1,548 @@
+// Group normalisation with an activation over channels-last activations x [N, S, Ch]:
+//
+//   z = (x - mean) rstd w + b,  y = z or z sigmoid(z),  mean and variance over the S positions and Ch / G channels of (n, group)
+//   dz = dy act'(z);  dw_c = sum dz x^,  db_c = sum dz,  dx = rstd (dz w - m1 - x^ m2),  m1 = mean(dz w), m2 = mean(dz w x^)
+//
+// HBM-bound: forward one read and one write, backward two reads and one write per value.
+//   * S = 1 (every token by itself, groups of up to 1024 channels): L lanes hold a group of one row in registers, so that one pass
+//     does it all; the lanes keep their group over the rows they walk and with it w, b and their shares of dw, db.
+//   * else: a thread keeps VEC channels and walks rows of a slice of a sample.  Forward: sums of x and x^2 about the slice's first
+//     row, joined over slices and channels as (count, mean, sum of squared deviations), then a second pass that applies.  Backward:
+//     per sample and channel the sums of dz and dz x^, which give dw, db and, weighted with w, m1 and m2; then dx.  The second pass
+//     reads from L2 what fits there.
+// Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
+#include "kda_common.cuh"
+
+namespace kda {
+namespace gn {
+
+using bf16 = __nv_bfloat16;
+constexpr int NTHR = 256;
+constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
+constexpr int MAX_SLICES = 256;
+
+struct Args {
+    const void *x, *dy;
+    void *y, *dx;
+    const float *w, *b;           // may be NULL: 1, 0
+    float *mean, *rstd;           // [N, G]
+    float *dw, *db;               // [Ch], may be NULL
+    float* part;                  // scratch
+    long long N, S;
+    int Ch, G, act, slices;
+    float eps;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
+    if constexpr (sizeof(T) * VEC == 16) {
+        const uint4 r = *reinterpret_cast<const uint4*>(p);
+        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                v[i] = __uint_as_float(u[i]);
+            } else {
+                v[2 * i] = __uint_as_float(u[i] << 16);
+                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[i] = ldf(p + i);
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
+    if constexpr (sizeof(T) * VEC == 16) {
+        uint32_t u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if constexpr (sizeof(T) == 4) {
+                u[i] = __float_as_uint(v[i]);
+            } else {
+                const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                u[i] = *reinterpret_cast<const uint32_t*>(&h);
+            }
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) stf(p + i, v[i]);
+    }
+}
+
+// FP32 values go through expf, BF16 ones through the hardware's 2^x (2 ulp, and |z| 2^-24 from its argument)
+template <typename T>
+__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + (sizeof(T) == 4 ? expf(-z) : __expf(-z))); }
+template <typename T>
+__device__ __forceinline__ float act(float z, bool silu) { return silu ? z * sigmoid<T>(z) : z; }
+// dy act'(z)
+template <typename T>
+__device__ __forceinline__ float act_grad(float z, float dy, bool silu) {
+    if (!silu) return dy;
+    const float s = sigmoid<T>(z);
+    return dy * s * fmaf(z, 1.f - s, 1.f);
+}
+__device__ __forceinline__ float lanes_sum(float v, int L) {
+    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// ---- one row at a time ------------------------------------------------------------------------------------------------
+// Slots of L lanes; slot s has group s mod G and rows s / G, s / G + step, ...  Every lane of a warp makes the same number of turns.
+template <typename T, int VEC, int NV, bool BWD>
+__global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int L) {
+    const int lane = threadIdx.x & (L - 1), Cg = a.Ch / a.G;
+    const long long slot = ((long long)blockIdx.x * NTHR + threadIdx.x) / L, slots = (long long)gridDim.x * NTHR / L;
+    const long long step = slots / a.G;            // rows between a slot's rows; slots beyond step * G have none
+    const bool idle = slot >= step * a.G;
+    const int g = (int)(slot % a.G), c0 = g * Cg;
+    const float inv = 1.f / Cg;
+    const bool silu = a.act;
+    pdl_wait();
+    const T* X = static_cast<const T*>(a.x);
+    float w[NV][VEC], b[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int c = (j * L + lane) * VEC + i;
+            const bool in = c < Cg;
+            w[j][i] = in && a.w ? a.w[c0 + c] : 1.f;
+            b[j][i] = in && a.b ? a.b[c0 + c] : 0.f;
+            dw[j][i] = db[j][i] = 0.f;
+        }
+    const long long turns = (a.N + step - 1) / step;
+    for (long long k = 0; k < turns; ++k) {
+        const long long n = slot / a.G + k * step;
+        const bool on = !idle && n < a.N;
+        const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
+        float x[NV][VEC], s = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * L + lane) * VEC;
+            if (on && c < Cg) load<T, VEC>(X + base + c, x[j]);
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) x[j][i] = 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) s += x[j][i];
+        }
+        float dy[NV][VEC];
+        if (BWD) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * L + lane) * VEC;
+                if (on && c < Cg) load<T, VEC>(static_cast<const T*>(a.dy) + base + c, dy[j]);
+                else
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) dy[j][i] = 0.f;
+            }
+        }
+        const float mean = lanes_sum(s, L) * inv;
+        float q = 0.f;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                x[j][i] = (j * L + lane) * VEC < Cg ? x[j][i] - mean : 0.f;
+                q = fmaf(x[j][i], x[j][i], q);
+            }
+        const float rstd = 1.f / sqrtf(lanes_sum(q, L) * inv + a.eps);
+        if (!BWD) {
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * L + lane) * VEC;
+                float y[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) y[i] = act<T>(fmaf(x[j][i] * rstd, w[j][i], b[j][i]), silu);
+                if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.y) + base + c, y);
+            }
+        } else {
+            float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int j = 0; j < NV; ++j)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    x[j][i] *= rstd;
+                    const float dz = act_grad<T>(fmaf(x[j][i], w[j][i], b[j][i]), dy[j][i], silu);
+                    db[j][i] += dz;
+                    dw[j][i] = fmaf(dz, x[j][i], dw[j][i]);
+                    dy[j][i] = dz * w[j][i];
+                    m1 += dy[j][i];
+                    m2 = fmaf(dy[j][i], x[j][i], m2);
+                }
+            m1 = lanes_sum(m1, L) * inv;
+            m2 = lanes_sum(m2, L) * inv;
+#pragma unroll
+            for (int j = 0; j < NV; ++j) {
+                const int c = (j * L + lane) * VEC;
+                float dx[VEC];
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) dx[i] = rstd * (dy[j][i] - m1 - x[j][i] * m2);
+                if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.dx) + base + c, dx);
+            }
+        }
+    }
+    if (BWD && a.dw && !idle) {  // part[step][2][Ch]
+        float* out = a.part + (size_t)(slot / a.G) * 2 * a.Ch + c0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const int c = (j * L + lane) * VEC + i;
+                if (c < Cg) {
+                    out[c] = dw[j][i];
+                    out[a.Ch + c] = db[j][i];
+                }
+            }
+    }
+}
+
+// dw, db: sums of part[count][2][Ch] over count, 32 channels a CTA
+__global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* part, long long count, int Ch, float* dw, float* db) {
+    __shared__ double s[32][33];
+    const int c = blockIdx.x * 32 + threadIdx.x, which = blockIdx.y;
+    pdl_wait();
+    double v = 0.0;
+    if (c < Ch)
+        for (long long i = threadIdx.y; i < count; i += 32) v += part[(i * 2 + which) * Ch + c];
+    s[threadIdx.y][threadIdx.x] = v;
+    __syncthreads();
+    if (threadIdx.y == 0 && c < Ch) {
+        for (int i = 1; i < 32; ++i) v += s[i][threadIdx.x];
+        (which ? db : dw)[c] = (float)v;
+    }
+}
+
+// ---- samples of several positions -------------------------------------------------------------------------------------
+// A CTA has one slice of one sample; thread = (row of TR, VEC channels), channels in blocks of NTHR * VEC where a row is wider than
+// the CTA.
+struct Slice {
+    long long n, s0, s1;
+    __device__ __forceinline__ Slice(const Args& a) {
+        n = blockIdx.x / a.slices;
+        const long long i = blockIdx.x % a.slices;
+        s0 = a.S * i / a.slices;
+        s1 = a.S * (i + 1) / a.slices;
+    }
+};
+
+// MODE 0: count-free sums of x - x0 and (x - x0)^2 about the slice's first row x0; 1: sums of dz x^ and dz
+template <typename T, int VEC, int MODE>
+__global__ void __launch_bounds__(NTHR) group_norm_sums_kernel(const Args a) {
+    extern __shared__ float sm[];                  // [2][TR][TC * VEC]
+    const int cols = a.Ch / VEC, TC = min(cols, NTHR), TR = NTHR / TC;
+    const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
+    const Slice sl(a);
+    const long long n = sl.n;
+    pdl_wait();
+    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
+    const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
+    float* out = a.part + (size_t)blockIdx.x * 2 * a.Ch;
+    const bool silu = a.act;
+    for (int v0 = 0; v0 < cols; v0 += TC) {
+        const int v = v0 + tc, c = v * VEC;
+        const bool on = tr < TR && v < cols;
+        float p[VEC], q[VEC], s1[VEC], s2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.f;
+        if (on) {
+            if (MODE == 0) {
+                load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    p[i] = a.mean[n * a.G + (c + i) / Cg];
+                    q[i] = a.rstd[n * a.G + (c + i) / Cg];
+                }
+            }
+            float w[VEC], b[VEC];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                w[i] = MODE && a.w ? a.w[c + i] : 1.f;
+                b[i] = MODE && a.b ? a.b[c + i] : 0.f;
+            }
+#pragma unroll 4
+            for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
+                float x[VEC];
+                load<T, VEC>(X + (size_t)s * a.Ch + c, x);
+                if (MODE == 0) {
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float d = x[i] - p[i];
+                        s1[i] += d;
+                        s2[i] = fmaf(d, d, s2[i]);
+                    }
+                } else {
+                    float dy[VEC];
+                    load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i) {
+                        const float xh = (x[i] - p[i]) * q[i], dz = act_grad<T>(fmaf(xh, w[i], b[i]), dy[i], silu);
+                        s1[i] = fmaf(dz, xh, s1[i]);
+                        s2[i] += dz;
+                    }
+                }
+            }
+        }
+        if (v0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (tr < TR) {
+                sm[tr * TC * VEC + tc * VEC + i] = s1[i];
+                sm[(TR + tr) * TC * VEC + tc * VEC + i] = s2[i];
+            }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 2 * TC * VEC; i += NTHR) {
+            const int which = i / (TC * VEC), cc = i % (TC * VEC);
+            if (v0 * VEC + cc >= a.Ch) continue;
+            float s = 0.f;
+            for (int r = 0; r < TR; ++r) s += sm[(which * TR + r) * TC * VEC + cc];
+            out[(size_t)which * a.Ch + v0 * VEC + cc] = s;
+        }
+    }
+}
+
+// mean and rstd of (sample, group) from the slices' sums: two passes over slices and channels, in 64 bits (channels and slices are
+// few).  A CTA per (group, sample).
+template <typename T>
+__global__ void __launch_bounds__(128) group_norm_stats_kernel(const Args a) {
+    __shared__ double s[128];
+    const int Cg = a.Ch / a.G, g = blockIdx.x % a.G;
+    const long long n = blockIdx.x / a.G;
+    pdl_wait();
+    const float* part = a.part + (size_t)n * a.slices * 2 * a.Ch;
+    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
+    auto sum = [&](double v) {
+        s[threadIdx.x] = v;
+        for (int o = 64; o > 0; o >>= 1) {
+            __syncthreads();
+            if (threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
+        }
+        __syncthreads();
+        const double r = s[0];
+        __syncthreads();
+        return r;
+    };
+    auto each = [&](auto f) {
+        double v = 0.0;
+        for (int i = threadIdx.x; i < a.slices * Cg; i += 128) {
+            const int sl = i / Cg, c = g * Cg + i % Cg;
+            const long long s0 = a.S * sl / a.slices, s1 = a.S * (sl + 1) / a.slices;
+            v += f((double)(s1 - s0), (double)ldf(X + (size_t)s0 * a.Ch + c), (double)part[(size_t)sl * 2 * a.Ch + c],
+                   (double)part[((size_t)sl * 2 + 1) * a.Ch + c]);
+        }
+        return sum(v);
+    };
+    const double count = (double)a.S * Cg;
+    const double mean = each([](double m, double x0, double d1, double) { return m * x0 + d1; }) / count;
+    // sum (x - mean)^2 = sum (x - x0)^2 + 2 (x0 - mean) sum (x - x0) + m (x0 - mean)^2
+    const double var = each([mean](double m, double x0, double d1, double d2) { return d2 + (x0 - mean) * (2.0 * d1 + m * (x0 - mean)); }) / count;
+    if (threadIdx.x == 0) {
+        a.mean[n * a.G + g] = (float)mean;
+        a.rstd[n * a.G + g] = (float)(1.0 / sqrt((var > 0.0 || !(var <= 0.0) ? var : 0.0) + (double)a.eps));
+    }
+}
+
+// m1, m2 of (sample, group) from the sums over its slices, [N, G, 2] behind them
+__global__ void __launch_bounds__(128) group_norm_means_kernel(const Args a) {
+    __shared__ double s[2][128];
+    const int Cg = a.Ch / a.G, g = blockIdx.x % a.G;
+    const long long n = blockIdx.x / a.G;
+    pdl_wait();
+    const float* part = a.part + (size_t)n * a.slices * 2 * a.Ch;
+    double m1 = 0.0, m2 = 0.0;
+    for (int i = threadIdx.x; i < a.slices * Cg; i += 128) {
+        const int sl = i / Cg, c = g * Cg + i % Cg;
+        const double w = a.w ? a.w[c] : 1.f;
+        m2 += w * part[(size_t)sl * 2 * a.Ch + c];
+        m1 += w * part[((size_t)sl * 2 + 1) * a.Ch + c];
+    }
+    s[0][threadIdx.x] = m1;
+    s[1][threadIdx.x] = m2;
+    for (int o = 64; o > 0; o >>= 1) {
+        __syncthreads();
+        if (threadIdx.x < o) {
+            s[0][threadIdx.x] += s[0][threadIdx.x + o];
+            s[1][threadIdx.x] += s[1][threadIdx.x + o];
+        }
+    }
+    if (threadIdx.x == 0) {
+        const double count = (double)a.S * Cg;
+        float* out = a.part + (size_t)a.N * a.slices * 2 * a.Ch + (n * a.G + g) * 2;
+        out[0] = (float)(s[0][0] / count);
+        out[1] = (float)(s[1][0] / count);
+    }
+}
+
+template <typename T, int VEC, bool BWD>
+__global__ void __launch_bounds__(NTHR) group_norm_apply_kernel(const Args a) {
+    const int cols = a.Ch / VEC, TC = min(cols, NTHR), TR = NTHR / TC;
+    const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
+    const Slice sl(a);
+    const long long n = sl.n;
+    pdl_wait();
+    if (tr >= TR) return;
+    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
+    const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
+    T* Y = static_cast<T*>(BWD ? a.dx : a.y) + (size_t)n * a.S * a.Ch;
+    const float* m = a.part + (size_t)a.N * a.slices * 2 * a.Ch + n * a.G * 2;
+    const bool silu = a.act;
+    for (int v = tc; v < cols; v += TC) {
+        const int c = v * VEC;
+        float mu[VEC], rs[VEC], w[VEC], b[VEC], m1[VEC], m2[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int g = (c + i) / Cg;
+            mu[i] = a.mean[n * a.G + g];
+            rs[i] = a.rstd[n * a.G + g];
+            w[i] = a.w ? a.w[c + i] : 1.f;
+            b[i] = a.b ? a.b[c + i] : 0.f;
+            m1[i] = BWD ? m[2 * g] : 0.f;
+            m2[i] = BWD ? m[2 * g + 1] : 0.f;
+        }
+#pragma unroll 4
+        for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
+            float x[VEC], dy[VEC], y[VEC];
+            load<T, VEC>(X + (size_t)s * a.Ch + c, x);
+            if (BWD) load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                const float xh = (x[i] - mu[i]) * rs[i], z = fmaf(xh, w[i], b[i]);
+                y[i] = BWD ? rs[i] * (act_grad<T>(z, dy[i], silu) * w[i] - m1[i] - xh * m2[i]) : act<T>(z, silu);
+            }
+            store<T, VEC>(Y + (size_t)s * a.Ch + c, y);
+        }
+    }
+}
+
+// ---- launches -----------------------------------------------------------------------------------------------------------
+static bool by_rows(long long S, int Ch, int G) { return S == 1 && Ch / G <= ROWS_MAX; }
+
+// slices of a sample: about four CTAs per SM over all samples, of at least 16 rows
+static int slice_count(long long N, long long S) {
+    long long want = (4LL * sm_count() + N - 1) / N, most = (S + 15) / 16;
+    if (want > most) want = most;
+    return (int)(want < 1 ? 1 : want > MAX_SLICES ? MAX_SLICES : want);
+}
+
+struct RowsGrid { int L; long long ctas, step; };
+static RowsGrid rows_grid(long long N, int Ch, int G, int vec, bool bwd) {
+    const int Cg = Ch / G;
+    RowsGrid r;
+    r.L = 1;
+    while (r.L < 32 && r.L * vec < Cg) r.L *= 2;
+    const long long per = NTHR / r.L, need = (N * G + per - 1) / per;
+    long long most = (bwd ? 4LL : 8LL) * sm_count();
+    const long long least = (G + per - 1) / per;   // every group has a slot
+    if (most < least) most = least;
+    r.ctas = need < least ? least : need < most ? need : most;
+    r.step = r.ctas * per / G;
+    return r;
+}
+// elements per access: 16 bytes where every group (or, for `rows_only`, every row) starts on 16 bytes
+static int vec_of(int unit, int es, const void* x, const void* y, const void* z) {
+    const int full = 16 / es;
+    return unit % full == 0 && (((uintptr_t)x | (uintptr_t)y | (uintptr_t)z) & 15) == 0 ? full : 1;
+}
+
+template <typename T, int VEC, bool BWD>
+static cudaError_t rows_launch(const Args& a, cudaStream_t s) {
+    const RowsGrid r = rows_grid(a.N, a.Ch, a.G, VEC, BWD);
+    const int nv = (a.Ch / a.G + r.L * VEC - 1) / (r.L * VEC);
+    cudaError_t e;
+    if (nv <= 1) e = launch_dependent(group_norm_rows_kernel<T, VEC, 1, BWD>, dim3((unsigned)r.ctas), NTHR, 0, s, a, r.L);
+    else if (nv <= 4) e = launch_dependent(group_norm_rows_kernel<T, VEC, 4, BWD>, dim3((unsigned)r.ctas), NTHR, 0, s, a, r.L);
+    else if (VEC > 1 && nv <= 32 / VEC) e = launch_dependent(group_norm_rows_kernel<T, VEC, 32 / VEC, BWD>, dim3((unsigned)r.ctas), NTHR, 0, s, a, r.L);
+    else e = launch_dependent(group_norm_rows_kernel<T, VEC, VEC == 1 ? 32 : 1, BWD>, dim3((unsigned)r.ctas), NTHR, 0, s, a, r.L);
+    if (e == cudaSuccess && BWD && a.dw)
+        e = launch_dependent(group_norm_params_kernel, dim3((a.Ch + 31) / 32, 2), dim3(32, 32), 0, s, (const float*)a.part, r.step, a.Ch, a.dw, a.db);
+    return e;
+}
+
+template <typename T, int VEC, bool BWD>
+static cudaError_t slices_launch(const Args& a, cudaStream_t s) {
+    const dim3 grid((unsigned)(a.N * a.slices)), groups((unsigned)(a.N * a.G));
+    const int cols = a.Ch / VEC, TC = cols < NTHR ? cols : NTHR, TR = NTHR / TC;
+    const size_t smem = (size_t)2 * TR * TC * VEC * sizeof(float);
+    cudaError_t e = launch_dependent(group_norm_sums_kernel<T, VEC, BWD ? 1 : 0>, grid, NTHR, smem, s, a);
+    if (e == cudaSuccess) e = BWD ? launch_dependent(group_norm_means_kernel, groups, 128, 0, s, a) : launch_dependent(group_norm_stats_kernel<T>, groups, 128, 0, s, a);
+    if (e == cudaSuccess) e = launch_dependent(group_norm_apply_kernel<T, VEC, BWD>, grid, NTHR, 0, s, a);
+    if (e == cudaSuccess && BWD && a.dw)
+        e = launch_dependent(group_norm_params_kernel, dim3((a.Ch + 31) / 32, 2), dim3(32, 32), 0, s, (const float*)a.part, a.N * a.slices, a.Ch, a.dw, a.db);
+    return e;
+}
+
+template <typename T, bool BWD>
+static cudaError_t dispatch(const Args& a, cudaStream_t s) {
+    constexpr int FULL = 16 / sizeof(T);
+    const bool rows = by_rows(a.S, a.Ch, a.G);
+    const int vec = vec_of(rows ? a.Ch / a.G : a.Ch, sizeof(T), a.x, BWD ? a.dx : a.y, a.dy);
+    if (rows) return vec == FULL ? rows_launch<T, FULL, BWD>(a, s) : rows_launch<T, 1, BWD>(a, s);
+    return vec == FULL ? slices_launch<T, FULL, BWD>(a, s) : slices_launch<T, 1, BWD>(a, s);
+}
+
+static int check(const Args& a, int dtype) {
+    if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
+    if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.G <= 0 || a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
+    // grids of samples x slices and samples x groups
+    if (!by_rows(a.S, a.Ch, a.G) && (a.N > 0x7fffffffLL / MAX_SLICES || a.N > 0x7fffffffLL / a.G)) return KDA_ERR_SHAPE;
+    if (by_rows(a.S, a.Ch, a.G) && a.N > (1LL << 40) / a.G) return KDA_ERR_SHAPE;
+    return KDA_OK;
+}
+static size_t scratch(long long N, long long S, int Ch, int G, int es, bool bwd) {
+    if (by_rows(S, Ch, G)) {
+        if (!bwd) return 0;
+        long long step = rows_grid(N, Ch, G, 1, true).step;  // (the element width is known only with the pointers)
+        const long long wide = (Ch / G) % (16 / es) ? 0 : rows_grid(N, Ch, G, 16 / es, true).step;
+        if (wide > step) step = wide;
+        return (size_t)step * 2 * Ch * sizeof(float);
+    }
+    return ((size_t)N * slice_count(N, S) * 2 * Ch + (size_t)N * G * 2) * sizeof(float);
+}
+
+}  // namespace gn
+}  // namespace kda
+
+using namespace kda;
+
+extern "C" int kda_group_norm_scratch_bytes(int64_t N, int64_t S, int32_t channels, int32_t groups, int32_t dtype, size_t* fwd_bytes,
+                                            size_t* bwd_bytes) {
+    gn::Args a = {};
+    a.N = N; a.S = S; a.Ch = channels; a.G = groups;
+    if (const int rc = gn::check(a, dtype)) return rc;
+    const int es = dtype == KDA_DTYPE_F32 ? 4 : 2;
+    if (fwd_bytes) *fwd_bytes = gn::scratch(N, S, channels, groups, es, false);
+    if (bwd_bytes) *bwd_bytes = gn::scratch(N, S, channels, groups, es, true);
+    return KDA_OK;
+}
+
+extern "C" int kda_group_norm_fwd(const void* x, const float* weight, const float* bias, void* y, float* mean, float* rstd,
+                                  float* scratch, int64_t N, int64_t S, int32_t channels, int32_t groups, float eps, int32_t silu,
+                                  int32_t dtype, void* stream) {
+    gn::Args a = {};
+    a.x = x; a.y = y; a.w = weight; a.b = bias; a.mean = mean; a.rstd = rstd; a.part = scratch;
+    a.N = N; a.S = S; a.Ch = channels; a.G = groups; a.act = silu; a.eps = eps;
+    if (const int rc = gn::check(a, dtype)) return rc;
+    if (!x || !y || (!gn::by_rows(S, channels, groups) && (!mean || !rstd || !scratch))) return KDA_ERR_NULL;
+    a.slices = gn::slice_count(N, S);
+    const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, false>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, false>(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? KDA_OK : fail_cuda(e);
+}
+
+extern "C" int kda_group_norm_bwd(const void* x, const float* weight, const float* bias, const float* mean, const float* rstd,
+                                  const void* dy, void* dx, float* dweight, float* dbias, float* scratch, int64_t N, int64_t S,
+                                  int32_t channels, int32_t groups, float eps, int32_t silu, int32_t dtype, void* stream) {
+    gn::Args a = {};
+    a.x = x; a.dy = dy; a.dx = dx; a.w = weight; a.b = bias; a.mean = const_cast<float*>(mean); a.rstd = const_cast<float*>(rstd);
+    a.dw = dweight; a.db = dbias; a.part = scratch;
+    a.N = N; a.S = S; a.Ch = channels; a.G = groups; a.act = silu; a.eps = eps;
+    if (const int rc = gn::check(a, dtype)) return rc;
+    const bool rows = gn::by_rows(S, channels, groups);
+    if (!x || !dy || !dx || (!rows && (!mean || !rstd || !scratch)) || (dweight && (!dbias || !scratch)) || (!dweight && dbias)) return KDA_ERR_NULL;
+    a.slices = gn::slice_count(N, S);
+    const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, true>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, true>(a, (cudaStream_t)stream);
+    return e == cudaSuccess ? KDA_OK : fail_cuda(e);
+}

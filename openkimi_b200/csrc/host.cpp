@@ -3,148 +3,13 @@
 // The Python modules keep the public signatures and everything that is not on such a path.
 //
 // No tensor is kept from one call for the next; the only state here is the table of the devices' status words.
-#include <ATen/MemoryOverlap.h>
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/extension.h>
+#include "host_util.h"
 
-#include <algorithm>
-#include <atomic>
-#include <cmath>
-#include <cstdlib>
-#include <optional>
-#include <string>
+using namespace kda_host;
 
-#include "../../include/kda_b200.h"
-
-namespace py = pybind11;
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+void bind_gdr(py::module_& m);  // host_gdr.cpp
 
 namespace {
-
-constexpr int CHUNK = KDA_CHUNK;
-
-// ---- per-device status word and its pinned host mirror (owned by ops._DeviceStatus) -------------------------
-constexpr int MAX_DEVICES = 64;
-struct StatusWord {
-    std::atomic<int32_t*> dev{nullptr};  // set after host: calls of other threads look without the interpreter lock
-    const volatile int32_t* host = nullptr;
-};
-StatusWord g_status[MAX_DEVICES];
-// Python callables: status_of(device_index) creates the words; report(device_index) raises and clears;
-// guard_span() reads the mutable span of the guard contract
-py::object* g_status_of = nullptr;
-py::object* g_report = nullptr;
-py::object* g_guard_span = nullptr;
-
-void set_status(int device, int64_t dev_ptr, int64_t host_ptr) {
-    TORCH_CHECK(device >= 0 && device < MAX_DEVICES, "device index out of range");
-    g_status[device].host = reinterpret_cast<const volatile int32_t*>(host_ptr);
-    g_status[device].dev.store(reinterpret_cast<int32_t*>(dev_ptr), std::memory_order_release);
-}
-
-void set_callbacks(py::object status_of, py::object report, py::object guard_span) {
-    g_status_of = new py::object(std::move(status_of));  // (never destroyed: they outlive the interpreter's modules)
-    g_report = new py::object(std::move(report));
-    g_guard_span = new py::object(std::move(guard_span));
-}
-
-const StatusWord& status_word(int device) {
-    TORCH_CHECK(device >= 0 && device < MAX_DEVICES, "device index out of range");
-    const StatusWord& st = g_status[device];
-    if (!st.dev.load(std::memory_order_acquire) || *st.host) {
-        py::gil_scoped_acquire gil;
-        if (!st.dev.load(std::memory_order_relaxed)) (*g_status_of)(device);
-        if (*st.host) (*g_report)(device);  // a wait that gave up in an earlier call surfaces here
-    }
-    return st;
-}
-
-// the guard contract's span is a module attribute that callers may change between calls; it is read at every call
-float guard_span() {
-    py::gil_scoped_acquire gil;
-    return (*g_guard_span)().cast<float>();
-}
-
-// debugging / A-B switches of the environment (ops.chunk_kda documents them), read at every call
-int64_t env_flags() {
-    auto is_one = [](const char* n) { const char* v = std::getenv(n); return v && v[0] == '1' && !v[1]; };
-    int64_t f = 0;
-    if (is_one("OPENKIMI_B200_FP32_MATH")) f |= KDA_FLAG_FORCE_SIMT;
-    if (is_one("OPENKIMI_B200_ROW_COPIES")) f |= KDA_FLAG_ROW_COPIES;
-    if (const char* v = std::getenv("OPENKIMI_B200_FP32_STAGES")) f |= (std::strtol(v, nullptr, 10) & 31) << 5;
-    return f;
-}
-
-void check_rc(int rc, const char* what) {
-    if (rc == KDA_OK) return;
-    std::string msg = std::string(what) + " failed: " + kda_status_string(rc);
-    const std::string extra = kda_last_cuda_error();
-    if (rc == KDA_ERR_LAUNCH && !extra.empty()) msg += " (" + extra + ")";
-    throw std::runtime_error(msg);
-}
-
-std::string shape_of(const Tensor& t) {
-    std::string s = "(";
-    for (int64_t i = 0; i < t.dim(); ++i) s += (i ? ", " : "") + std::to_string(t.size(i));
-    return s + (t.dim() == 1 ? ",)" : ")");
-}
-[[noreturn]] void value_error(const std::string& m) { throw py::value_error(m); }
-[[noreturn]] void type_error(const std::string& m) { throw py::type_error(m); }
-
-void require_cuda(const Tensor& t) {
-    if (!t.is_cuda()) throw std::runtime_error("chunk_kda runs only on a CUDA device (sm_100a); there is no CPU fallback");
-}
-
-// the kernels follow raw pointers: every tensor of a call has to be where q is
-void require_device(const Tensor& q, const char* name, const Tensor& t) {
-    if (t.defined() && t.device() != q.device())
-        throw std::runtime_error(std::string("expected ") + name + " on " + q.device().str() + ", the device of q, but it is on " +
-                                 t.device().str());
-}
-
-// A call that nobody differentiates backward does not pass through its autograd node, which refuses forward-mode inputs.
-template <class Tensors>
-void refuse_tangents(const Tensors& inputs) {
-    for (const Tensor* t : inputs)
-        if (t->defined() && t->_fw_grad(0).defined())
-            throw std::runtime_error("the KDA kernels have no forward-mode derivative (an input carries a tangent)");
-}
-
-int dtype_code(const Tensor& t) {
-    if (t.scalar_type() == at::kBFloat16) return KDA_DTYPE_BF16;
-    if (t.scalar_type() == at::kFloat) return KDA_DTYPE_F32;
-    type_error(std::string("q/k/v must be float32 or bfloat16, got ") + c10::toString(t.scalar_type()));
-}
-
-// contiguous, in dtype dt, starting on a 16-byte boundary (a view into the middle of a buffer is copied)
-Tensor ready(const Tensor& t, at::ScalarType dt) {
-    Tensor r = t.scalar_type() == dt ? t : t.to(dt);
-    if (!r.is_contiguous()) r = r.contiguous();
-    return (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0 ? r : r.clone();
-}
-// the same without a new reference where t is that already or undefined; copy holds what else it becomes
-const Tensor& ready(const Tensor& t, at::ScalarType dt, Tensor& copy) {
-    if (!t.defined() || (t.scalar_type() == dt && t.is_contiguous() && (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0)) return t;
-    return copy = ready(t, dt);
-}
-// a new tensor without the dispatcher's detour (half of what at::empty costs)
-Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const Tensor& like) {
-    return Tensor(at::detail::empty_cuda(sizes, dt, like.device(), std::nullopt));
-}
-const Tensor& val(const OptTensor& t) {
-    static const Tensor none;
-    return t ? *t : none;
-}
-template <class T>
-T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
-
-void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
 // ---- recurrent steps -----------------------------------------------------------------------------------------
 // q, k, g, v: [N, (T,) H, K]; multi says whether the token axis is there
@@ -261,9 +126,6 @@ Prepared prepare(const Inputs& in, const Spec& sp, int flags) {
     check_rc(kda_workspace_bytes(&p, &r.fwd_bytes, &r.bwd_bytes), "kda_workspace_bytes");
     return r;
 }
-
-Tensor bytes(size_t n, const Tensor& like) { return fresh({(int64_t)n}, at::kByte, like); }
-Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
 
 std::array<int64_t, 4> state_shape(const Inputs& in, const Spec& sp, int64_t N) {
     const int64_t H = in.q.size(2), dk = in.q.size(3), dv = in.v.size(3);
@@ -404,8 +266,6 @@ Spec load_spec(AutogradContext* ctx) {
     return sp;
 }
 Tensor as_filter(const Tensor& w) { return w.defined() ? w.view({w.size(0), 1, w.size(1)}) : w; }
-
-OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }  // (a node's inputs must be defined tensors)
 
 struct ChunkKda : torch::autograd::Function<ChunkKda> {
     static variable_list forward(AutogradContext* ctx, Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, OptTensor A_log,
@@ -776,4 +636,5 @@ PYBIND11_MODULE(_host, m) {
     m.def("chunk_kda", &chunk_kda, unlocked);
     m.def("layer", &layer, unlocked);
     m.def("layer_takes", &layer_takes);
+    bind_gdr(m);
 }

@@ -107,7 +107,8 @@ struct ChunkInfo {
     int len;        // valid rows, 1..64
 };
 
-__device__ __forceinline__ ChunkInfo chunk_info(const KdaParams& p, int c) {
+template <class Params>  // KdaParams or KdaGdrParams
+__device__ __forceinline__ ChunkInfo chunk_info(const Params& p, int c) {
     ChunkInfo ci;
     if (p.cu_seqlens != nullptr && p.chunk_tab != nullptr) {
         const int4 t = reinterpret_cast<const int4*>(p.chunk_tab)[c];
@@ -134,7 +135,8 @@ __device__ __forceinline__ ChunkInfo chunk_info(const KdaParams& p, int c) {
 }
 
 // first chunk and number of chunks of sequence n
-__device__ __forceinline__ void seq_chunks(const KdaParams& p, int n, int& c0, int& nc) {
+template <class Params>  // KdaParams or KdaGdrParams
+__device__ __forceinline__ void seq_chunks(const Params& p, int n, int& c0, int& nc) {
     if (p.cu_seqlens != nullptr) {
         c0 = p.seq_chunk_off[n];
         nc = p.seq_chunk_off[n + 1] - c0;
@@ -147,7 +149,8 @@ __device__ __forceinline__ void seq_chunks(const KdaParams& p, int n, int& c0, i
 // first and one-past-last flattened token index of sequence n; chunk lc of the sequence then starts at
 // first + lc * C and holds min(C, end - start) rows (what chunk_info returns, without its division / table load:
 // for the kernels that walk the chunks of ONE sequence)
-__device__ __forceinline__ void seq_tokens(const KdaParams& p, int n, long long& first, long long& end) {
+template <class Params>  // KdaParams or KdaGdrParams
+__device__ __forceinline__ void seq_tokens(const Params& p, int n, long long& first, long long& end) {
     if (p.cu_seqlens != nullptr) {
         first = p.cu_seqlens[n];
         end = p.cu_seqlens[n + 1];

@@ -17,7 +17,7 @@
 //
 // 1536 units, one token: 48.2 us with the state in shared memory -> 36.1 us, 5.6 TB/s; one sequence of six heads:
 // 6.6 -> 3.6 us; eight tokens of four sequences: eight launches of 7 us -> 7.0 us.
-#include "kda_common.cuh"
+#include "kda_decode.cuh"
 
 namespace kda {
 
@@ -27,60 +27,6 @@ constexpr int TB = 16;    // tokens whose prologue is in shared memory at a time
 // floats of one token's prologue: k alpha, scale q alpha, alpha, k (4 x D), v (D), beta, scale q.k, padding
 __host__ __device__ constexpr int tok_floats(int D) { return 5 * D + 4; }
 }  // namespace dec
-
-template <typename T, int N>
-__device__ __forceinline__ void load_n(const T* p, float (&v)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = ldf(p + i);
-}
-template <>
-__device__ __forceinline__ void load_n<__nv_bfloat16, 4>(const __nv_bfloat16* p, float (&v)[4]) {
-    const uint2 r = *reinterpret_cast<const uint2*>(p);
-    v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
-    v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
-}
-template <>
-__device__ __forceinline__ void load_n<float, 4>(const float* p, float (&v)[4]) {
-    const float4 r = *reinterpret_cast<const float4*>(p);
-    v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
-}
-
-// vec: the caller's rows start on a four-element boundary
-template <typename T, int N>
-__device__ __forceinline__ void load_row(const T* p, float (&v)[N], int vec) {
-    if (vec) {
-        load_n(p, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = ldf(p + i);
-    }
-}
-
-// Sums val[0..M) over the LD lanes that differ in the given lane bits (bit0, 2 bit0, ..., LD / 2 * bit0), halving the
-// number of values a lane carries at every level: afterwards val[0] of a lane is the total of value `which`
-// (the lane bits read from the lowest level up as the most significant bit of the index first).
-template <int M, int LD, int BIT0>
-struct TransposeSum {
-    static __device__ __forceinline__ void run(float (&val)[M], int lane, int& which) {
-        if constexpr (LD > 1) {
-            const bool up = lane & BIT0;
-            if constexpr (M > 1) {
-                float half[M / 2];
-#pragma unroll
-                for (int i = 0; i < M / 2; ++i) {
-                    const float keep = up ? val[M / 2 + i] : val[i], send = up ? val[i] : val[M / 2 + i];
-                    half[i] = keep + __shfl_xor_sync(0xffffffffu, send, BIT0);
-                }
-                which = 2 * which + (up ? 1 : 0);
-                TransposeSum<M / 2, LD / 2, 2 * BIT0>::run(half, lane, which);
-                val[0] = half[0];
-            } else {
-                val[0] += __shfl_xor_sync(0xffffffffu, val[0], BIT0);
-                TransposeSum<1, LD / 2, 2 * BIT0>::run(val, lane, which);
-            }
-        }
-    }
-};
 
 // T: element type; D: channels; VF: [dv][dk] state; R: value columns per warp
 template <typename T, int D, bool VF, int R>

@@ -204,6 +204,35 @@ def _plain(m, cls):
                                                                    or m._backward_pre_hooks)
 
 
+def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
+    """Group normalisation of channels-last x [N, ..., channels] with an activation: mean and variance over everything between the
+    first and the last axis and over the channels of a group, then ``weight``, ``bias`` (each [channels] or None) and ``activation``
+    (None or "silu").  x of shape [tokens, channels] normalises every token by itself (the heads of a layer's output, say).
+    BF16 or FP32; statistics and parameter gradients in FP32 or more."""
+    if activation not in (None, "silu", "swish"):
+        raise ValueError(f"group_norm supports activation None or 'silu', got {activation!r}")
+    return _lib.host().group_norm(x, num_groups, weight, bias, eps, activation is not None)
+
+
+class FusedGroupNorm(nn.Module):
+    """``group_norm`` with learned weight and bias: y = act(norm(x) * weight + bias) over x [N, ..., channels]."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation=None):
+        super().__init__()
+        if num_groups < 1 or num_channels % num_groups:
+            raise ValueError(f"num_channels ({num_channels}) must be divisible by num_groups ({num_groups})")
+        if activation not in (None, "silu", "swish"):
+            raise ValueError(f"FusedGroupNorm supports activation None or 'silu', got {activation!r}")
+        self.num_groups, self.num_channels, self.eps, self.activation = num_groups, num_channels, eps, activation
+        self.weight = nn.Parameter(torch.ones(num_channels)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(num_channels)) if affine else None
+
+    def forward(self, x):
+        if x.shape[-1] != self.num_channels:
+            raise ValueError(f"expected last dimension {self.num_channels}, got {x.shape[-1]}")
+        return group_norm(x, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+
 class KimiDeltaAttention(nn.Module):
     """The KDA sublayer of k3mini/model.py:132-227 on the B200 kernels: q/k/v projections,
     short conv + SiLU, decay and beta projections, ``chunk_kda`` with the fused L2 norm /
