@@ -309,6 +309,7 @@ typedef struct KdaGdrParams {
     float *grad_h0;              /* may be NULL */
     void *bwd_scratch;
     size_t bwd_scratch_bytes;
+    int32_t *status, *status_host; /* as in KdaParams; may be NULL */
 } KdaGdrParams;
 int kda_gdr_workspace_bytes(const KdaGdrParams *p, size_t *fwd_bytes, size_t *bwd_bytes);
 int kda_gdr_fwd(const KdaGdrParams *p, void *cuda_stream);

@@ -54,7 +54,8 @@ class KdaGdrParams(C.Structure):
         + [(n, C.c_void_p) for n in ("q", "k", "v", "g", "beta", "A_log", "dt_bias", "h0", "cu_seqlens", "chunk_seq", "seq_chunk_off",
                                      "chunk_tab", "o", "ht", "workspace")] + [("workspace_bytes", C.c_size_t)]
         + [(n, C.c_void_p) for n in ("grad_o", "grad_ht", "grad_q", "grad_k", "grad_v", "grad_g", "grad_beta", "grad_A_log",
-                                     "grad_dt_bias", "grad_h0", "bwd_scratch")] + [("bwd_scratch_bytes", C.c_size_t)])
+                                     "grad_dt_bias", "grad_h0", "bwd_scratch")] + [("bwd_scratch_bytes", C.c_size_t),
+                                                                                    ("status", C.c_void_p), ("status_host", C.c_void_p)])
 
 
 EXPORTS = {

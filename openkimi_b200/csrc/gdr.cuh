@@ -20,8 +20,13 @@ using bf16 = __nv_bfloat16;
 constexpr int NBLK = 10;           // 16 x 16 blocks of a lower triangular 64 x 64 matrix
 constexpr int BLK = 256;           // elements of one
 constexpr int TRI = NBLK * BLK;    // elements of one part of such a matrix
-constexpr int AUX = 8 * C;         // floats of a unit's per-row numbers
-enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST };  // e^G, e^(G_last - G), beta, 1/|q|, 1/|k|, G in two floats; [A_LAST][0] = e^G_last
+constexpr int AUX = 12 * C;        // floats of a unit's per-row numbers
+// e^G, e^(G_last - G), beta, 1/|q|, 1/|k|, G in two floats, [A_LAST][0] = e^G_last; and the factors that the walks use:
+// beta e^G / |k|, e^(G_last - G) / |k|, scale e^G / |q|
+enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST, A_BGK, A_FK, A_OQ };
+constexpr int SQ = C * C;          // elements of one part of a 64 x 64 matrix in core-matrix order (cm_idx)
+// BF16 with 128 value columns walks the chunks on tcgen05; T and A are then whole matrices in core-matrix order
+__host__ __device__ __forceinline__ bool on_tc(const KdaGdrParams& p) { return p.dtype == KDA_DTYPE_BF16 && p.dv == 128; }
 constexpr float G_MIN = -1000.f;   // log decays below count as this: e^-1000 is 0 in FP32, and sums of 64 stay finite
 
 __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I * (I + 1) / 2 + J; }
@@ -32,12 +37,14 @@ struct Layout {
     size_t dS, Y, part, dqk, bwd_total;                   // backward scratch
 };
 __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
-    const size_t n = (size_t)p.NT * p.HV;
+    const size_t n = (size_t)p.NT * p.HV, mat = 3 * (on_tc(p) ? SQ : TRI) * 2;
     Layout l;
     size_t off = 0;
     l.aux = off; off = align256(off + n * AUX * 4);
-    l.T = off;   off = align256(off + n * 3 * TRI * 2);   // (I + diag(beta) L)^-1 and scale (q k^T) D as three BF16 parts, blocks of
-    l.A = off;   off = align256(off + n * 3 * TRI * 2);   // the lower triangle in blk() order, rows swizzled as tri_frag reads them
+    // (I + diag(beta) L)^-1 and scale (q k^T) D as three BF16 parts: blocks of the lower triangle in blk() order, rows swizzled as
+    // tri_frag reads them, or (on_tc) [64][64] in core-matrix order of which only those blocks are written
+    l.T = off;   off = align256(off + n * mat);
+    l.A = off;   off = align256(off + n * mat);
     l.total_nosave = off;
     l.S0 = off;  off = align256(off + n * p.dk * p.dv * 4);  // state at the chunk's start [dk][dv]
     l.Vn = off;  off = align256(off + n * C * p.dv * 4);     // V' [64][dv]

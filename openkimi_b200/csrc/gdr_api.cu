@@ -7,6 +7,8 @@ namespace kda {
 namespace gdr {
 cudaError_t intra(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
 cudaError_t fwd_state(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
+cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
+cudaError_t bwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
 cudaError_t bwd_state(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
 cudaError_t grad(const KdaGdrParams& p, const Layout& l, cudaStream_t s);
 
@@ -63,14 +65,14 @@ extern "C" int kda_gdr_fwd(const KdaGdrParams* p, void* stream) {
     if (const int rc = gdr::validate(p, false)) return rc;
     const gdr::Layout l = gdr::layout(*p);
     cudaError_t e = gdr::intra(*p, l, (cudaStream_t)stream);
-    if (e == cudaSuccess) e = gdr::fwd_state(*p, l, (cudaStream_t)stream);
+    if (e == cudaSuccess) e = gdr::on_tc(*p) ? gdr::fwd_tc(*p, l, (cudaStream_t)stream) : gdr::fwd_state(*p, l, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }
 
 extern "C" int kda_gdr_bwd(const KdaGdrParams* p, void* stream) {
     if (const int rc = gdr::validate(p, true)) return rc;
     const gdr::Layout l = gdr::layout(*p);
-    cudaError_t e = gdr::bwd_state(*p, l, (cudaStream_t)stream);
+    cudaError_t e = gdr::on_tc(*p) ? gdr::bwd_tc(*p, l, (cudaStream_t)stream) : gdr::bwd_state(*p, l, (cudaStream_t)stream);
     if (e == cudaSuccess) e = gdr::grad(*p, l, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }

@@ -14,9 +14,9 @@ namespace gdr {
 
 constexpr int LDL = 68;  // floats per row of L / T
 
-template <typename T, int K>
+template <typename T, int K, bool CM>  // CM: records in core-matrix order
 __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, const Layout lay) {
-    constexpr int P = In<T>::P, LD = K + 8, TILE = C * LD;
+    constexpr int P = In<T>::P, LD = K + 8, TILE = C * LD, PART = CM ? SQ : TRI;
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* sq = reinterpret_cast<bf16*>(smem);
     bf16* sk = sq + P * TILE;
@@ -106,8 +106,12 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
                 const int r = 2 * lane + i;
                 const float hi = (float)G[i], lo = (float)(G[i] - hi);
                 ghi[r] = hi; glo[r] = lo; sb[r] = be[i];
-                aux[A_GAM * C + r] = expf(hi) * (1.f + lo);
-                aux[A_FALL * C + r] = expf((float)(last - G[i]));
+                const float gam = expf(hi) * (1.f + lo), fall = expf((float)(last - G[i]));
+                aux[A_GAM * C + r] = gam;
+                aux[A_FALL * C + r] = fall;
+                aux[A_BGK * C + r] = be[i] * gam * rk[r];
+                aux[A_FK * C + r] = fall * rk[r];
+                aux[A_OQ * C + r] = p.scale * gam * rq[r];
                 aux[A_BETA * C + r] = be[i];
                 aux[A_RQ * C + r] = rq[r];
                 aux[A_RK * C + r] = rk[r];
@@ -117,7 +121,7 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
             if (lane == 0) aux[A_LAST * C] = expf((float)last);
         }
         __syncthreads();
-        bf16* A = reinterpret_cast<bf16*>(static_cast<char*>(p.workspace) + lay.A) + unit * 3 * TRI;
+        bf16* A = reinterpret_cast<bf16*>(static_cast<char*>(p.workspace) + lay.A) + unit * 3 * PART;
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
             if (n / 2 > w) break;
@@ -132,7 +136,7 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
                     a[x] = i >= jj ? p.scale * qk[n][2 * r + x] * rq[i] * rk[jj] * d : 0.f;
                     l[x] = i > jj ? sb[i] * (kk[n][2 * r + x] * rk[i] * rk[jj] * d) : 0.f;
                 }
-                put<3>(A, TRI, blk(w, n / 2) * BLK + tri_idx(i & 15, j & 15), a[0], a[1]);
+                put<3>(A, PART, CM ? cm_idx(i, j, C) : blk(w, n / 2) * BLK + tri_idx(i & 15, j & 15), a[0], a[1]);
                 *reinterpret_cast<float2*>(L + i * LDL + j) = make_float2(l[0], l[1]);
             }
         }
@@ -183,28 +187,29 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
             for (int i = 0; i < s / 4; ++i) L[(R + r) * LDL + Cc + c0 + i] = -acc[i];
             __syncthreads();
         }
-        bf16* Tm = reinterpret_cast<bf16*>(static_cast<char*>(p.workspace) + lay.T) + unit * 3 * TRI;
+        bf16* Tm = reinterpret_cast<bf16*>(static_cast<char*>(p.workspace) + lay.T) + unit * 3 * PART;
         for (int i = tid; i < NBLK * 128; i += 128) {
             const int b = i >> 7, r = (i >> 3) & 15, cc = (i & 7) * 2;
             const int I = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, J = b - blk(I, 0);
             const float2 x = *reinterpret_cast<const float2*>(L + (16 * I + r) * LDL + 16 * J + cc);
-            put<3>(Tm, TRI, b * BLK + tri_idx(r, cc), x.x, x.y);
+            put<3>(Tm, PART, CM ? cm_idx(16 * I + r, 16 * J + cc, C) : b * BLK + tri_idx(r, cc), x.x, x.y);
         }
         __syncthreads();
     }
 }
 
-template <typename T, int K>
+template <typename T, int K, bool CM>
 static cudaError_t launch_intra(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
     constexpr int bytes = 2 * In<T>::P * C * (K + 8) * 2 + (C * LDL + 32 * 36 + 5 * C) * 4;
-    cudaError_t e = allow_smem(gdr_intra_kernel<T, K>, bytes);
+    cudaError_t e = allow_smem(gdr_intra_kernel<T, K, CM>, bytes);
     if (e != cudaSuccess) return e;
-    return launch_dependent(gdr_intra_kernel<T, K>, p.NT * p.H, 128, bytes, s, p, l);
+    return launch_dependent(gdr_intra_kernel<T, K, CM>, p.NT * p.H, 128, bytes, s, p, l);
 }
 
 cudaError_t intra(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    if (p.dtype == KDA_DTYPE_F32) return p.dk == 64 ? launch_intra<float, 64>(p, l, s) : launch_intra<float, 128>(p, l, s);
-    return p.dk == 64 ? launch_intra<bf16, 64>(p, l, s) : launch_intra<bf16, 128>(p, l, s);
+    if (p.dtype == KDA_DTYPE_F32) return p.dk == 64 ? launch_intra<float, 64, false>(p, l, s) : launch_intra<float, 128, false>(p, l, s);
+    if (on_tc(p)) return p.dk == 64 ? launch_intra<bf16, 64, true>(p, l, s) : launch_intra<bf16, 128, true>(p, l, s);
+    return p.dk == 64 ? launch_intra<bf16, 64, false>(p, l, s) : launch_intra<bf16, 128, false>(p, l, s);
 }
 
 }  // namespace gdr

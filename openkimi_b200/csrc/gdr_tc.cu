@@ -1,0 +1,749 @@
+// Gated delta rule, the walks along the chunks on tcgen05 (BF16, 128 value columns; gdr_state.cu has the other sizes and FP32).
+//
+// One CTA per (sequence, value head).  Everything is transposed, value column e = TMEM lane e, so that the 128 lanes are full:
+//   P^T = S^T k^T    R^T = beta v^T - (beta e^G / |k|) P^T    V'^T = R^T T^T    W^T = e^(G_last-G) / |k| V'^T
+//   S^T <- e^G_last S^T + W^T k          o^T = scale e^G / |q| (S^T q^T) + V'^T A^T
+// The state stays in registers in FP32 (256 threads: lane e, half of the key channels).  A computed operand goes to tensor memory in
+// three BF16 parts and multiplies q, k, T, A from shared memory, where T and A have three parts too; products of the smallest
+// parts are accumulated first, so that the accumulator's truncation falls on small sums.  The update is accumulated from zero and
+// added to the decayed state in FP32.
+// Bound by the chain of a chunk: split S - S k - R - R T - V' - W k - S.  Everything else is off it: two producer warps bring the next
+// chunk's rows (core-matrix order) and records, one warp issues all products, four warps turn finished outputs into rows.
+#include "gdr.cuh"
+
+namespace kda {
+namespace gdr {
+
+namespace ft {
+constexpr int MAIN = 256, OUT = 128, PROD = 64, NTHR = MAIN + OUT + PROD + 32;
+template <int K>
+struct Map {
+    static constexpr int DH = K / 2;                       // key channels of a main thread
+    static constexpr uint32_t ROWS = C * K * 2, MAT = SQ * 2;
+    static constexpr uint32_t KK = 0, Q = ROWS, V = 2 * ROWS, TM = V + C * 256, AM = TM + 3 * MAT, AU = AM + 2 * MAT, STAGE = AU + AUX * 4;
+    static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
+    // tensor memory columns.  S parts: per half three blocks of DH / 2; over them, once S k and S q are done, the update (DH columns)
+    // and, with K = 128, in the third block the parts of V'.  V' itself over S k, W over R.
+    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, VPS = K == 128 ? HB : 32, VP = K == 128 ? DH : 2 * HB,
+                              KS = K == 128 ? 2 * HB : 2 * HB + 64, QS = KS + 64, AV = QS + 64, R = AV + 64, COLS = R + 96;
+    static_assert(COLS <= 512 && TOTAL <= 232448, "fits");
+};
+}  // namespace ft
+
+// 16 consecutive values as P parts: 8 TMEM columns each, `stride` columns apart
+template <int P>
+__device__ __forceinline__ void st_parts(uint32_t at, uint32_t stride, const float (&x)[16]) {
+    uint32_t w[P][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t s[P];
+        split(x[2 * j], x[2 * j + 1], s);
+#pragma unroll
+        for (int i = 0; i < P; ++i) w[i][j] = s[i];
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) tmem_st8(at + i * stride, w[i]);
+}
+__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
+#pragma unroll
+    for (int j = 0; j < 16; j += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p + j);
+        x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
+    }
+}
+// rows of COLS elements, `stride` apart in memory, into core-matrix order; lanes take 8 rows x 4 chunks of 16 bytes at a time
+template <int COLS, int NTHR>
+__device__ __forceinline__ void load_cm(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
+    constexpr int CG = COLS / 32;
+    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
+#pragma unroll 4
+    for (int i = tid >> 5; i < 8 * CG; i += NTHR / 32) {
+        const int rr = i / CG * 8 + r, cc = (i % CG * 4 + c) * 8;
+        const bool in = rr < rows;
+        cp_async16_z(dst + cm_idx(rr, cc, COLS), src + (in ? rr * stride + cc : 0), in);
+    }
+}
+
+// the same with rows of 128 elements into two halves of 64 with 128-byte swizzle (swz_bf16)
+template <int NTHR>
+__device__ __forceinline__ void load_swz(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
+    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
+#pragma unroll 4
+    for (int i = tid >> 5; i < 32; i += NTHR / 32) {
+        const int rr = (i >> 2) * 8 + r, cc = ((i & 3) * 4 + c) * 8;
+        const bool in = rr < rows;
+        cp_async16_z(dst + swz_bf16(rr, cc), src + (in ? rr * stride + cc : 0), in);
+    }
+}
+
+struct Walk {
+    int n, h, kh, c0, nc;
+    long long tok_begin, tok_end;
+    __device__ __forceinline__ long long tok(int c) const { return tok_begin + (long long)c * C; }
+    __device__ __forceinline__ int rows(int c) const { return (int)min((long long)C, tok_end - tok(c)); }
+};
+
+template <int K, bool SAVE>
+__global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
+    using namespace ft;
+    using M = Map<K>;
+    constexpr int DH = M::DH;
+    extern __shared__ __align__(1024) unsigned char dyn[];
+    __shared__ uint64_t full[2], empty[2], sready, ksbar, rready, vbar, wready, sibar, obar, ofree;
+    __shared__ uint32_t tmem_s;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (warp == 0) {
+        tmem_alloc(&tmem_s, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&full[i], 1 + PROD / 32);
+            mbar_init(&empty[i], OUT / 32);
+        }
+        mbar_init(&sready, MAIN / 32);
+        mbar_init(&rready, MAIN / 32);
+        mbar_init(&wready, MAIN / 32);
+        mbar_init(&ksbar, 1);
+        mbar_init(&vbar, 1);
+        mbar_init(&sibar, 1);
+        mbar_init(&obar, 1);
+        mbar_init(&ofree, OUT / 32);
+        mbar_fence_init();
+    }
+    pdl_wait();
+    Walk wk;
+    wk.h = blockIdx.x % p.HV; wk.n = blockIdx.x / p.HV; wk.kh = wk.h / (p.HV / p.H);
+    seq_chunks(p, wk.n, wk.c0, wk.nc);
+    seq_tokens(p, wk.n, wk.tok_begin, wk.tok_end);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem0 = tmem_s;
+    const char* ws = static_cast<const char*>(p.workspace);
+    bool ok = true;
+
+    if (warp < MAIN / 32) {
+        const int e = tid & 127, half = warp >> 2, d0 = half * DH, t0 = half * 32;
+        const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
+        const size_t sbase = (size_t)(wk.n * (size_t)p.HV + wk.h) * K * 128;
+        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST;
+        float S[DH];
+#pragma unroll
+        for (int j = 0; j < DH; j += 4) {
+            if (!p.h0) {
+                S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
+            } else if (vf) {
+                const float4 x = *reinterpret_cast<const float4*>(p.h0 + sbase + (size_t)e * K + d0 + j);
+                S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[j + i] = p.h0[sbase + (size_t)(d0 + j + i) * 128 + e];
+            }
+        }
+        for (int c = 0; c < wk.nc; ++c) {
+            const int stage = c & 1, ph = c & 1;
+            const unsigned char* b = dyn + stage * M::STAGE;
+            const float* aux = reinterpret_cast<const float*>(b + M::AU);
+            const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+            // ---- the state's parts.  The third goes where V' of the previous chunk is read until its outputs are done.
+            uint32_t low[DH / 16][8];
+#pragma unroll
+            for (int g = 0; g < DH / 16; ++g) {
+                uint32_t w[2][8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t s[3];
+                    split(S[16 * g + 2 * j], S[16 * g + 2 * j + 1], s);
+                    w[0][j] = s[0]; w[1][j] = s[1]; low[g][j] = s[2];
+                }
+                tmem_st8(tm + M::SP + half * M::HB + 8 * g, w[0]);
+                tmem_st8(tm + M::SP + half * M::HB + DH / 2 + 8 * g, w[1]);
+            }
+            if (c > 0) {
+                ok = mbar_wait(&obar, ph ^ 1, p, 1 << 12) && ok;
+                tc_fence_after();
+            }
+#pragma unroll
+            for (int g = 0; g < DH / 16; ++g) tmem_st8(tm + M::SP + half * M::HB + DH + 8 * g, low[g]);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sready);
+            if (SAVE) {
+                float* S0 = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.S0) + unit * K * 128;
+#pragma unroll
+                for (int j = 0; j < DH; ++j) S0[(size_t)(d0 + j) * 128 + e] = S[j];
+            }
+            // ---- R
+            ok = mbar_wait(&full[stage], (c >> 1) & 1, p, 1 << 12) && ok;
+            const float last = aux[A_LAST * C];
+            float x[2][16];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                load16(aux + A_BETA * C + t0 + 16 * g, x[g]);
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    x[g][j] *= __bfloat162float(reinterpret_cast<const bf16*>(b + M::V)[(t0 + 16 * g + j) * 128 + e]);
+            }
+            ok = mbar_wait(&ksbar, ph, p, 1 << 13) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            uint32_t r[2][16];
+            tmem_ld16(tm + M::KS + t0, r[0]);
+            tmem_ld16(tm + M::KS + t0 + 16, r[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[16];
+                load16(aux + A_BGK * C + t0 + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[g][j] = fmaf(-f[j], __uint_as_float(r[g][j]), x[g][j]);
+                st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, x[g]);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&rready);
+            // ---- V'
+            ok = mbar_wait(&vbar, ph, p, 1 << 14) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            tmem_ld16(tm + M::KS + t0, r[0]);
+            tmem_ld16(tm + M::KS + t0 + 16, r[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[16];
+                load16(aux + A_FK * C + t0 + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    x[g][j] = __uint_as_float(r[g][j]);
+                    f[j] *= x[g][j];
+                }
+                st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, f);
+                st_parts<2>(tm + M::VP + half * 16 + 8 * g, M::VPS, x[g]);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&wready);
+            if (SAVE) {
+                float* V = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.Vn) + unit * C * 128;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) V[(t0 + 16 * g + j) * 128 + e] = x[g][j];
+            }
+            // ---- the state at the end of the chunk
+            ok = mbar_wait(&sibar, ph, p, 1 << 15) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+#pragma unroll
+            for (int g = 0; g < DH / 16; g += 2) {
+                tmem_ld16(tm + M::SP + half * M::HB + 16 * g, r[0]);
+                tmem_ld16(tm + M::SP + half * M::HB + 16 * g + 16, r[1]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) S[16 * (g + i) + j] = fmaf(last, S[16 * (g + i) + j], __uint_as_float(r[i][j]));
+            }
+        }
+        if (p.ht && ok) {
+#pragma unroll
+            for (int j = 0; j < DH; ++j) p.ht[sbase + (vf ? (size_t)e * K + d0 + j : (size_t)(d0 + j) * 128 + e)] = S[j];
+        }
+    } else if (warp < (MAIN + OUT) / 32) {
+        const int e = tid & 127;
+        const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
+        bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
+        for (int c = 0; c < wk.nc; ++c) {
+            const int stage = c & 1;
+            const float* oq = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_OQ * C;
+            ok = mbar_wait(&obar, c & 1, p, 1 << 16) && ok;
+            ok = bar_and(2, OUT, ok);  // (also: the tile of the previous chunk has been stored)
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t o[C / 2];
+#pragma unroll
+            for (int g = 0; g < C / 16; ++g) {
+                uint32_t a[16], q[16];
+                tmem_ld16(tm + M::QS + 16 * g, q);
+                tmem_ld16(tm + M::AV + 16 * g, a);
+                tmem_wait_ld();
+                float f[16];
+                load16(oq + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; j += 2)
+                    o[8 * g + j / 2] = pack_bf16(fmaf(f[j], __uint_as_float(q[j]), __uint_as_float(a[j])),
+                                                 fmaf(f[j + 1], __uint_as_float(q[j + 1]), __uint_as_float(a[j + 1])));
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ofree);
+                mbar_arrive(&empty[stage]);
+            }
+#pragma unroll
+            for (int j = 0; j < C / 2; ++j) {
+                reinterpret_cast<uint16_t*>(tile)[(2 * j) * 128 + e] = (uint16_t)o[j];
+                reinterpret_cast<uint16_t*>(tile)[(2 * j + 1) * 128 + e] = (uint16_t)(o[j] >> 16);
+            }
+            bar_sync(2, OUT);
+            const int rows = wk.rows(c);
+            bf16* dst = static_cast<bf16*>(p.o) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
+#pragma unroll
+            for (int i = e; i < C * 16; i += OUT) {
+                const int rr = i >> 4, cc = (i & 15) * 8;
+                if (rr < rows) *reinterpret_cast<uint4*>(dst + (size_t)rr * p.HV * 128 + cc) = *reinterpret_cast<const uint4*>(tile + rr * 128 + cc);
+            }
+        }
+    } else if (warp < (MAIN + OUT + PROD) / 32) {
+        const int pt = tid - MAIN - OUT;
+        int c = 0;
+        for (; c < wk.nc; ++c) {
+            const int stage = c & 1;
+            unsigned char* b = dyn + stage * M::STAGE;
+            if (c > 1) ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((c >> 1) & 1) ^ 1, p, 1 << 17));
+            if (!ok) break;
+            const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+            const int rows = wk.rows(c);
+            if (pt == 0) {
+                mbar_expect_tx(&full[stage], 5 * M::MAT + AUX * 4);
+                tma_load_1d(b + M::TM, ws + lay.T + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
+                tma_load_1d(b + M::AU, ws + lay.aux + unit * AUX * 4, AUX * 4, &full[stage]);
+                tma_load_1d(b + M::AM, ws + lay.A + unit * 3 * M::MAT, 2 * M::MAT, &full[stage]);
+            }
+            __syncwarp();
+            const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
+            load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::KK), static_cast<const bf16*>(p.k) + krow, (size_t)p.H * K, rows, pt);
+            load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
+            load_tile<128, 128, PROD>(reinterpret_cast<bf16*>(b + M::V), static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
+                                      (size_t)p.HV * 128, rows, pt);
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        // given up: the records on their way land before the CTA's memory goes
+        for (int i = max(c - 2, 0); !ok && i < c; ++i) mbar_wait(&full[i & 1], (i >> 1) & 1, p, 1 << 17);
+    } else {
+        constexpr uint32_t id64 = make_idesc(128, 64, false, false), idu = make_idesc(128, DH, false, true);
+        for (int c = 0; c < wk.nc && ok; ++c) {
+            const int stage = c & 1, ph = c & 1;
+            const uint32_t b = smem_u32(dyn + stage * M::STAGE);
+            auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p, what));
+                tc_fence_after();
+                return ok;
+            };
+            if (!wait(&full[stage], (c >> 1) & 1, 1 << 18) || !wait(&sready, ph, 1 << 19)) break;
+            auto with_rows = [&](uint32_t acc, uint32_t rows_at, int parts) {  // S parts times rows, K-major
+#pragma unroll
+                for (int i = parts - 1; i >= 0; --i)
+#pragma unroll
+                    for (int s = 0; s < K / 16; ++s)
+                        mma_ts(tmem0 + acc, tmem0 + M::SP + (s / (DH / 16)) * M::HB + i * (DH / 2) + (s % (DH / 16)) * 8,
+                               make_desc(b + rows_at + s * 256, 128, K * 16), id64, i < parts - 1 || s > 0);
+            };
+            auto with_matrix = [&](uint32_t acc, uint32_t a, uint32_t as, uint32_t mat, int parts) {  // x M^T, M lower triangular
+                bool first = true;
+#pragma unroll
+                for (int o = parts - 1; o >= 0; --o)
+#pragma unroll
+                    for (int i = o; i >= 0; --i) {
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            mma_ts(tmem0 + acc + 16 * s, tmem0 + a + i * as + s * 8, make_desc(b + mat + (o - i) * M::MAT + s * 256 + s * 2048, 128, 1024),
+                                   make_idesc(128, 64 - 16 * s, false, false), !first || s > 0);
+                        first = false;
+                    }
+            };
+            if (elect_one()) {
+                with_rows(M::KS, M::KK, 3);
+                mma_commit(&ksbar);
+            }
+            __syncwarp();
+            if (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20)) break;
+            if (elect_one()) with_rows(M::QS, M::Q, 2);
+            __syncwarp();
+            if (!wait(&rready, ph, 1 << 21)) break;
+            if (elect_one()) {
+                with_matrix(M::KS, M::R, 32, M::TM, 3);
+                mma_commit(&vbar);
+            }
+            __syncwarp();
+            if (!wait(&wready, ph, 1 << 22)) break;
+            if (elect_one()) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int i = 2; i >= 0; --i)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + M::R + i * 32 + s * 8,
+                                   make_desc(b + M::KK + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu, i < 2 || s > 0);
+                mma_commit(&sibar);
+                with_matrix(M::AV, M::VP, M::VPS, M::AM, 2);
+                mma_commit(&obar);
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem0, 512);
+}
+
+// ---- backward: dS^T in registers, from the last chunk to the first -------------------------------------------------------
+//   dV'^T = e^(G_last-G) / |k| dS^T k^T + do^T A      Y^T = dV'^T T      X^T = -beta e^G / |k| Y^T      dv = beta Y
+//   dS^T <- e^G_last dS^T + (scale e^G / |q| do)^T q + X^T k
+// The products with do only are issued beside the chain dS - dS k - dV' - dV' T - X - X k - dS.
+namespace bt {
+using ft::MAIN;
+using ft::OUT;
+using ft::PROD;
+using ft::NTHR;
+template <int K>
+struct Map {
+    static constexpr int DH = K / 2;
+    static constexpr uint32_t ROWS = C * K * 2, MAT = SQ * 2;
+    static constexpr uint32_t KK = 0, Q = ROWS, DO = 2 * ROWS, TM = DO + C * 256, AM = TM + 3 * MAT, AU = AM + 3 * MAT, STAGE = AU + AUX * 4;
+    static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
+    // tensor memory: the parts of dS, over them the update; of the scaled do; of dV', over them X; dS k^T, over it Y; do^T A
+    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, DOS = 2 * HB, DV = DOS + 96, KD = DV + 96, AD = KD + 64, COLS = AD + 64;
+    static_assert(COLS <= 512 && TOTAL <= 232448 && STAGE % 1024 == 0, "fits");
+};
+}  // namespace bt
+
+template <int K>
+__global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
+    using namespace bt;
+    using M = Map<K>;
+    constexpr int DH = M::DH;
+    extern __shared__ __align__(1024) unsigned char dyn[];
+    __shared__ uint64_t full[2], empty[2], sready, kdbar, dosready, dvready, ybar, xready, sibar, ofree;
+    __shared__ uint32_t tmem_s;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (warp == 0) {
+        tmem_alloc(&tmem_s, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&full[i], 1 + PROD / 32);
+            mbar_init(&empty[i], (MAIN + OUT) / 32);
+        }
+        mbar_init(&sready, MAIN / 32);
+        mbar_init(&dosready, MAIN / 32);
+        mbar_init(&dvready, MAIN / 32);
+        mbar_init(&xready, MAIN / 32);
+        mbar_init(&kdbar, 1);
+        mbar_init(&ybar, 1);
+        mbar_init(&sibar, 1);
+        mbar_init(&ofree, OUT / 32);
+        mbar_fence_init();
+    }
+    pdl_wait();
+    Walk wk;
+    wk.h = blockIdx.x % p.HV; wk.n = blockIdx.x / p.HV; wk.kh = wk.h / (p.HV / p.H);
+    seq_chunks(p, wk.n, wk.c0, wk.nc);
+    seq_tokens(p, wk.n, wk.tok_begin, wk.tok_end);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem0 = tmem_s;
+    const char* ws = static_cast<const char*>(p.workspace);
+    char* sc = static_cast<char*>(p.bwd_scratch);
+    bool ok = true;
+
+    // step i is chunk nc - 1 - i
+    if (warp < MAIN / 32) {
+        const int e = tid & 127, half = warp >> 2, d0 = half * DH, t0 = half * 32;
+        const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
+        const size_t sbase = (size_t)(wk.n * (size_t)p.HV + wk.h) * K * 128;
+        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST;
+        float S[DH];
+#pragma unroll
+        for (int j = 0; j < DH; j += 4) {
+            if (!p.grad_ht) {
+                S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
+            } else if (vf) {
+                const float4 x = *reinterpret_cast<const float4*>(p.grad_ht + sbase + (size_t)e * K + d0 + j);
+                S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[j + i] = p.grad_ht[sbase + (size_t)(d0 + j + i) * 128 + e];
+            }
+        }
+        for (int i = 0; i < wk.nc; ++i) {
+            const int c = wk.nc - 1 - i, stage = i & 1, ph = i & 1;
+            const unsigned char* b = dyn + stage * M::STAGE;
+            const float* aux = reinterpret_cast<const float*>(b + M::AU);
+            const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+#pragma unroll
+            for (int g = 0; g < DH / 16; ++g) {
+                float x[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) x[j] = S[16 * g + j];
+                st_parts<3>(tm + M::SP + half * M::HB + 8 * g, DH / 2, x);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sready);
+            // ---- scaled rows of do
+            ok = mbar_wait(&full[stage], (i >> 1) & 1, p, 1 << 12) && ok;
+            const float last = aux[A_LAST * C];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[16];
+                load16(aux + A_OQ * C + t0 + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] *= __bfloat162float(reinterpret_cast<const bf16*>(b + M::DO)[swz_bf16(t0 + 16 * g + j, e)]);
+                st_parts<3>(tm + M::DOS + half * 16 + 8 * g, 32, f);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&dosready);
+            {
+                float* dS = reinterpret_cast<float*>(sc + lay.dS) + unit * K * 128;
+#pragma unroll
+                for (int j = 0; j < DH; ++j) dS[(size_t)(d0 + j) * 128 + e] = S[j];
+            }
+            // ---- dV'
+            ok = mbar_wait(&kdbar, ph, p, 1 << 13) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            uint32_t r[2][16];
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[16];
+                tmem_ld16(tm + M::KD + t0 + 16 * g, r[0]);
+                tmem_ld16(tm + M::AD + t0 + 16 * g, r[1]);
+                load16(aux + A_FK * C + t0 + 16 * g, f);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] = fmaf(f[j], __uint_as_float(r[0][j]), __uint_as_float(r[1][j]));
+                st_parts<3>(tm + M::DV + half * 16 + 8 * g, 32, f);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&dvready);
+            // ---- X
+            ok = mbar_wait(&ybar, ph, p, 1 << 14) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            tmem_ld16(tm + M::KD + t0, r[0]);
+            tmem_ld16(tm + M::KD + t0 + 16, r[1]);
+            tmem_wait_ld();
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                float f[16];
+                load16(aux + A_BGK * C + t0 + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) f[j] *= -__uint_as_float(r[g][j]);
+                st_parts<3>(tm + M::DV + half * 16 + 8 * g, 32, f);
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&xready);
+            // ---- dS at the start of the chunk
+            ok = mbar_wait(&sibar, ph, p, 1 << 15) && ok;
+            if (!__all_sync(0xffffffffu, ok)) break;
+            tc_fence_after();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+#pragma unroll
+            for (int g = 0; g < DH / 16; g += 2) {
+                tmem_ld16(tm + M::SP + half * M::HB + 16 * g, r[0]);
+                tmem_ld16(tm + M::SP + half * M::HB + 16 * g + 16, r[1]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) S[16 * (g + x) + j] = fmaf(last, S[16 * (g + x) + j], __uint_as_float(r[x][j]));
+            }
+        }
+        if (p.grad_h0 && ok) {
+#pragma unroll
+            for (int j = 0; j < DH; ++j) p.grad_h0[sbase + (vf ? (size_t)e * K + d0 + j : (size_t)(d0 + j) * 128 + e)] = S[j];
+        }
+    } else if (warp < (MAIN + OUT) / 32) {
+        const int e = tid & 127;
+        const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
+        bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
+        for (int i = 0; i < wk.nc; ++i) {
+            const int c = wk.nc - 1 - i, stage = i & 1;
+            const float* be = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_BETA * C;
+            const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+            ok = mbar_wait(&ybar, i & 1, p, 1 << 16) && ok;
+            ok = bar_and(2, OUT, ok);
+            if (!ok) break;
+            tc_fence_after();
+            uint32_t y[C / 16][16];
+#pragma unroll
+            for (int g = 0; g < C / 16; ++g) tmem_ld16(tm + M::KD + 16 * g, y[g]);
+            tmem_wait_ld();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ofree);
+            float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128 + e;
+#pragma unroll
+            for (int g = 0; g < C / 16; ++g) {
+                float f[16];
+                load16(be + 16 * g, f);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float v = __uint_as_float(y[g][j]);
+                    Y[(16 * g + j) * 128] = v;
+                    tile[(16 * g + j) * 128 + e] = __float2bfloat16_rn(f[j] * v);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[stage]);
+            bar_sync(2, OUT);
+            const int rows = wk.rows(c);
+            bf16* dst = static_cast<bf16*>(p.grad_v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
+#pragma unroll
+            for (int x = e; x < C * 16; x += OUT) {
+                const int rr = x >> 4, cc = (x & 15) * 8;
+                if (rr < rows) *reinterpret_cast<uint4*>(dst + (size_t)rr * p.HV * 128 + cc) = *reinterpret_cast<const uint4*>(tile + rr * 128 + cc);
+            }
+        }
+    } else if (warp < (MAIN + OUT + PROD) / 32) {
+        const int pt = tid - MAIN - OUT;
+        int i = 0;
+        for (; i < wk.nc; ++i) {
+            const int c = wk.nc - 1 - i, stage = i & 1;
+            unsigned char* b = dyn + stage * M::STAGE;
+            if (i > 1) ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((i >> 1) & 1) ^ 1, p, 1 << 17));
+            if (!ok) break;
+            const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+            const int rows = wk.rows(c);
+            if (pt == 0) {
+                mbar_expect_tx(&full[stage], 6 * M::MAT + AUX * 4);
+                tma_load_1d(b + M::AM, ws + lay.A + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
+                tma_load_1d(b + M::AU, ws + lay.aux + unit * AUX * 4, AUX * 4, &full[stage]);
+                tma_load_1d(b + M::TM, ws + lay.T + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
+            }
+            __syncwarp();
+            const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
+            load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::KK), static_cast<const bf16*>(p.k) + krow, (size_t)p.H * K, rows, pt);
+            load_swz<PROD>(reinterpret_cast<bf16*>(b + M::DO), static_cast<const bf16*>(p.grad_o) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
+                           (size_t)p.HV * 128, rows, pt);
+            load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[stage]);
+        }
+        for (int x = max(i - 2, 0); !ok && x < i; ++x) mbar_wait(&full[x & 1], (x >> 1) & 1, p, 1 << 17);
+    } else {
+        constexpr uint32_t id64 = make_idesc(128, 64, false, false), idu = make_idesc(128, DH, false, true);
+        for (int i = 0; i < wk.nc && ok; ++i) {
+            const int stage = i & 1, ph = i & 1;
+            const uint32_t b = smem_u32(dyn + stage * M::STAGE);
+            auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
+                ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p, what));
+                tc_fence_after();
+                return ok;
+            };
+            // columns j of x M for lower triangular M: block s of the inner index reaches columns up to 16 (s + 1)
+            auto update = [&](uint32_t parts_at, uint32_t rows_at, bool first) {  // update (+)= parts times rows
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int x = 2; x >= 0; --x)
+#pragma unroll
+                        for (int s = 0; s < 4; ++s)
+                            mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + parts_at + x * 32 + s * 8,
+                                   make_desc(b + rows_at + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu,
+                                   !first || x < 2 || s > 0);
+            };
+            if (!wait(&full[stage], (i >> 1) & 1, 1 << 18)) break;
+            if (elect_one()) {  // (the accumulator's last reader has arrived at dvready of the chunk before)
+#pragma unroll
+                for (int x = 2; x >= 0; --x)
+#pragma unroll
+                    for (int s = 3; s >= 0; --s)
+                        mma_ss(tmem0 + M::AD, make_desc_sw128(b + M::DO + s * 2048, 8192, 1024),
+                               make_desc(b + M::AM + x * M::MAT + s * 2048, 1024, 128), make_idesc(128, 16 * (s + 1), true, true), x < 2 || s < 3);
+            }
+            __syncwarp();
+            if (!wait(&sready, ph, 1 << 19) || (i > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
+            if (elect_one()) {
+#pragma unroll
+                for (int x = 2; x >= 0; --x)
+#pragma unroll
+                    for (int s = 0; s < K / 16; ++s)
+                        mma_ts(tmem0 + M::KD, tmem0 + M::SP + (s / (DH / 16)) * M::HB + x * (DH / 2) + (s % (DH / 16)) * 8,
+                               make_desc(b + M::KK + s * 256, 128, K * 16), id64, x < 2 || s > 0);
+                mma_commit(&kdbar);
+            }
+            __syncwarp();
+            if (!wait(&dosready, ph, 1 << 21) || !wait(&kdbar, ph, 1 << 22)) break;
+            if (elect_one()) update(M::DOS, M::Q, true);
+            __syncwarp();
+            if (!wait(&dvready, ph, 1 << 23)) break;
+            if (elect_one()) {
+                bool first = true;
+#pragma unroll
+                for (int o = 2; o >= 0; --o)
+#pragma unroll
+                    for (int x = o; x >= 0; --x) {
+#pragma unroll
+                        for (int s = 3; s >= 0; --s)
+                            mma_ts(tmem0 + M::KD, tmem0 + M::DV + x * 32 + s * 8, make_desc(b + M::TM + (o - x) * M::MAT + s * 2048, 1024, 128),
+                                   make_idesc(128, 16 * (s + 1), false, true), !first || s < 3);
+                        first = false;
+                    }
+                mma_commit(&ybar);
+            }
+            __syncwarp();
+            if (!wait(&xready, ph, 1 << 24)) break;
+            if (elect_one()) {
+                update(M::DV, M::KK, false);
+                mma_commit(&sibar);
+            }
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 0) tmem_dealloc(tmem0, 512);
+}
+
+template <int K, bool SAVE>
+static cudaError_t launch(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    constexpr int bytes = ft::Map<K>::TOTAL;
+    cudaError_t e = allow_smem(gdr_fwd_tc_kernel<K, SAVE>, bytes);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(gdr_fwd_tc_kernel<K, SAVE>, p.N * p.HV, ft::NTHR, bytes, s, p, l);
+}
+
+template <int K>
+static cudaError_t launch_bwd(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    constexpr int bytes = bt::Map<K>::TOTAL;
+    cudaError_t e = allow_smem(gdr_bwd_tc_kernel<K>, bytes);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(gdr_bwd_tc_kernel<K>, p.N * p.HV, bt::NTHR, bytes, s, p, l);
+}
+
+cudaError_t bwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) { return p.dk == 64 ? launch_bwd<64>(p, l, s) : launch_bwd<128>(p, l, s); }
+
+cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    const bool save = !(p.flags & KDA_FLAG_NO_SAVE);
+    if (p.dk == 64) return save ? launch<64, true>(p, l, s) : launch<64, false>(p, l, s);
+    return save ? launch<128, true>(p, l, s) : launch<128, false>(p, l, s);
+}
+
+}  // namespace gdr
+}  // namespace kda

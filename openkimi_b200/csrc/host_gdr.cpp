@@ -90,6 +90,9 @@ KdaGdrParams params(const Inputs& in, const Spec& sp, int flags) {
         p.cu_seqlens = ptr<int64_t>(in.cu); p.chunk_seq = ptr<int32_t>(in.chunk_seq);
         p.seq_chunk_off = ptr<int32_t>(in.seq_off); p.chunk_tab = ptr<int32_t>(in.chunk_tab);
     }
+    const StatusWord& st = status_word(in.q.device().index());
+    p.status = st.dev.load(std::memory_order_relaxed);
+    p.status_host = const_cast<int32_t*>(st.host);
     return p;
 }
 Tensor state_like(const Inputs& in, const Spec& sp) {
