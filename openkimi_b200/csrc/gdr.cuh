@@ -22,8 +22,8 @@ constexpr int BLK = 256;           // elements of one
 constexpr int TRI = NBLK * BLK;    // elements of one part of such a matrix
 constexpr int AUX = 12 * C;        // floats of a unit's per-row numbers
 // e^G, e^(G_last - G), beta, 1/|q|, 1/|k|, G in two floats, [A_LAST][0] = e^G_last; and the factors that the walks use:
-// beta e^G / |k|, e^(G_last - G) / |k|, scale e^G / |q|
-enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST, A_BGK, A_FK, A_OQ };
+// beta e^G / |k|, e^(G_last - G) / |k|, scale e^G / |q|, e^G / |k|
+enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST, A_BGK, A_FK, A_OQ, A_GK };
 constexpr int SQ = C * C;          // elements of one part of a 64 x 64 matrix in core-matrix order (cm_idx)
 // BF16 with 128 value columns walks the chunks on tcgen05; T and A are then whole matrices in core-matrix order
 __host__ __device__ __forceinline__ bool on_tc(const KdaGdrParams& p) { return p.dtype == KDA_DTYPE_BF16 && p.dv == 128; }
@@ -33,8 +33,8 @@ __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I *
 
 // per (chunk, value head) unit, byte offsets
 struct Layout {
-    size_t aux, T, A, total_nosave, S0, Vn, total;        // workspace
-    size_t dS, Y, part, dqk, bwd_total;                   // backward scratch
+    size_t aux, T, A, total_nosave, S0, Vn, Tb, total;    // workspace
+    size_t dS, Y, part, yv, dqk, bwd_total;               // backward scratch
 };
 __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     const size_t n = (size_t)p.NT * p.HV, mat = 3 * (on_tc(p) ? SQ : TRI) * 2;
@@ -42,21 +42,29 @@ __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     size_t off = 0;
     l.aux = off; off = align256(off + n * AUX * 4);
     // (I + diag(beta) L)^-1 and scale (q k^T) D as three BF16 parts: blocks of the lower triangle in blk() order, rows swizzled as
-    // tri_frag reads them, or (on_tc) [64][64] in core-matrix order of which only those blocks are written
+    // tri_frag reads them; or (on_tc) [64][64] in core-matrix order of which only those blocks are written, the columns of T times
+    // beta, and T itself for the backward
     l.T = off;   off = align256(off + n * mat);
     l.A = off;   off = align256(off + n * mat);
     l.total_nosave = off;
-    l.S0 = off;  off = align256(off + n * p.dk * p.dv * 4);  // state at the chunk's start [dk][dv]
-    l.Vn = off;  off = align256(off + n * C * p.dv * 4);     // V' [64][dv]
+    // state at the chunk's start [dk][dv] and V' [64][dv], on_tc in the order of rec_idx()
+    l.S0 = off;  off = align256(off + n * p.dk * p.dv * 4);
+    l.Vn = off;  off = align256(off + n * C * p.dv * 4);
+    l.Tb = off;  if (on_tc(p)) off = align256(off + n * mat);
     l.total = off;
     off = 0;
-    l.dS = off;   off = align256(off + n * p.dk * p.dv * 4); // gradient of the state at the chunk's end
-    l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV'
+    l.dS = off;   off = align256(off + n * p.dk * p.dv * 4); // gradient of the state at the chunk's end, as S0
+    l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV', as V'
     l.part = off; off = align256(off + n * 2 * 4);           // this unit's share of dA_log and ddt_bias
+    l.yv = off;   if (on_tc(p)) off = align256(off + n * C * 4);  // row sums of Y v
     l.dqk = off;  if (p.HV != p.H) off = align256(off + n * 2 * C * p.dk * 4);  // shared key heads: this value head's share of dq, dk
     l.bwd_total = off;
     return l;
 }
+
+// Records of the transposed walks: FP32 [128 value columns][cols], 16 value columns at a time, each [16][cols] in core-matrix order:
+// what one K-step of a product over the value columns reads lies together, eight consecutive columns as one piece of 32 bytes.
+__host__ __device__ __forceinline__ int rec_idx(int e, int col, int cols) { return (e >> 4) * 16 * cols + cm_idx(e & 15, col, cols); }
 
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -118,8 +126,11 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&w)[P]) {
     for (int i = 0; i < P; ++i) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
-        x0 -= __uint_as_float(w[i] << 16);
-        x1 -= __uint_as_float(w[i] & 0xffff0000u);
+        if (i + 1 < P) {  // (packed: x - p)
+const float2 r = __ffma2_rn(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), make_float2(-1.f, -1.f), make_float2(x0, x1));
+            x0 = r.x;
+            x1 = r.y;
+        }
     }
 }
 // two neighbouring elements into the P part tiles at element offset idx
@@ -176,6 +187,19 @@ __device__ __forceinline__ void load_tile(bf16* dst, const float* src, size_t st
         put4<3>(dst, C * LD, r * LD + c, x);
     }
 }
+// rows of COLS elements, `stride` apart in memory, into core-matrix order; lanes take 8 rows x 4 chunks of 16 bytes at a time
+template <int COLS, int NTHR>
+__device__ __forceinline__ void load_cm(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
+    constexpr int CG = COLS / 32;
+    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
+#pragma unroll 4
+    for (int i = tid >> 5; i < 8 * CG; i += NTHR / 32) {
+        const int rr = i / CG * 8 + r, cc = (i % CG * 4 + c) * 8;
+        const bool in = rr < rows;
+        cp_async16_z(dst + cm_idx(rr, cc, COLS), src + (in ? rr * stride + cc : 0), in);
+    }
+}
+
 // `count` 16-byte words
 template <int NTHR>
 __device__ __forceinline__ void load_words(bf16* dst, const bf16* src, int count, int tid) {

@@ -16,7 +16,7 @@ static int sizes_ok(const KdaGdrParams& p) {
     if (p.B <= 0 || p.T <= 0 || p.H <= 0 || p.HV <= 0 || p.HV % p.H || p.N <= 0 || p.NT <= 0) return KDA_ERR_SHAPE;
     if ((p.dk != 64 && p.dk != 128) || (p.dv != 64 && p.dv != 128)) return KDA_ERR_SHAPE;
     // grids are one-dimensional, and a state panel has at least 16 of the 64 or 128 columns
-    if ((long long)p.NT * p.HV > 0x7fffffffLL || (long long)p.N * p.HV > 0x7fffffffLL / 8) return KDA_ERR_SHAPE;
+    if ((long long)p.NT * p.HV > 0x7fffffffLL / 2 || (long long)p.N * p.HV > 0x7fffffffLL / 8) return KDA_ERR_SHAPE;
     return KDA_OK;
 }
 

@@ -12,13 +12,13 @@
 //
 // One CTA of eight warps per (chunk, value head): warp w has rows 16 (w mod 4).. and half w / 4 of the columns of every product.
 // The value columns come in panels of 32, as three BF16 parts each of S0, dS, Y, V'.
-#include "gdr.cuh"
+#include "gdr_grad.cuh"
 
 namespace kda {
 namespace gdr {
 
 namespace gr {
-constexpr int NTHR = 256, EP = 32, LDE = EP + 8, PAN = C * LDE, LDZ = C + 8;
+constexpr int NTHR = 256, EP = 32, LDE = EP + 8, PAN = C * LDE;
 }
 
 template <typename T, int K>
@@ -36,15 +36,13 @@ template <typename T, int K>
 __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, const Layout lay) {
     using namespace gr;
     using M = GradMap<T, K>;
-    constexpr int P = M::P, PO = M::PO, LDK = M::LDK, NK = K / 16;  // NK column tiles of a warp's half of K
+    constexpr int P = M::P, LDK = M::LDK, NK = K / 16;  // NK column tiles of a warp's half of K
     extern __shared__ __align__(16) unsigned char smem[];
     bf16* sm = reinterpret_cast<bf16*>(smem);
     const uint32_t sa = smem_u32(sm);
     float* sx = reinterpret_cast<float*>(smem + 2 * M::END);
-    float *gam = sx, *fall = sx + C, *be = sx + 2 * C, *rq = sx + 3 * C, *rk = sx + 4 * C, *ghi = sx + 5 * C, *glo = sx + 6 * C;
-    float* red = sx + 7 * C;   // [16][C]: row sums N (2 halves), dL KKD (2), q.F (2), k.E (2), k.H (2), Y.v (1), column sums (4), spare
-    enum { R_N = 0, R_B = 2, R_F = 4, R_E = 6, R_H = 8, R_Y = 10, R_COL = 11, R_X = 15 };
-    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3, rb = w & 3, half = w >> 2;
+    float* red = sx + 7 * C;   // [RED] sums, then the warps' shares of <S0, dS>
+    const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, rb = w & 3, half = w >> 2;
     const int c = blockIdx.x / p.HV, h = blockIdx.x % p.HV, grp = p.HV / p.H, kh = h / grp;
     const size_t unit = blockIdx.x;
     pdl_wait();
@@ -57,7 +55,8 @@ __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, con
     cp_async_commit();
     const float* aux = reinterpret_cast<const float*>(ws + lay.aux) + unit * AUX;
     for (int i = tid; i < 7 * C; i += NTHR) sx[i] = aux[i];
-    const float last = aux[A_LAST * C];
+    const GradRows<T, K> m = {sm + M::Q, sm + M::KK, sa + 2 * M::Q, sa + 2 * M::KK, sm + M::Z, sm + M::X, sa + 2 * M::Z, sa + 2 * M::X,
+                              sx, sx + C, sx + 2 * C, sx + 3 * C, sx + 4 * C, sx + 5 * C, sx + 6 * C, red, aux[A_LAST * C]};
 
     float F[NK][4], E[NK][4], H[NK][4], dA[4][4], dL[4][4];
 #pragma unroll
@@ -140,30 +139,8 @@ __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, con
             }
         }
     }
-    // q k^T, k k^T again
     float qk[4][4], kk[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) qk[j][i] = kk[j][i] = 0.f;
-#pragma unroll 1
-    for (int d = 0; d < K; d += 16) {
-        uint32_t fq[P][4], fk[P][4];
-#pragma unroll
-        for (int i = 0; i < P; ++i) {
-            a_frag<LDK>(fq[i], sa + 2 * (M::Q + i * M::ROWS), 16 * rb, d, lane);
-            a_frag<LDK>(fk[i], sa + 2 * (M::KK + i * M::ROWS), 16 * rb, d, lane);
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            if (2 * half + j > rb) break;
-            uint32_t b[P][4];
-#pragma unroll
-            for (int i = 0; i < P; ++i) b_frag<LDK>(b[i], sa + 2 * (M::KK + i * M::ROWS), 32 * half + 16 * j, d, lane);
-            mma_parts<P, P, P>(qk, j, fq, b);
-            mma_parts<P, P, P>(kk, j, fk, b);
-        }
-    }
+    grad_rows_products(m, rb, half, lane, qk, kk);
     // Y . v: eight lanes have a row
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -172,220 +149,13 @@ __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, con
         if ((tid & 7) == 0) red[R_Y * C + pr + 32 * i] = yv[i];
     }
     ss = warp_sum(ss);
-    if (lane == 0) red[R_X * C + w] = ss;
+    if (lane == 0) red[RED * C + w] = ss;
     __syncthreads();  // the panels have been used
-    const int r0 = 16 * rb + g;
-    float rn[2] = {0.f, 0.f}, rbeta[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (2 * half + j / 2 > rb) break;
-        float col[2] = {0.f, 0.f};
-        const int j0 = 32 * half + 8 * j + 2 * t;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i;
-            float z[2], x[2];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int cc = j0 + y;
-                const float d = r >= cc ? expf(ghi[r] - ghi[cc] + (glo[r] - glo[cc])) : 0.f;
-                const float a = r >= cc ? dA[j][2 * i + y] * p.scale * d * rq[r] * rk[cc] : 0.f;
-                const float kkd = rk[r] * rk[cc] * d, l = r > cc ? -dL[j][2 * i + y] * kkd : 0.f;
-                z[y] = a;
-                x[y] = l * be[r];
-                const float lk = l * kk[j][2 * i + y];
-                const float nn = r > cc ? fmaf(a, qk[j][2 * i + y], be[r] * lk) : 0.f;
-                rn[i] += nn;
-                rbeta[i] += r > cc ? lk : 0.f;
-                col[y] += nn;
-            }
-            put<PO>(sm + M::Z, C * LDZ, r * LDZ + j0, z[0], z[1]);
-            put<PO>(sm + M::X, C * LDZ, r * LDZ + j0, x[0], x[1]);
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) col[y] += __shfl_xor_sync(0xffffffffu, col[y], o);
-            if (g == 0) red[(R_COL + rb) * C + j0 + y] = col[y];
-        }
-    }
-    // this half's share of the row sums; scale the products with the states to the rows' units
-    float rf[2] = {0.f, 0.f}, re[2] = {0.f, 0.f}, rh[2] = {0.f, 0.f};
-#pragma unroll
-    for (int j = 0; j < NK; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i, d = half * (K / 2) + 8 * j + 2 * t;
-            const float2 q = get2<P>(sm + M::Q, M::ROWS, r * LDK + d), k = get2<P>(sm + M::KK, M::ROWS, r * LDK + d);
-            const float ff = p.scale * gam[r] * rq[r], fe = gam[r] * rk[r], fh = fall[r] * rk[r];
-            float &f0 = F[j][2 * i], &f1 = F[j][2 * i + 1];
-            f0 *= ff; f1 *= ff;
-            const float e0 = E[j][2 * i] * fe, e1 = E[j][2 * i + 1] * fe, h0 = H[j][2 * i] * fh, h1 = H[j][2 * i + 1] * fh;
-            rf[i] += q.x * f0 + q.y * f1;
-            re[i] += k.x * e0 + k.y * e1;
-            rh[i] += k.x * h0 + k.y * h1;
-            E[j][2 * i] = h0 - be[r] * e0;
-            E[j][2 * i + 1] = h1 - be[r] * e1;
-        }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-        for (int o = 1; o < 4; o <<= 1) {
-            rn[i] += __shfl_xor_sync(0xffffffffu, rn[i], o);
-            rbeta[i] += __shfl_xor_sync(0xffffffffu, rbeta[i], o);
-            rf[i] += __shfl_xor_sync(0xffffffffu, rf[i], o);
-            re[i] += __shfl_xor_sync(0xffffffffu, re[i], o);
-            rh[i] += __shfl_xor_sync(0xffffffffu, rh[i], o);
-        }
-        if (t == 0) {
-            const int r = r0 + 8 * i;
-            red[(R_N + half) * C + r] = rn[i];
-            red[(R_B + half) * C + r] = rbeta[i];
-            red[(R_F + half) * C + r] = rf[i];
-            red[(R_E + half) * C + r] = re[i];
-            red[(R_H + half) * C + r] = rh[i];
-        }
-    }
-    __syncthreads();  // Z, X and the sums are there
-    // dq (in F) and dk (in E) of 16 rows and this half of the channels
-#pragma unroll
-    for (int b = 0; b < 4; ++b) {
-        uint32_t fz[PO][4], fx[PO][4], zt[PO][4], xt[PO][4];
-#pragma unroll
-        for (int i = 0; i < PO; ++i) {
-            if (b <= rb) {
-                a_frag<LDZ>(fz[i], sa + 2 * (M::Z + i * C * LDZ), 16 * rb, 16 * b, lane);
-                a_frag<LDZ>(fx[i], sa + 2 * (M::X + i * C * LDZ), 16 * rb, 16 * b, lane);
-            }
-            if (b >= rb) {
-                a_frag_t<LDZ>(zt[i], sa + 2 * (M::Z + i * C * LDZ), 16 * rb, 16 * b, lane);
-                a_frag_t<LDZ>(xt[i], sa + 2 * (M::X + i * C * LDZ), 16 * rb, 16 * b, lane);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < NK / 2; ++j) {
-            uint32_t bk[P][4], bq[P][4];
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                b_frag_t<LDK>(bk[i], sa + 2 * (M::KK + i * M::ROWS), half * (K / 2) + 16 * j, 16 * b, lane);
-                b_frag_t<LDK>(bq[i], sa + 2 * (M::Q + i * M::ROWS), half * (K / 2) + 16 * j, 16 * b, lane);
-            }
-            if (b <= rb) {
-                mma_parts<PO, P, PO>(F, j, fz, bk);
-                mma_parts<PO, P, PO>(E, j, fx, bk);
-            }
-            if (b >= rb) {
-                mma_parts<PO, P, PO>(E, j, xt, bk);
-                mma_parts<PO, P, PO>(E, j, zt, bq);
-            }
-        }
-    }
-    if (w == 0) {  // the gate's and beta's gradients, two neighbouring rows per lane
-        float total = 0.f;
-        for (int i = 0; i < 8; ++i) total += red[R_X * C + i];
-        double dG[2], hsum = 0.0;
-        float db[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = 2 * lane + i, I = r >> 4;
-            float colsum = 0.f;
-            for (int x = I; x < 4; ++x) colsum += red[(R_COL + x) * C + r];
-            const float n = red[R_N * C + r] + red[(R_N + 1) * C + r], bb = red[R_B * C + r] + red[(R_B + 1) * C + r];
-            const float f = red[R_F * C + r] + red[(R_F + 1) * C + r], e = red[R_E * C + r] + red[(R_E + 1) * C + r],
-                        hh = red[R_H * C + r] + red[(R_H + 1) * C + r];
-            dG[i] = (double)n - colsum + f - (double)be[r] * e - hh;
-            hsum += hh;
-            db[i] = red[R_Y * C + r] - e + bb;
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
-        double run = dG[0] + dG[1];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double dn = __shfl_down_sync(0xffffffffu, run, o);
-            if (lane + o < 32) run += dn;
-        }
-        run += (double)last * total + hsum;
-        const double dg[2] = {run, run - dG[0]};
-        float dAl = 0.f, dbi = 0.f;
-        const float eA = (p.flags & KDA_FLAG_GATE) ? expf(p.A_log[h]) : 0.f, bias = (p.flags & KDA_FLAG_GATE) && p.dt_bias ? p.dt_bias[h] : 0.f;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = 2 * lane + i;
-            if (r < ci.len) {
-                const size_t at = (size_t)(ci.tok0 + r) * p.HV + h;
-                float d = (float)dg[i], b = db[i];
-                if (p.flags & KDA_FLAG_GATE) {
-                    const float a = load_g(p, p.g, at) + bias, sp = softplus_f(a);
-                    dAl += d * fmaxf(-eA * sp, G_MIN);
-                    d *= -eA * (a > 20.f ? 1.f : sigmoid_f(a));
-                    dbi += d;
-                }
-                if (p.flags & KDA_FLAG_BETA_SIGMOID) b *= be[r] * (1.f - be[r]);
-                store_g(p, p.grad_g, at, d);
-                store_g(p, p.grad_beta, at, b);
-            }
-        }
-        if (p.flags & KDA_FLAG_GATE) {
-            dAl = warp_sum(dAl);
-            dbi = warp_sum(dbi);
-            if (lane == 0) *reinterpret_cast<float2*>(static_cast<char*>(p.bwd_scratch) + lay.part + unit * 8) = make_float2(dAl, dbi);
-        }
-    }
-    if (grp > 1) {  // the group's value heads are added up by gdr_heads_kernel
-        float* out = reinterpret_cast<float*>(static_cast<char*>(p.bwd_scratch) + lay.dqk) + unit * 2 * C * K;
-#pragma unroll
-        for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int at = (r0 + 8 * i) * K + half * (K / 2) + 8 * j + 2 * t;
-                store2(out + at, F[j][2 * i], F[j][2 * i + 1]);
-                store2(out + C * K + at, E[j][2 * i], E[j][2 * i + 1]);
-            }
-        return;
-    }
-    float dot[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
-    if (p.flags & KDA_FLAG_QK_L2NORM) {
-#pragma unroll
-        for (int j = 0; j < NK; ++j)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int at = (r0 + 8 * i) * LDK + half * (K / 2) + 8 * j + 2 * t;
-                const float2 q = get2<P>(sm + M::Q, M::ROWS, at), k = get2<P>(sm + M::KK, M::ROWS, at);
-                dot[0][i] += q.x * F[j][2 * i] + q.y * F[j][2 * i + 1];
-                dot[1][i] += k.x * E[j][2 * i] + k.y * E[j][2 * i + 1];
-            }
-        __syncthreads();  // (the sums above have been read)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) dot[x][i] += __shfl_xor_sync(0xffffffffu, dot[x][i], o);
-                if (t == 0) red[(2 * x + half) * C + r0 + 8 * i] = dot[x][i];
-            }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = r0 + 8 * i;
-            // a row shorter than 1e-6 is divided by that, whatever its length
-            dot[0][i] = rq[r] < 1e6f ? rq[r] * rq[r] * (red[r] + red[C + r]) : 0.f;
-            dot[1][i] = rk[r] < 1e6f ? rk[r] * rk[r] * (red[2 * C + r] + red[3 * C + r]) : 0.f;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = r0 + 8 * i;
-        if (r >= ci.len) continue;
-#pragma unroll
-        for (int j = 0; j < NK; ++j) {
-            const int d = half * (K / 2) + 8 * j + 2 * t;
-            const float2 q = get2<P>(sm + M::Q, M::ROWS, r * LDK + d), k = get2<P>(sm + M::KK, M::ROWS, r * LDK + d);
-            const size_t at = (qrow + (size_t)r * p.H) * K + d;
-            store2(static_cast<T*>(p.grad_q) + at, F[j][2 * i] - q.x * dot[0][i], F[j][2 * i + 1] - q.y * dot[0][i]);
-            store2(static_cast<T*>(p.grad_k) + at, E[j][2 * i] - k.x * dot[1][i], E[j][2 * i + 1] - k.y * dot[1][i]);
-        }
-    }
+    grad_pairs(m, p.scale, rb, half, lane, dA, dL, qk, kk);
+    grad_scale(m, p.scale, rb, half, lane, F, E, H);
+    float total = 0.f;
+    for (int i = 0; i < 8; ++i) total += red[RED * C + i];
+    grad_finish(p, lay, m, ci, unit, h, kh, grp, total, F, E, w, lane, [] { __syncthreads(); });
 }
 
 // dq and dk of shared key heads: the shares of a group's value heads in their order, then the gradient of the L2 norm.  A warp per
@@ -457,12 +227,19 @@ __global__ void __launch_bounds__(256) gdr_param_kernel(const KdaGdrParams p, co
     }
 }
 
+cudaError_t grad_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s);  // gdr_grad_tc.cu
+
 template <typename T, int K>
 static cudaError_t launch_grad(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
     constexpr int bytes = GradMap<T, K>::BYTES;
     static_assert(bytes <= 232448, "shared memory");
-    cudaError_t e = allow_smem(gdr_grad_kernel<T, K>, bytes);
-    if (e == cudaSuccess) e = launch_dependent(gdr_grad_kernel<T, K>, p.NT * p.HV, gr::NTHR, bytes, s, p, l);
+    cudaError_t e = cudaSuccess;
+    if (on_tc(p)) {
+        e = grad_tc(p, l, s);
+    } else {
+        e = allow_smem(gdr_grad_kernel<T, K>, bytes);
+        if (e == cudaSuccess) e = launch_dependent(gdr_grad_kernel<T, K>, p.NT * p.HV, gr::NTHR, bytes, s, p, l);
+    }
     if (e == cudaSuccess && p.HV != p.H) e = launch_dependent(gdr_heads_kernel<T, K>, p.NT * p.H, 256, 0, s, p, l);
     if (e == cudaSuccess && (p.flags & KDA_FLAG_GATE)) e = launch_dependent(gdr_param_kernel, p.HV, 256, 0, s, p, l);
     return e;

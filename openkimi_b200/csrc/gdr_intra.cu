@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
                 aux[A_BGK * C + r] = be[i] * gam * rk[r];
                 aux[A_FK * C + r] = fall * rk[r];
                 aux[A_OQ * C + r] = p.scale * gam * rq[r];
+                aux[A_GK * C + r] = gam * rk[r];
                 aux[A_BETA * C + r] = be[i];
                 aux[A_RQ * C + r] = rq[r];
                 aux[A_RK * C + r] = rk[r];
@@ -192,7 +193,13 @@ __global__ void __launch_bounds__(128) gdr_intra_kernel(const KdaGdrParams p, co
             const int b = i >> 7, r = (i >> 3) & 15, cc = (i & 7) * 2;
             const int I = b < 1 ? 0 : b < 3 ? 1 : b < 6 ? 2 : 3, J = b - blk(I, 0);
             const float2 x = *reinterpret_cast<const float2*>(L + (16 * I + r) * LDL + 16 * J + cc);
-            put<3>(Tm, PART, CM ? cm_idx(16 * I + r, 16 * J + cc, C) : b * BLK + tri_idx(r, cc), x.x, x.y);
+            if (CM) {
+                const int at = cm_idx(16 * I + r, 16 * J + cc, C);
+                put<3>(Tm, PART, at, x.x * sb[16 * J + cc], x.y * sb[16 * J + cc + 1]);
+                if (!(p.flags & KDA_FLAG_NO_SAVE)) put<3>(reinterpret_cast<bf16*>(static_cast<char*>(p.workspace) + lay.Tb) + unit * 3 * PART, PART, at, x.x, x.y);
+            } else {
+                put<3>(Tm, PART, b * BLK + tri_idx(r, cc), x.x, x.y);
+            }
         }
         __syncthreads();
     }

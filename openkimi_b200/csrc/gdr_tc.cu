@@ -1,8 +1,8 @@
 // Gated delta rule, the walks along the chunks on tcgen05 (BF16, 128 value columns; gdr_state.cu has the other sizes and FP32).
 //
 // One CTA per (sequence, value head).  Everything is transposed, value column e = TMEM lane e, so that the 128 lanes are full:
-//   P^T = S^T k^T    R^T = beta v^T - (beta e^G / |k|) P^T    V'^T = R^T T^T    W^T = e^(G_last-G) / |k| V'^T
-//   S^T <- e^G_last S^T + W^T k          o^T = scale e^G / |q| (S^T q^T) + V'^T A^T
+//   P^T = S^T k^T    R^T = -e^G / |k| P^T    V'^T = (v^T + R^T) T'^T    W^T = e^(G_last-G) / |k| V'^T          T' = T diag(beta)
+//   S^T <- e^G_last S^T + W^T k              o^T = scale e^G / |q| (S^T q^T) + V'^T A^T
 // The state stays in registers in FP32 (256 threads: lane e, half of the key channels).  A computed operand goes to tensor memory in
 // three BF16 parts and multiplies q, k, T, A from shared memory, where T and A have three parts too; products of the smallest
 // parts are accumulated first, so that the accumulator's truncation falls on small sums.  The update is accumulated from zero and
@@ -23,9 +23,9 @@ struct Map {
     static constexpr uint32_t KK = 0, Q = ROWS, V = 2 * ROWS, TM = V + C * 256, AM = TM + 3 * MAT, AU = AM + 2 * MAT, STAGE = AU + AUX * 4;
     static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
     // tensor memory columns.  S parts: per half three blocks of DH / 2; over them, once S k and S q are done, the update (DH columns)
-    // and, with K = 128, in the third block the parts of V'.  V' itself over S k, W over R.
+    // and, with K = 128, in the third block the parts of V'.  V' A^T over S k, W over R.
     static constexpr uint32_t SP = 0, HB = 3 * DH / 2, VPS = K == 128 ? HB : 32, VP = K == 128 ? DH : 2 * HB,
-                              KS = K == 128 ? 2 * HB : 2 * HB + 64, QS = KS + 64, AV = QS + 64, R = AV + 64, COLS = R + 96;
+                              KS = K == 128 ? 2 * HB : 2 * HB + 64, AV = KS, QS = KS + 64, VA = QS + 64, R = VA + 64, COLS = R + 96;
     static_assert(COLS <= 512 && TOTAL <= 232448, "fits");
 };
 }  // namespace ft
@@ -44,6 +44,16 @@ __device__ __forceinline__ void st_parts(uint32_t at, uint32_t stride, const flo
 #pragma unroll
     for (int i = 0; i < P; ++i) tmem_st8(at + i * stride, w[i]);
 }
+// N consecutive columns of a record's row (col a multiple of 8)
+template <int N>
+__device__ __forceinline__ void store_record(float* rec, int e, int col, int cols, const float* x) {
+#pragma unroll
+    for (int j = 0; j < N; j += 8) {
+        float4* at = reinterpret_cast<float4*>(rec + rec_idx(e, col + j, cols));
+        at[0] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        at[1] = make_float4(x[j + 4], x[j + 5], x[j + 6], x[j + 7]);
+    }
+}
 __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
@@ -51,20 +61,7 @@ __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
         x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
     }
 }
-// rows of COLS elements, `stride` apart in memory, into core-matrix order; lanes take 8 rows x 4 chunks of 16 bytes at a time
-template <int COLS, int NTHR>
-__device__ __forceinline__ void load_cm(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
-    constexpr int CG = COLS / 32;
-    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
-#pragma unroll 4
-    for (int i = tid >> 5; i < 8 * CG; i += NTHR / 32) {
-        const int rr = i / CG * 8 + r, cc = (i % CG * 4 + c) * 8;
-        const bool in = rr < rows;
-        cp_async16_z(dst + cm_idx(rr, cc, COLS), src + (in ? rr * stride + cc : 0), in);
-    }
-}
-
-// the same with rows of 128 elements into two halves of 64 with 128-byte swizzle (swz_bf16)
+// rows of 128 elements into two halves of 64 with 128-byte swizzle (swz_bf16)
 template <int NTHR>
 __device__ __forceinline__ void load_swz(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
     const int lane = tid & 31, r = lane & 7, c = lane >> 3;
@@ -73,6 +70,20 @@ __device__ __forceinline__ void load_swz(bf16* dst, const bf16* src, size_t stri
         const int rr = (i >> 2) * 8 + r, cc = ((i & 3) * 4 + c) * 8;
         const bool in = rr < rows;
         cp_async16_z(dst + swz_bf16(rr, cc), src + (in ? rr * stride + cc : 0), in);
+    }
+}
+
+// val[i] summed over the 32 lanes; lane l ends with values l M / 32 .. in val[0 .. M / 32)
+template <int M, int O = 16>
+__device__ __forceinline__ void lanes_total(float* val, int lane) {
+    if constexpr (O > 0) {
+        const bool up = lane & O;
+#pragma unroll
+        for (int i = 0; i < M / 2; ++i) {
+            const float keep = up ? val[M / 2 + i] : val[i], send = up ? val[i] : val[M / 2 + i];
+            val[i] = keep + __shfl_xor_sync(0xffffffffu, send, O);
+        }
+        lanes_total<M / 2, O / 2>(val, lane);
     }
 }
 
@@ -171,22 +182,10 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sready);
-            if (SAVE) {
-                float* S0 = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.S0) + unit * K * 128;
-#pragma unroll
-                for (int j = 0; j < DH; ++j) S0[(size_t)(d0 + j) * 128 + e] = S[j];
-            }
+            if (SAVE) store_record<DH>(reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.S0) + unit * K * 128, e, d0, K, S);
             // ---- R
             ok = mbar_wait(&full[stage], (c >> 1) & 1, p, 1 << 12) && ok;
             const float last = aux[A_LAST * C];
-            float x[2][16];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-                load16(aux + A_BETA * C + t0 + 16 * g, x[g]);
-#pragma unroll
-                for (int j = 0; j < 16; ++j)
-                    x[g][j] *= __bfloat162float(reinterpret_cast<const bf16*>(b + M::V)[(t0 + 16 * g + j) * 128 + e]);
-            }
             ok = mbar_wait(&ksbar, ph, p, 1 << 13) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
@@ -197,10 +196,10 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 float f[16];
-                load16(aux + A_BGK * C + t0 + 16 * g, f);
+                load16(aux + A_GK * C + t0 + 16 * g, f);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) x[g][j] = fmaf(-f[j], __uint_as_float(r[g][j]), x[g][j]);
-                st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, x[g]);
+                for (int j = 0; j < 16; ++j) f[j] *= -__uint_as_float(r[g][j]);
+                st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, f);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -210,9 +209,10 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             ok = mbar_wait(&vbar, ph, p, 1 << 14) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            tmem_ld16(tm + M::KS + t0, r[0]);
-            tmem_ld16(tm + M::KS + t0 + 16, r[1]);
+            tmem_ld16(tm + M::VA + t0, r[0]);
+            tmem_ld16(tm + M::VA + t0 + 16, r[1]);
             tmem_wait_ld();
+            float x[2][16];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 float f[16];
@@ -232,9 +232,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             if (SAVE) {
                 float* V = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.Vn) + unit * C * 128;
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) V[(t0 + 16 * g + j) * 128 + e] = x[g][j];
+                for (int g = 0; g < 2; ++g) store_record<16>(V, e, t0 + 16 * g, C, x[g]);
             }
             // ---- the state at the end of the chunk
             ok = mbar_wait(&sibar, ph, p, 1 << 15) && ok;
@@ -320,8 +318,8 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
             load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::KK), static_cast<const bf16*>(p.k) + krow, (size_t)p.H * K, rows, pt);
             load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
-            load_tile<128, 128, PROD>(reinterpret_cast<bf16*>(b + M::V), static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
-                                      (size_t)p.HV * 128, rows, pt);
+            load_cm<128, PROD>(reinterpret_cast<bf16*>(b + M::V), static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
+                               (size_t)p.HV * 128, rows, pt);
             cp_async_commit();
             cp_async_wait<0>();
             fence_async_smem();
@@ -340,7 +338,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                 tc_fence_after();
                 return ok;
             };
-            if (!wait(&full[stage], (c >> 1) & 1, 1 << 18) || !wait(&sready, ph, 1 << 19)) break;
+            if (!wait(&full[stage], (c >> 1) & 1, 1 << 18)) break;
             auto with_rows = [&](uint32_t acc, uint32_t rows_at, int parts) {  // S parts times rows, K-major
 #pragma unroll
                 for (int i = parts - 1; i >= 0; --i)
@@ -349,8 +347,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                         mma_ts(tmem0 + acc, tmem0 + M::SP + (s / (DH / 16)) * M::HB + i * (DH / 2) + (s % (DH / 16)) * 8,
                                make_desc(b + rows_at + s * 256, 128, K * 16), id64, i < parts - 1 || s > 0);
             };
-            auto with_matrix = [&](uint32_t acc, uint32_t a, uint32_t as, uint32_t mat, int parts) {  // x M^T, M lower triangular
-                bool first = true;
+            auto with_matrix = [&](uint32_t acc, uint32_t a, uint32_t as, uint32_t mat, int parts, bool first) {  // (+)= x M^T, M lower triangular
 #pragma unroll
                 for (int o = parts - 1; o >= 0; --o)
 #pragma unroll
@@ -362,17 +359,25 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                         first = false;
                     }
             };
+            if (elect_one()) {  // v^T T'^T (V' has been read since wready of the chunk before)
+#pragma unroll
+                for (int i = 2; i >= 0; --i)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+                        mma_ss(tmem0 + M::VA + 16 * s, make_desc(b + M::V + s * 4096, 2048, 128), make_desc(b + M::TM + i * M::MAT + s * 256 + s * 2048, 128, 1024),
+                               make_idesc(128, 64 - 16 * s, true, false), i < 2 || s > 0);
+            }
+            __syncwarp();
+            if (!wait(&sready, ph, 1 << 19) || (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
             if (elect_one()) {
                 with_rows(M::KS, M::KK, 3);
                 mma_commit(&ksbar);
+                with_rows(M::QS, M::Q, 2);
             }
-            __syncwarp();
-            if (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20)) break;
-            if (elect_one()) with_rows(M::QS, M::Q, 2);
             __syncwarp();
             if (!wait(&rready, ph, 1 << 21)) break;
             if (elect_one()) {
-                with_matrix(M::KS, M::R, 32, M::TM, 3);
+                with_matrix(M::VA, M::R, 32, M::TM, 3, false);
                 mma_commit(&vbar);
             }
             __syncwarp();
@@ -387,7 +392,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                             mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + M::R + i * 32 + s * 8,
                                    make_desc(b + M::KK + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu, i < 2 || s > 0);
                 mma_commit(&sibar);
-                with_matrix(M::AV, M::VP, M::VPS, M::AM, 2);
+                with_matrix(M::AV, M::VP, M::VPS, M::AM, 2, true);
                 mma_commit(&obar);
             }
             __syncwarp();
@@ -412,7 +417,7 @@ struct Map {
     static constexpr int DH = K / 2;
     static constexpr uint32_t ROWS = C * K * 2, MAT = SQ * 2;
     static constexpr uint32_t KK = 0, Q = ROWS, DO = 2 * ROWS, TM = DO + C * 256, AM = TM + 3 * MAT, AU = AM + 3 * MAT, STAGE = AU + AUX * 4;
-    static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
+    static constexpr uint32_t OT = 2 * STAGE, SUMS = OT + C * 256, TOTAL = SUMS + 4 * C * 4;
     // tensor memory: the parts of dS, over them the update; of the scaled do; of dV', over them X; dS k^T, over it Y; do^T A
     static constexpr uint32_t SP = 0, HB = 3 * DH / 2, DOS = 2 * HB, DV = DOS + 96, KD = DV + 96, AD = KD + 64, COLS = AD + 64;
     static_assert(COLS <= 512 && TOTAL <= 232448 && STAGE % 1024 == 0, "fits");
@@ -511,11 +516,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&dosready);
-            {
-                float* dS = reinterpret_cast<float*>(sc + lay.dS) + unit * K * 128;
-#pragma unroll
-                for (int j = 0; j < DH; ++j) dS[(size_t)(d0 + j) * 128 + e] = S[j];
-            }
+            store_record<DH>(reinterpret_cast<float*>(sc + lay.dS) + unit * K * 128, e, d0, K, S);
             // ---- dV'
             ok = mbar_wait(&kdbar, ph, p, 1 << 13) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -579,10 +580,20 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         const int e = tid & 127;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
+        float* sums = reinterpret_cast<float*>(dyn + M::SUMS);
         for (int i = 0; i < wk.nc; ++i) {
             const int c = wk.nc - 1 - i, stage = i & 1;
             const float* be = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_BETA * C;
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
+            const int rows = wk.rows(c);
+            // v ahead of Y: two tokens per register
+            const bf16* V = static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128 + e;
+            uint32_t v[C / 2];
+#pragma unroll
+            for (int j = 0; j < C; ++j) {
+                const uint32_t x = j < rows ? *reinterpret_cast<const uint16_t*>(V + (size_t)j * p.HV * 128) : 0u;
+                v[j / 2] = j & 1 ? v[j / 2] | x << 16 : x;
+            }
             ok = mbar_wait(&ybar, i & 1, p, 1 << 16) && ok;
             ok = bar_and(2, OUT, ok);
             if (!ok) break;
@@ -594,22 +605,32 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ofree);
-            float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128 + e;
+            float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128;
+            float yv[C];
 #pragma unroll
             for (int g = 0; g < C / 16; ++g) {
                 float f[16];
                 load16(be + 16 * g, f);
+                float x[16];
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
-                    const float v = __uint_as_float(y[g][j]);
-                    Y[(16 * g + j) * 128] = v;
-                    tile[(16 * g + j) * 128 + e] = __float2bfloat16_rn(f[j] * v);
+                    x[j] = __uint_as_float(y[g][j]);
+                    const uint32_t vv = v[8 * g + j / 2];
+                    yv[16 * g + j] = x[j] * __uint_as_float(j & 1 ? vv & 0xffff0000u : vv << 16);
+                    tile[(16 * g + j) * 128 + e] = __float2bfloat16_rn(f[j] * x[j]);
                 }
+                store_record<16>(Y, e, 16 * g, C, x);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[stage]);
+            // sums over the value columns: halve the number of tokens a lane carries at every step; lane l ends with tokens 2 l, 2 l + 1
+            lanes_total<C>(yv, lane);
+            *reinterpret_cast<float2*>(sums + (warp & 3) * C + 2 * lane) = make_float2(yv[0], yv[1]);
             bar_sync(2, OUT);
-            const int rows = wk.rows(c);
+            if (e < C) {
+                const float s = (sums[e] + sums[C + e]) + (sums[2 * C + e] + sums[3 * C + e]);
+                reinterpret_cast<float*>(sc + lay.yv)[unit * C + e] = s;
+            }
             bf16* dst = static_cast<bf16*>(p.grad_v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
 #pragma unroll
             for (int x = e; x < C * 16; x += OUT) {
@@ -631,7 +652,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                 mbar_expect_tx(&full[stage], 6 * M::MAT + AUX * 4);
                 tma_load_1d(b + M::AM, ws + lay.A + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
                 tma_load_1d(b + M::AU, ws + lay.aux + unit * AUX * 4, AUX * 4, &full[stage]);
-                tma_load_1d(b + M::TM, ws + lay.T + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
+                tma_load_1d(b + M::TM, ws + lay.Tb + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
             }
             __syncwarp();
             const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
