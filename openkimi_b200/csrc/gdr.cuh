@@ -25,8 +25,8 @@ constexpr int AUX = 12 * C;        // floats of a unit's per-row numbers
 // beta e^G / |k|, e^(G_last - G) / |k|, scale e^G / |q|, e^G / |k|
 enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST, A_BGK, A_FK, A_OQ, A_GK };
 constexpr int SQ = C * C;          // elements of one part of a 64 x 64 matrix in core-matrix order (cm_idx)
-// BF16 with 128 value columns walks the chunks on tcgen05; T and A are then whole matrices in core-matrix order
-__host__ __device__ __forceinline__ bool on_tc(const KdaGdrParams& p) { return p.dtype == KDA_DTYPE_BF16 && p.dv == 128; }
+// BF16 with 128 key channels and value columns goes on tcgen05; T and A are then whole matrices in core-matrix order
+__host__ __device__ __forceinline__ bool on_tc(const KdaGdrParams& p) { return p.dtype == KDA_DTYPE_BF16 && p.dk == 128 && p.dv == 128; }
 constexpr float G_MIN = -1000.f;   // log decays below count as this: e^-1000 is 0 in FP32, and sums of 64 stay finite
 
 __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I * (I + 1) / 2 + J; }
@@ -34,7 +34,7 @@ __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I *
 // per (chunk, value head) unit, byte offsets
 struct Layout {
     size_t aux, T, A, total_nosave, S0, Vn, Tb, total;    // workspace
-    size_t dS, Y, part, yv, dqk, bwd_total;               // backward scratch
+    size_t dS, Y, part, dqk, bwd_total;                   // backward scratch
 };
 __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     const size_t n = (size_t)p.NT * p.HV, mat = 3 * (on_tc(p) ? SQ : TRI) * 2;
@@ -56,7 +56,6 @@ __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     l.dS = off;   off = align256(off + n * p.dk * p.dv * 4); // gradient of the state at the chunk's end, as S0
     l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV', as V'
     l.part = off; off = align256(off + n * 2 * 4);           // this unit's share of dA_log and ddt_bias
-    l.yv = off;   if (on_tc(p)) off = align256(off + n * C * 4);  // row sums of Y v
     l.dqk = off;  if (p.HV != p.H) off = align256(off + n * 2 * C * p.dk * 4);  // shared key heads: this value head's share of dq, dk
     l.bwd_total = off;
     return l;
@@ -187,19 +186,28 @@ __device__ __forceinline__ void load_tile(bf16* dst, const float* src, size_t st
         put4<3>(dst, C * LD, r * LD + c, x);
     }
 }
-// rows of COLS elements, `stride` apart in memory, into core-matrix order; lanes take 8 rows x 4 chunks of 16 bytes at a time
-template <int COLS, int NTHR>
+// 64 rows of COLS elements, `stride` apart in memory, into core-matrix order (SWZ: two halves of 64 columns with 128-byte swizzle,
+// swz_bf16).  A lane has row lane mod 8 of every block of eight and, of four chunks of 16 bytes, one; warps share the column blocks.
+// Addresses advance by constants: two instructions a copy.
+template <int COLS, int NTHR, bool SWZ = false>
 __device__ __forceinline__ void load_cm(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
-    constexpr int CG = COLS / 32;
-    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
-#pragma unroll 4
-    for (int i = tid >> 5; i < 8 * CG; i += NTHR / 32) {
-        const int rr = i / CG * 8 + r, cc = (i % CG * 4 + c) * 8;
-        const bool in = rr < rows;
-        cp_async16_z(dst + cm_idx(rr, cc, COLS), src + (in ? rr * stride + cc : 0), in);
+    static_assert(!SWZ || COLS == 128, "two halves");
+    constexpr int NW = NTHR / 32, CG = COLS / 32;
+    static_assert(CG % NW == 0, "whole column blocks per warp");
+    const int lane = tid & 31, w = tid >> 5, r = lane & 7, c = lane >> 3;
+#pragma unroll
+    for (int g = 0; g < CG / NW; ++g) {
+        const int cc = ((g * NW + w) * 4 + c) * 8;
+        const bf16* s = src + (size_t)r * stride + cc;
+        const uint32_t d = smem_u32(dst + (SWZ ? swz_bf16(r, cc) : cm_idx(r, cc, COLS)));
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+            const bool in = 8 * b + r < rows;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + b * (SWZ ? 1024 : COLS * 16)), "l"(in ? s : src), "r"(in ? 16 : 0) : "memory");
+            s += 8 * stride;
+        }
     }
 }
-
 // `count` 16-byte words
 template <int NTHR>
 __device__ __forceinline__ void load_words(bf16* dst, const bf16* src, int count, int tid) {
@@ -230,6 +238,45 @@ __device__ __forceinline__ float log_decay(const KdaGdrParams& p, size_t i, int 
 // the three index tables take the same fields as KdaParams
 __device__ __forceinline__ size_t state_at(const KdaGdrParams& p, int d, int e) {
     return (p.flags & KDA_FLAG_STATE_V_FIRST) ? (size_t)e * p.dk + d : (size_t)d * p.dv + e;
+}
+
+// the gradients of g, beta and a unit's share of those of A_log, dt_bias from those of log decay and beta; a lane has two neighbouring rows
+__device__ __forceinline__ void gate_gradients(const KdaGdrParams& p, const Layout& lay, const ChunkInfo& ci, size_t unit, int h, float dg0, float dg1,
+                                               float db0, float db1, float be0, float be1, int lane) {
+    float dA = 0.f, dbias = 0.f;
+    const bool gate = p.flags & KDA_FLAG_GATE;
+    const float eA = gate ? expf(p.A_log[h]) : 0.f, bias = gate && p.dt_bias ? p.dt_bias[h] : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = 2 * lane + i;
+        if (r >= ci.len) continue;
+        const size_t at = (size_t)(ci.tok0 + r) * p.HV + h;
+        float d = i ? dg1 : dg0, b = i ? db1 : db0;
+        const float be = i ? be1 : be0;
+        if (gate) {
+            const float a = load_g(p, p.g, at) + bias;
+            dA += d * fmaxf(-eA * softplus_f(a), G_MIN);
+            d *= -eA * (a > 20.f ? 1.f : sigmoid_f(a));
+            dbias += d;
+        }
+        if (p.flags & KDA_FLAG_BETA_SIGMOID) b *= be * (1.f - be);
+        store_g(p, p.grad_g, at, d);
+        store_g(p, p.grad_beta, at, b);
+    }
+    if (gate) {
+        dA = warp_sum(dA);
+        dbias = warp_sum(dbias);
+        if (lane == 0) *reinterpret_cast<float2*>(static_cast<char*>(p.bwd_scratch) + lay.part + unit * 8) = make_float2(dA, dbias);
+    }
+}
+// 32 bytes at a time: eight floats
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+    asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]) : "l"(p) : "memory");
+}
+__device__ __forceinline__ void store8(float* p, const float* x) {
+    asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]), "f"(x[4]), "f"(x[5]),
+                 "f"(x[6]), "f"(x[7]) : "memory");
 }
 
 }  // namespace gdr

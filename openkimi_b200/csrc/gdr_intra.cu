@@ -215,7 +215,7 @@ static cudaError_t launch_intra(const KdaGdrParams& p, const Layout& l, cudaStre
 
 cudaError_t intra(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
     if (p.dtype == KDA_DTYPE_F32) return p.dk == 64 ? launch_intra<float, 64, false>(p, l, s) : launch_intra<float, 128, false>(p, l, s);
-    if (on_tc(p)) return p.dk == 64 ? launch_intra<bf16, 64, true>(p, l, s) : launch_intra<bf16, 128, true>(p, l, s);
+    if (on_tc(p)) return launch_intra<bf16, 128, true>(p, l, s);
     return p.dk == 64 ? launch_intra<bf16, 64, false>(p, l, s) : launch_intra<bf16, 128, false>(p, l, s);
 }
 

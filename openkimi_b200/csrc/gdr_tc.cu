@@ -15,17 +15,14 @@ namespace kda {
 namespace gdr {
 
 namespace ft {
-constexpr int MAIN = 256, OUT = 128, PROD = 64, NTHR = MAIN + OUT + PROD + 32;
-template <int K>
+constexpr int MAIN = 256, OUT = 128, PROD = 64, NTHR = MAIN + OUT + PROD + 32, K = 128, DH = K / 2;  // DH: key channels of a main thread
 struct Map {
-    static constexpr int DH = K / 2;                       // key channels of a main thread
     static constexpr uint32_t ROWS = C * K * 2, MAT = SQ * 2;
     static constexpr uint32_t KK = 0, Q = ROWS, V = 2 * ROWS, TM = V + C * 256, AM = TM + 3 * MAT, AU = AM + 2 * MAT, STAGE = AU + AUX * 4;
     static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
-    // tensor memory columns.  S parts: per half three blocks of DH / 2; over them, once S k and S q are done, the update (DH columns)
-    // and, with K = 128, in the third block the parts of V'.  V' A^T over S k, W over R.
-    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, VPS = K == 128 ? HB : 32, VP = K == 128 ? DH : 2 * HB,
-                              KS = K == 128 ? 2 * HB : 2 * HB + 64, AV = KS, QS = KS + 64, VA = QS + 64, R = VA + 64, COLS = R + 96;
+    // tensor memory columns.  S parts: per half three blocks of DH / 2; over them, once S k and S q are done, the update (DH columns).
+    // V' A^T over S k, W over R, the parts of V' over V' itself, each half of the rows over its own columns.
+    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, KS = 2 * HB, AV = KS, QS = KS + 64, VA = QS + 64, R = VA + 64, COLS = R + 96;
     static_assert(COLS <= 512 && TOTAL <= 232448, "fits");
 };
 }  // namespace ft
@@ -48,11 +45,7 @@ __device__ __forceinline__ void st_parts(uint32_t at, uint32_t stride, const flo
 template <int N>
 __device__ __forceinline__ void store_record(float* rec, int e, int col, int cols, const float* x) {
 #pragma unroll
-    for (int j = 0; j < N; j += 8) {
-        float4* at = reinterpret_cast<float4*>(rec + rec_idx(e, col + j, cols));
-        at[0] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-        at[1] = make_float4(x[j + 4], x[j + 5], x[j + 6], x[j + 7]);
-    }
+    for (int j = 0; j < N; j += 8) store8(rec + rec_idx(e, col + j, cols), x + j);
 }
 __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
 #pragma unroll
@@ -61,32 +54,6 @@ __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
         x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
     }
 }
-// rows of 128 elements into two halves of 64 with 128-byte swizzle (swz_bf16)
-template <int NTHR>
-__device__ __forceinline__ void load_swz(bf16* dst, const bf16* src, size_t stride, int rows, int tid) {
-    const int lane = tid & 31, r = lane & 7, c = lane >> 3;
-#pragma unroll 4
-    for (int i = tid >> 5; i < 32; i += NTHR / 32) {
-        const int rr = (i >> 2) * 8 + r, cc = ((i & 3) * 4 + c) * 8;
-        const bool in = rr < rows;
-        cp_async16_z(dst + swz_bf16(rr, cc), src + (in ? rr * stride + cc : 0), in);
-    }
-}
-
-// val[i] summed over the 32 lanes; lane l ends with values l M / 32 .. in val[0 .. M / 32)
-template <int M, int O = 16>
-__device__ __forceinline__ void lanes_total(float* val, int lane) {
-    if constexpr (O > 0) {
-        const bool up = lane & O;
-#pragma unroll
-        for (int i = 0; i < M / 2; ++i) {
-            const float keep = up ? val[M / 2 + i] : val[i], send = up ? val[i] : val[M / 2 + i];
-            val[i] = keep + __shfl_xor_sync(0xffffffffu, send, O);
-        }
-        lanes_total<M / 2, O / 2>(val, lane);
-    }
-}
-
 struct Walk {
     int n, h, kh, c0, nc;
     long long tok_begin, tok_end;
@@ -94,11 +61,10 @@ struct Walk {
     __device__ __forceinline__ int rows(int c) const { return (int)min((long long)C, tok_end - tok(c)); }
 };
 
-template <int K, bool SAVE>
+template <bool SAVE>
 __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
     using namespace ft;
-    using M = Map<K>;
-    constexpr int DH = M::DH;
+    using M = Map;
     extern __shared__ __align__(1024) unsigned char dyn[];
     __shared__ uint64_t full[2], empty[2], sready, ksbar, rready, vbar, wready, sibar, obar, ofree;
     __shared__ uint32_t tmem_s;
@@ -158,26 +124,13 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             const unsigned char* b = dyn + stage * M::STAGE;
             const float* aux = reinterpret_cast<const float*>(b + M::AU);
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
-            // ---- the state's parts.  The third goes where V' of the previous chunk is read until its outputs are done.
-            uint32_t low[DH / 16][8];
 #pragma unroll
             for (int g = 0; g < DH / 16; ++g) {
-                uint32_t w[2][8];
+                float x[16];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    uint32_t s[3];
-                    split(S[16 * g + 2 * j], S[16 * g + 2 * j + 1], s);
-                    w[0][j] = s[0]; w[1][j] = s[1]; low[g][j] = s[2];
-                }
-                tmem_st8(tm + M::SP + half * M::HB + 8 * g, w[0]);
-                tmem_st8(tm + M::SP + half * M::HB + DH / 2 + 8 * g, w[1]);
+                for (int j = 0; j < 16; ++j) x[j] = S[16 * g + j];
+                st_parts<3>(tm + M::SP + half * M::HB + 8 * g, DH / 2, x);
             }
-            if (c > 0) {
-                ok = mbar_wait(&obar, ph ^ 1, p, 1 << 12) && ok;
-                tc_fence_after();
-            }
-#pragma unroll
-            for (int g = 0; g < DH / 16; ++g) tmem_st8(tm + M::SP + half * M::HB + DH + 8 * g, low[g]);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
@@ -223,7 +176,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                     f[j] *= x[g][j];
                 }
                 st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, f);
-                st_parts<2>(tm + M::VP + half * 16 + 8 * g, M::VPS, x[g]);
+                st_parts<2>(tm + M::VA + half * 32 + 8 * g, 16, x[g]);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -347,37 +300,36 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                         mma_ts(tmem0 + acc, tmem0 + M::SP + (s / (DH / 16)) * M::HB + i * (DH / 2) + (s % (DH / 16)) * 8,
                                make_desc(b + rows_at + s * 256, 128, K * 16), id64, i < parts - 1 || s > 0);
             };
-            auto with_matrix = [&](uint32_t acc, uint32_t a, uint32_t as, uint32_t mat, int parts, bool first) {  // (+)= x M^T, M lower triangular
+            // (+)= x M^T, M lower triangular: K-step s of x's part i is at a(i, s)
+            auto with_matrix = [&](uint32_t acc, auto a, uint32_t mat, int parts, bool first) {
 #pragma unroll
                 for (int o = parts - 1; o >= 0; --o)
 #pragma unroll
                     for (int i = o; i >= 0; --i) {
 #pragma unroll
                         for (int s = 0; s < 4; ++s)
-                            mma_ts(tmem0 + acc + 16 * s, tmem0 + a + i * as + s * 8, make_desc(b + mat + (o - i) * M::MAT + s * 256 + s * 2048, 128, 1024),
+                            mma_ts(tmem0 + acc + 16 * s, tmem0 + a(i, s), make_desc(b + mat + (o - i) * M::MAT + s * 256 + s * 2048, 128, 1024),
                                    make_idesc(128, 64 - 16 * s, false, false), !first || s > 0);
                         first = false;
                     }
             };
-            if (elect_one()) {  // v^T T'^T (V' has been read since wready of the chunk before)
+            if (!wait(&sready, ph, 1 << 19) || (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
+            if (elect_one()) {
+                with_rows(M::KS, M::KK, 3);
+                mma_commit(&ksbar);
+                // v^T T'^T (the parts of V' that were here have been used: their products' outputs have been read)
 #pragma unroll
                 for (int i = 2; i >= 0; --i)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
                         mma_ss(tmem0 + M::VA + 16 * s, make_desc(b + M::V + s * 4096, 2048, 128), make_desc(b + M::TM + i * M::MAT + s * 256 + s * 2048, 128, 1024),
                                make_idesc(128, 64 - 16 * s, true, false), i < 2 || s > 0);
-            }
-            __syncwarp();
-            if (!wait(&sready, ph, 1 << 19) || (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
-            if (elect_one()) {
-                with_rows(M::KS, M::KK, 3);
-                mma_commit(&ksbar);
                 with_rows(M::QS, M::Q, 2);
             }
             __syncwarp();
             if (!wait(&rready, ph, 1 << 21)) break;
             if (elect_one()) {
-                with_matrix(M::VA, M::R, 32, M::TM, 3, false);
+                with_matrix(M::VA, [](int i, int s) { return M::R + i * 32 + s * 8; }, M::TM, 3, false);
                 mma_commit(&vbar);
             }
             __syncwarp();
@@ -392,7 +344,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                             mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + M::R + i * 32 + s * 8,
                                    make_desc(b + M::KK + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu, i < 2 || s > 0);
                 mma_commit(&sibar);
-                with_matrix(M::AV, M::VP, M::VPS, M::AM, 2, true);
+                with_matrix(M::AV, [](int i, int s) { return M::VA + (s >> 1) * 32 + i * 16 + (s & 1) * 8; }, M::AM, 2, true);
                 mma_commit(&obar);
             }
             __syncwarp();
@@ -412,23 +364,21 @@ using ft::MAIN;
 using ft::OUT;
 using ft::PROD;
 using ft::NTHR;
-template <int K>
+using ft::K;
+using ft::DH;
 struct Map {
-    static constexpr int DH = K / 2;
     static constexpr uint32_t ROWS = C * K * 2, MAT = SQ * 2;
     static constexpr uint32_t KK = 0, Q = ROWS, DO = 2 * ROWS, TM = DO + C * 256, AM = TM + 3 * MAT, AU = AM + 3 * MAT, STAGE = AU + AUX * 4;
-    static constexpr uint32_t OT = 2 * STAGE, SUMS = OT + C * 256, TOTAL = SUMS + 4 * C * 4;
+    static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
     // tensor memory: the parts of dS, over them the update; of the scaled do; of dV', over them X; dS k^T, over it Y; do^T A
     static constexpr uint32_t SP = 0, HB = 3 * DH / 2, DOS = 2 * HB, DV = DOS + 96, KD = DV + 96, AD = KD + 64, COLS = AD + 64;
     static_assert(COLS <= 512 && TOTAL <= 232448 && STAGE % 1024 == 0, "fits");
 };
 }  // namespace bt
 
-template <int K>
 __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
     using namespace bt;
-    using M = Map<K>;
-    constexpr int DH = M::DH;
+    using M = Map;
     extern __shared__ __align__(1024) unsigned char dyn[];
     __shared__ uint64_t full[2], empty[2], sready, kdbar, dosready, dvready, ybar, xready, sibar, ofree;
     __shared__ uint32_t tmem_s;
@@ -580,20 +530,10 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         const int e = tid & 127;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
-        float* sums = reinterpret_cast<float*>(dyn + M::SUMS);
         for (int i = 0; i < wk.nc; ++i) {
             const int c = wk.nc - 1 - i, stage = i & 1;
             const float* be = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_BETA * C;
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
-            const int rows = wk.rows(c);
-            // v ahead of Y: two tokens per register
-            const bf16* V = static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128 + e;
-            uint32_t v[C / 2];
-#pragma unroll
-            for (int j = 0; j < C; ++j) {
-                const uint32_t x = j < rows ? *reinterpret_cast<const uint16_t*>(V + (size_t)j * p.HV * 128) : 0u;
-                v[j / 2] = j & 1 ? v[j / 2] | x << 16 : x;
-            }
             ok = mbar_wait(&ybar, i & 1, p, 1 << 16) && ok;
             ok = bar_and(2, OUT, ok);
             if (!ok) break;
@@ -606,7 +546,6 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             __syncwarp();
             if (lane == 0) mbar_arrive(&ofree);
             float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128;
-            float yv[C];
 #pragma unroll
             for (int g = 0; g < C / 16; ++g) {
                 float f[16];
@@ -615,22 +554,14 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     x[j] = __uint_as_float(y[g][j]);
-                    const uint32_t vv = v[8 * g + j / 2];
-                    yv[16 * g + j] = x[j] * __uint_as_float(j & 1 ? vv & 0xffff0000u : vv << 16);
                     tile[(16 * g + j) * 128 + e] = __float2bfloat16_rn(f[j] * x[j]);
                 }
                 store_record<16>(Y, e, 16 * g, C, x);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[stage]);
-            // sums over the value columns: halve the number of tokens a lane carries at every step; lane l ends with tokens 2 l, 2 l + 1
-            lanes_total<C>(yv, lane);
-            *reinterpret_cast<float2*>(sums + (warp & 3) * C + 2 * lane) = make_float2(yv[0], yv[1]);
             bar_sync(2, OUT);
-            if (e < C) {
-                const float s = (sums[e] + sums[C + e]) + (sums[2 * C + e] + sums[3 * C + e]);
-                reinterpret_cast<float*>(sc + lay.yv)[unit * C + e] = s;
-            }
+            const int rows = wk.rows(c);
             bf16* dst = static_cast<bf16*>(p.grad_v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
 #pragma unroll
             for (int x = e; x < C * 16; x += OUT) {
@@ -657,7 +588,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             __syncwarp();
             const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
             load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::KK), static_cast<const bf16*>(p.k) + krow, (size_t)p.H * K, rows, pt);
-            load_swz<PROD>(reinterpret_cast<bf16*>(b + M::DO), static_cast<const bf16*>(p.grad_o) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
+            load_cm<128, PROD, true>(reinterpret_cast<bf16*>(b + M::DO), static_cast<const bf16*>(p.grad_o) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
                            (size_t)p.HV * 128, rows, pt);
             load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
             cp_async_commit();
@@ -742,28 +673,21 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
     if (warp == 0) tmem_dealloc(tmem0, 512);
 }
 
-template <int K, bool SAVE>
-static cudaError_t launch(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    constexpr int bytes = ft::Map<K>::TOTAL;
-    cudaError_t e = allow_smem(gdr_fwd_tc_kernel<K, SAVE>, bytes);
+template <bool SAVE>
+static cudaError_t launch_fwd(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    cudaError_t e = allow_smem(gdr_fwd_tc_kernel<SAVE>, ft::Map::TOTAL);
     if (e != cudaSuccess) return e;
-    return launch_dependent(gdr_fwd_tc_kernel<K, SAVE>, p.N * p.HV, ft::NTHR, bytes, s, p, l);
+    return launch_dependent(gdr_fwd_tc_kernel<SAVE>, p.N * p.HV, ft::NTHR, ft::Map::TOTAL, s, p, l);
 }
-
-template <int K>
-static cudaError_t launch_bwd(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    constexpr int bytes = bt::Map<K>::TOTAL;
-    cudaError_t e = allow_smem(gdr_bwd_tc_kernel<K>, bytes);
-    if (e != cudaSuccess) return e;
-    return launch_dependent(gdr_bwd_tc_kernel<K>, p.N * p.HV, bt::NTHR, bytes, s, p, l);
-}
-
-cudaError_t bwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) { return p.dk == 64 ? launch_bwd<64>(p, l, s) : launch_bwd<128>(p, l, s); }
 
 cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    const bool save = !(p.flags & KDA_FLAG_NO_SAVE);
-    if (p.dk == 64) return save ? launch<64, true>(p, l, s) : launch<64, false>(p, l, s);
-    return save ? launch<128, true>(p, l, s) : launch<128, false>(p, l, s);
+    return p.flags & KDA_FLAG_NO_SAVE ? launch_fwd<false>(p, l, s) : launch_fwd<true>(p, l, s);
+}
+
+cudaError_t bwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
+    cudaError_t e = allow_smem(gdr_bwd_tc_kernel, bt::Map::TOTAL);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(gdr_bwd_tc_kernel, p.N * p.HV, bt::NTHR, bt::Map::TOTAL, s, p, l);
 }
 
 }  // namespace gdr
