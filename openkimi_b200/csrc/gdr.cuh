@@ -54,7 +54,7 @@ __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     l.total = off;
     off = 0;
     l.dS = off;   off = align256(off + n * p.dk * p.dv * 4); // gradient of the state at the chunk's end, as S0
-    l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV', as V'
+    l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV' [64][dv]
     l.part = off; off = align256(off + n * 2 * 4);           // this unit's share of dA_log and ddt_bias
     l.dqk = off;  if (p.HV != p.H) off = align256(off + n * 2 * C * p.dk * 4);  // shared key heads: this value head's share of dq, dk
     l.bwd_total = off;

@@ -1,36 +1,42 @@
 // Gated delta rule, backward: the gradients of a chunk on tcgen05, from the records that the transposed walks leave (gdr_tc.cu).  The
 // formulas stand in gdr_grad.cu; here
-//   F^T = S0 do^T   E^T = S0 Y^T   H^T = dS V'^T  [128 x 64]      dA = do V'^T   dL = Y V'^T  [64 x 64]
+//   F^T = S0 do^T   E^T = S0 Y^T   H^T = dS V'^T  [128 x 64]      dA^T = V' do^T   dL^T = V' Y^T  [64 x 64]
 // are products over the 128 value columns in K-steps of 16, and then
 //   dq^T = F^T scaled + k^T Z^T       dk^T = E^T and H^T scaled + k^T X^T + k^T X + q^T Z
 // with the key channels as the 128 lanes, so that products with the states run at M = 128.  What L2 norm's gradient needs of q . dq and
 // k . dk comes from the same sums as dG: q . F, k . E, k . H, and rows and columns of Z (q k^T) and X (k k^T).
 //
-// One CTA per SM walks the (chunk, value head) units.  What bounds it: 256 KB of records and rows per unit, 5.9 us of an SM's share
-// of HBM, so everything runs beside the loads: four warps read the records (FP32, in the order in which a K-step wants them), take
-// <S0, dS> and leave three BF16 parts in a ring of two K-steps; a warp issues the products; two bring the next unit's rows; eight do
-// the rest of a unit while the next unit's accumulators fill.  Records of two BF16 parts take the same bytes and no conversion, but
-// dg is a difference of larger sums: 2e-5 off for 15 tokens.
+// One CTA per SM walks the (chunk, value head) units.  Four warps read the records (FP32), take <S0, dS> and leave three BF16 parts in
+// a ring of two K-steps; one issues the products; two bring the next unit's rows; eight do the rest of a unit while the next unit's
+// accumulators fill.  What bounds it: 256 KB of records and rows per unit are 5.9 us of an SM's share of HBM, its products about as
+// much: an MMA whose A operand lies in shared memory takes N / 2 + 43 cycles here (M = 128; M = 64: N / 2 + 27), so do and the parts
+// of Y lie side by side and go through as one operand of up to 192 columns.  Loads from tensor memory wait for the MMAs issued before
+// them, so a unit's accumulators are read at once, before the next unit's first K-step, and the last products of a unit slip in
+// between two K-steps of the next.
+// Records of two BF16 parts take the same bytes and no conversion, but dg is a difference of larger sums: 2e-5 off for 15 tokens.
 #include "gdr.cuh"
 
 namespace kda {
 namespace gdr {
 
 namespace gt {
-constexpr int MAIN = 256, CONV = 128, ROWS = 64, NTHR = MAIN + CONV + 32 + ROWS, RING = 2, K = 128;
+constexpr int MAIN = 256, CONV = 128, ROWS = 64, NTHR = 512, RING = 2, K = 128;  // and a warp for the products, one idle
+// registers of the main, converting and other warps: 8 x 168 + 4 x 104 + 4 x 72 = 16 x 128 a lane
+constexpr int REG_MAIN = 168, REG_CONV = 104, REG_REST = 72;
 constexpr uint32_t MAT = SQ * 2;
-// the rows of a unit: q, k, do as two halves of 64 columns with 128-byte swizzle
-constexpr uint32_t Q = 0, KK = 16384, DO = 32768, AU = 49152, TILE = AU + AUX * 4;
-// a K-step: three parts each of S0, dS [16][128] and V', Y [16][64] in core-matrix order
-constexpr uint32_t SPART = 4096, VPART = 2048, S0 = 0, DS = 3 * SPART, V = 6 * SPART, Y = V + 3 * VPART, STAGE = Y + 3 * VPART;
-// Z, X: two parts each in core-matrix order, then dq and dk as rows
-constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 14 * C * 4, TOTAL = DOTS + 12 * C * 4;
+// the rows of a unit: q, k as two halves of 64 columns with 128-byte swizzle
+constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;
+// a K-step: three parts each of S0, dS [16][128]; of V' the parts side by side [16][3 x 64]; do and the parts of Y one after the other
+// [4 x 64][16], all in core-matrix order
+constexpr uint32_t SPART = 4096, YPART = 2048, S0 = 0, DS = 3 * SPART, V = 6 * SPART, B = V + 6144, STAGE = B + 4 * YPART;
+// Z^T, X^T: two parts each in core-matrix order, then dq and dk as rows
+constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 21 * C * 4, TOTAL = DOTS + 12 * C * 4;
 static_assert(TOTAL <= 231000 && TILE % 1024 == 0, "fits");
-// tensor memory columns; q k^T and k k^T lie where dq and dk go later
-constexpr uint32_t T_F = 0, T_E = 64, T_H = 128, T_DA = 192, T_DL = 256, T_DQ = 320, T_DK = 384;
-// sums over rows or columns of the 64 x 64 matrices: of N (row halves 0, 1), Z qk^T (2), dL KKD (2); columns of N by row block (4);
-// diagonals of Z qk^T and of Y V'^T; then the factors of q and k in the gradient of the L2 norm
-enum { R_N = 0, R_ZQ = 2, R_B = 4, R_COL = 6, R_DZ = 10, R_DY = 11, R_CQ = 12, R_CK = 13 };
+// tensor memory columns; E^T in two halves that are added up (products with the first and the second part of Y)
+constexpr uint32_t T_F = 0, T_E = 64, T_H = 192, T_DA = 256, T_DL = 320, T_DQ = 384, T_DK = 448;
+// sums over 64 x 64 matrices with rows i, columns j: of N over its columns j (two halves of i); by block of j, over rows i: N (4), Z qk^T (4), dL KKD
+// (4); diagonals of Z qk^T and of Y V'^T; the factors of q and k in the gradient of the L2 norm; sums over rows of N, Z qk^T, dL KKD
+enum { R_COL = 0, R_N = 2, R_ZQ = 6, R_B = 10, R_DZ = 14, R_DY = 15, R_CQ = 16, R_CK = 17 };
 }  // namespace gt
 
 // 16 lanes x 32 consecutive columns as fragments: registers 4 i .. 4 i + 3 are (row g, columns 8 i + 2 t, + 1), (row g + 8, the same)
@@ -47,14 +53,25 @@ __device__ __forceinline__ void tmem_frag4(uint32_t at, float (&f)[4][4]) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[i][j] = __uint_as_float(r[4 * i + j]);
 }
-// 32 consecutive columns of this thread's lane
-__device__ __forceinline__ void tmem_row32(uint32_t at, float (&x)[32]) {
-    uint32_t r[2][16];
-    tmem_ld16(at, r[0]);
-    tmem_ld16(at + 16, r[1]);
+// 32 consecutive columns of this thread's lane, from two places, or the sum of two
+__device__ __forceinline__ void tmem_row32(uint32_t at0, uint32_t at1, float (&x)[32], float (&y)[32]) {
+    uint32_t r[4][16];
+    tmem_ld16(at0, r[0]);
+    tmem_ld16(at0 + 16, r[1]);
+    tmem_ld16(at1, r[2]);
+    tmem_ld16(at1 + 16, r[3]);
     tmem_wait_ld();
 #pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] = __uint_as_float(r[j >> 4][j & 15]);
+    for (int j = 0; j < 32; ++j) {
+        x[j] = __uint_as_float(r[j >> 4][j & 15]);
+        y[j] = __uint_as_float(r[2 + (j >> 4)][j & 15]);
+    }
+}
+__device__ __forceinline__ void tmem_row32(uint32_t at0, uint32_t at1, int t0, float (&x)[32]) {
+    float y[32];
+    tmem_row32(at0 + t0, at1 + t0, x, y);
+#pragma unroll
+    for (int j = 0; j < 32; ++j) x[j] += y[j];
 }
 // val[i] summed over the 32 lanes; lane l ends with value l in val[0]: the number of values a lane carries halves at every step
 template <int M, int O = 16>
@@ -69,8 +86,15 @@ __device__ __forceinline__ void lanes_total(float* val, int lane) {
         lanes_total<M / 2, O / 2>(val, lane);
     }
 }
-// K-major operand with 128-byte swizzle: rows of 64 elements (128 bytes), eight rows 1024 bytes; 16 elements along K are 32 bytes
-__device__ __forceinline__ uint64_t desc_rows(uint32_t at, int kstep) { return make_desc_sw128(at + (kstep >> 2) * 8192 + (kstep & 3) * 32, 16, 1024); }
+// A and B fragments of 16 rows from `row` on of a [64][128] tile with 128-byte swizzle, channels c..c + 15 (a_frag, b_frag)
+__device__ __forceinline__ void swz_a_frag(uint32_t (&f)[4], uint32_t x, int row, int c, int lane) {
+    ldsm(f, x + 2 * swz_bf16(row + (lane & 15), c + (lane >> 4) * 8));
+}
+__device__ __forceinline__ void swz_b_frag(uint32_t (&f)[4], uint32_t x, int row, int c, int lane) {
+    ldsm(f, x + 2 * swz_bf16(row + (lane & 7) + (lane >> 4) * 8, c + ((lane >> 3) & 1) * 8));
+}
+template <int N> __device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
 __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrParams p, const Layout lay) {
     using namespace gt;
@@ -110,6 +134,9 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
     const char* ws = static_cast<const char*>(p.workspace);
     char* sc = static_cast<char*>(p.bwd_scratch);
     bool ok = true;
+    if (warp < MAIN / 32) registers_up<REG_MAIN>();  // (one instruction for the four warps of a group)
+    else if (warp < (MAIN + CONV) / 32) registers_down<REG_CONV>();
+    else registers_down<REG_REST>();
 
     if (warp < MAIN / 32) {
         const int rb = warp & 3, half = warp >> 2, g = lane >> 2, t = lane & 3, d = tid & 127, t0 = 32 * half;
@@ -128,80 +155,103 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             ok = bar_and(1, MAIN, ok);  // (also: the unit before is done with Z, X and the sums)
             if (!ok) break;
             // (a wait below that gives up finishes the unit with what there is, for the barriers' sake)
+            const bool any = 2 * half + 1 >= rb;  // rows j = 16 rb.. meet columns i = 32 half.. from the diagonal on
+            const bool tiny = __any_sync(0xffffffffu, (2 * lane < ci.len && fabsf(be[2 * lane]) <= 1e-18f) || (2 * lane + 1 < ci.len && fabsf(be[2 * lane + 1]) <= 1e-18f));
+            float qk[4][4], kk[4][4];  // k_j . q_i, k_j . k_i
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) qk[j][i] = kk[j][i] = 0.f;
+            if (any)
+#pragma unroll 2
+                for (int k = 0; k < K; k += 16) {
+                    uint32_t fk[4], bq[4], bk[4];
+                    swz_a_frag(fk, smem_u32(sk), 16 * rb, k, lane);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        swz_b_frag(bq, smem_u32(sq), t0 + 16 * j, k, lane);
+                        swz_b_frag(bk, smem_u32(sk), t0 + 16 * j, k, lane);
+                        mma(qk[2 * j], fk, bq[0], bq[1]);
+                        mma(qk[2 * j + 1], fk, bq[2], bq[3]);
+                        mma(kk[2 * j], fk, bk[0], bk[1]);
+                        mma(kk[2 * j + 1], fk, bk[2], bk[3]);
+                    }
+                }
             ok = mbar_wait(&accbar, it & 1, p, 1 << 13) && ok;
             tc_fence_after();
-            {   // ---- pairs of rows: 16 rows x 32 columns
-                float dA[4][4], dL[4][4], qk[4][4], kk[4][4];
-                const bool any = 2 * half <= rb;
-                if (any) {
-                    tmem_frag4(tm + T_DA + 32 * half, dA);
-                    tmem_frag4(tm + T_DL + 32 * half, dL);
-                    tmem_frag4(tm + T_DQ + 32 * half, qk);
-                    tmem_frag4(tm + T_DK + 32 * half, kk);
-                }
+            // ---- everything out of the accumulators
+            float fq[32], fk[32], hh[32], dA[4][4], dL[4][4];
+            tmem_row32(tm + T_E, tm + T_E + 64, t0, fk);
+            tmem_row32(tm + T_F + t0, tm + T_H + t0, fq, hh);
+            tmem_frag4(tm + T_DA + t0, dA);
+            tmem_frag4(tm + T_DL + t0, dL);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&accfree);
+            {   // ---- pairs of rows: 16 rows j x 32 columns i
                 const int r0 = 16 * rb + g;
-                float rn[2] = {0.f, 0.f}, rz[2] = {0.f, 0.f}, rl[2] = {0.f, 0.f};
+                float cn[2] = {0.f, 0.f};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    if (2 * half + j / 2 > rb) break;
-                    float col[2] = {0.f, 0.f};
-                    const int j0 = 32 * half + 8 * j + 2 * t;
+                    if (2 * half + j / 2 < rb) continue;
+                    float rn[2] = {0.f, 0.f}, rz[2] = {0.f, 0.f}, rl[2] = {0.f, 0.f};
+                    const int i0 = t0 + 8 * j + 2 * t;
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int r = r0 + 8 * i;
+                        const int jj = r0 + 8 * i;
                         float z[2], x[2];
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
-                            const int cc = j0 + y;
-                            const float e = r >= cc ? expf(ghi[r] - ghi[cc] + (glo[r] - glo[cc])) * rk[cc] : 0.f;
-                            z[y] = r >= cc ? dA[j][2 * i + y] * p.scale * rq[r] * e : 0.f;
-                            const float l = r > cc ? -dL[j][2 * i + y] * rk[r] * e : 0.f;
-                            x[y] = l * be[r];
+                            const int ii = i0 + y;
+                            const float e = ii >= jj ? expf(ghi[ii] - ghi[jj] + (glo[ii] - glo[jj])) * rk[jj] : 0.f;
+                            z[y] = ii >= jj ? dA[j][2 * i + y] * p.scale * rq[ii] * e : 0.f;
+                            const float l = ii > jj ? -dL[j][2 * i + y] * rk[ii] * e : 0.f;
+                            x[y] = l * be[ii];
                             const float zq = z[y] * qk[j][2 * i + y], lk = l * kk[j][2 * i + y];
-                            const float nn = r > cc ? fmaf(be[r], lk, zq) : 0.f;
-                            rz[i] += zq;
-                            rl[i] += lk;
-                            rn[i] += nn;
-                            col[y] += nn;
-                            if (r == cc) {
-                                red[R_DZ * C + r] = zq;
-                                red[R_DY * C + r] = dL[j][2 * i + y];
+                            const float nn = ii > jj ? fmaf(be[ii], lk, zq) : 0.f;
+                            rz[y] += zq;
+                            rl[y] += lk;
+                            rn[y] += nn;
+                            cn[i] += nn;
+                            if (ii == jj) {
+                                red[R_DZ * C + ii] = zq;
+                                red[R_DY * C + ii] = dL[j][2 * i + y];
                             }
                         }
-                        put<2>(sZ, SQ, cm_idx(r, j0, C), z[0], z[1]);
-                        put<2>(sX, SQ, cm_idx(r, j0, C), x[0], x[1]);
+                        put<2>(sZ, SQ, cm_idx(jj, i0, C), z[0], z[1]);
+                        put<2>(sX, SQ, cm_idx(jj, i0, C), x[0], x[1]);
                     }
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) col[y] += __shfl_xor_sync(0xffffffffu, col[y], o);
-                        if (g == 0) red[(R_COL + rb) * C + j0 + y] = col[y];
+                        for (int o = 4; o < 32; o <<= 1) {
+                            rn[y] += __shfl_xor_sync(0xffffffffu, rn[y], o);
+                            rz[y] += __shfl_xor_sync(0xffffffffu, rz[y], o);
+                        }
+                        if (g == 0) {
+                            red[(R_N + rb) * C + i0 + y] = rn[y];
+                            red[(R_ZQ + rb) * C + i0 + y] = rz[y];
+                        }
+                        if (tiny) {
+#pragma unroll
+                            for (int o = 4; o < 32; o <<= 1) rl[y] += __shfl_xor_sync(0xffffffffu, rl[y], o);
+                            if (g == 0) red[(R_B + rb) * C + i0 + y] = rl[y];
+                        }
                     }
                 }
                 fence_async_smem();
-                tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&zready);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
-                    for (int o = 1; o < 4; o <<= 1) {
-                        rn[i] += __shfl_xor_sync(0xffffffffu, rn[i], o);
-                        rz[i] += __shfl_xor_sync(0xffffffffu, rz[i], o);
-                        rl[i] += __shfl_xor_sync(0xffffffffu, rl[i], o);
-                    }
-                    if (t == 0) {
-                        red[(R_N + half) * C + r0 + 8 * i] = rn[i];
-                        red[(R_ZQ + half) * C + r0 + 8 * i] = rz[i];
-                        red[(R_B + half) * C + r0 + 8 * i] = rl[i];
-                    }
+                    for (int o = 1; o < 4; o <<= 1) cn[i] += __shfl_xor_sync(0xffffffffu, cn[i], o);
+                    if (t == 0) red[(R_COL + half) * C + r0 + 8 * i] = cn[i];
                 }
             }
             // ---- the products with the states: lane d, 32 rows
-            float fq[32], fk[32];
             {
                 float s[32];
-                tmem_row32(tm + T_F + t0, fq);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
                     fq[j] *= aux[A_OQ * C + t0 + j];
@@ -209,41 +259,34 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 }
                 lanes_total<32>(s, lane);
                 dots[rb * C + t0 + lane] = s[0];
-                tmem_row32(tm + T_E + t0, fk);
 #pragma unroll
                 for (int j = 0; j < 32; ++j) {
+                    const float k = __bfloat162float(sk[swz_bf16(t0 + j, d)]);
                     fk[j] *= aux[A_GK * C + t0 + j];
-                    s[j] = fk[j] * __bfloat162float(sk[swz_bf16(t0 + j, d)]);
-                    fk[j] *= -be[t0 + j];
+                    s[j] = fk[j] * k;
+                    hh[j] *= aux[A_FK * C + t0 + j];
+                    fk[j] = hh[j] - be[t0 + j] * fk[j];
+                    hh[j] *= k;
                 }
                 lanes_total<32>(s, lane);
                 dots[(4 + rb) * C + t0 + lane] = s[0];
-                tmem_row32(tm + T_H + t0, s);
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&accfree);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    s[j] *= aux[A_FK * C + t0 + j];
-                    fk[j] += s[j];
-                    s[j] *= __bfloat162float(sk[swz_bf16(t0 + j, d)]);
-                }
-                lanes_total<32>(s, lane);
-                dots[(8 + rb) * C + t0 + lane] = s[0];
+                lanes_total<32>(hh, lane);
+                dots[(8 + rb) * C + t0 + lane] = hh[0];
             }
             bar_sync(1, MAIN);
             auto dot = [&](int which, int r) {
                 const float* x = dots + which * 4 * C + r;
                 return (x[0] + x[C]) + (x[2 * C] + x[3 * C]);
             };
-            auto cols = [&](int r) {  // column r of N: the row blocks from its own on
+            auto rows = [&](int which, int r) {  // sum over row r, the blocks of columns up to its own
                 float s = 0.f;
-                for (int i = r >> 4; i < 4; ++i) s += red[(R_COL + i) * C + r];
+                for (int j = 0; j <= r >> 4; ++j) s += red[(which + j) * C + r];
                 return s;
             };
+            auto cols = [&](int r) { return red[R_COL * C + r] + red[(R_COL + 1) * C + r]; };
             if (warp < 2) {  // a row shorter than 1e-6 is divided by that, whatever its length
                 const int r = tid;
-                const float n = red[R_N * C + r] + red[(R_N + 1) * C + r], z = red[R_ZQ * C + r] + red[(R_ZQ + 1) * C + r], dz = red[R_DZ * C + r];
+                const float n = rows(R_N, r), z = rows(R_ZQ, r), dz = red[R_DZ * C + r];
                 const bool l2 = p.flags & KDA_FLAG_QK_L2NORM;
                 red[R_CQ * C + r] = l2 && rq[r] < 1e6f ? rq[r] * rq[r] * (dot(0, r) + z) : 0.f;
                 red[R_CK * C + r] = l2 && rk[r] < 1e6f ? rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + (n - (z - dz)) + cols(r) + dz) : 0.f;
@@ -254,20 +297,21 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const int r = 2 * lane + i;
-                    const float n = red[R_N * C + r] + red[(R_N + 1) * C + r], e = dot(1, r), hh = dot(2, r);
-                    dG[i] = (double)n - cols(r) + dot(0, r) - (double)be[r] * e - hh;
-                    hsum += hh;
+                    const float e = dot(1, r), h1 = dot(2, r);
+                    dG[i] = (double)rows(R_N, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
+                    hsum += h1;
                     // Y_i . V'_i / beta_i; where beta_i is 0, or so small that the quotient means nothing, Y_i . v_i less what the chunk
                     // predicts for v_i
                     if (fabsf(be[r]) > 1e-18f) {
                         db[i] = red[R_DY * C + r] / be[r];
                     } else {
-                        const float* y = reinterpret_cast<const float*>(sc + lay.Y) + (size_t)u * C * 128;
+                        const float* y = reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + r) * 128;
                         float yv = 0.f;
-                        if (r < ci.len)
-                            for (int x = 0; x < 128; ++x)
-                                yv = fmaf(y[rec_idx(x, r, C)], ldf(static_cast<const bf16*>(p.v) + (((size_t)ci.tok0 + r) * p.HV + h) * 128 + x), yv);
-                        db[i] = yv - e + red[R_B * C + r] + red[(R_B + 1) * C + r];
+                        if (r < ci.len) {
+                            for (int x = 0; x < 128; ++x) yv = fmaf(y[x], ldf(static_cast<const bf16*>(p.v) + (((size_t)ci.tok0 + r) * p.HV + h) * 128 + x), yv);
+                            yv += rows(R_B, r) - e;
+                        }
+                        db[i] = yv;
                     }
                 }
 #pragma unroll
@@ -287,15 +331,15 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             tc_fence_after();
             {
                 float s[32];
-                tmem_row32(tm + T_DQ + t0, s);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) fq[j] += s[j] - red[R_CQ * C + t0 + j] * __bfloat162float(sq[swz_bf16(t0 + j, d)]);
-                tmem_row32(tm + T_DK + t0, s);
+                tmem_row32(tm + T_DQ + t0, tm + T_DK + t0, s, hh);
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&dqfree);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) fk[j] += s[j] - red[R_CK * C + t0 + j] * __bfloat162float(sk[swz_bf16(t0 + j, d)]);
+                for (int j = 0; j < 32; ++j) {
+                    fq[j] += s[j] - red[R_CQ * C + t0 + j] * __bfloat162float(sq[swz_bf16(t0 + j, d)]);
+                    fk[j] += hh[j] - red[R_CK * C + t0 + j] * __bfloat162float(sk[swz_bf16(t0 + j, d)]);
+                }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&tempty[tb]);
@@ -323,8 +367,10 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             }
         }
     } else if (warp < (MAIN + CONV) / 32) {
-        const int t = tid - MAIN;
+        const int t = tid - MAIN, row = t >> 1, e8 = (t & 1) * 8;
         float x[6][8];  // pieces of eight values: S0 and dS two each, V' and Y
+        uint4 od;       // do
+        const bf16* dsrc = nullptr;
         auto request = [&](int u, int k) {
             const float* a = reinterpret_cast<const float*>(ws + lay.S0) + (size_t)u * K * 128 + k * 16 * K + 8 * t;
             const float* e = reinterpret_cast<const float*>(sc + lay.dS) + (size_t)u * K * 128 + k * 16 * K + 8 * t;
@@ -333,7 +379,12 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             load8(e, x[2]);
             load8(e + 8 * CONV, x[3]);
             load8(reinterpret_cast<const float*>(ws + lay.Vn) + (size_t)u * C * 128 + k * 16 * C + 8 * t, x[4]);
-            load8(reinterpret_cast<const float*>(sc + lay.Y) + (size_t)u * C * 128 + k * 16 * C + 8 * t, x[5]);
+            load8(reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + row) * 128 + k * 16 + e8, x[5]);
+            if (k == 0) {
+                const ChunkInfo ci = chunk_info(p, u / p.HV);
+                dsrc = row < ci.len ? static_cast<const bf16*>(p.grad_o) + (((size_t)ci.tok0 + row) * p.HV + u % p.HV) * 128 + e8 : nullptr;
+            }
+            od = dsrc ? *reinterpret_cast<const uint4*>(dsrc + k * 16) : make_uint4(0, 0, 0, 0);
         };
         auto leave = [&](unsigned char* at, uint32_t part, const float (&v)[8]) {
             uint32_t w[4][3];
@@ -358,8 +409,10 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                     leave(b + S0 + 16 * (t + CONV * j), SPART, x[j]);
                     leave(b + DS + 16 * (t + CONV * j), SPART, x[2 + j]);
                 }
-                leave(b + V + 16 * t, VPART, x[4]);
-                leave(b + Y + 16 * t, VPART, x[5]);
+                leave(b + V + (t >> 6) * 3072 + 16 * (t & 63), 1024, x[4]);
+                unsigned char* rows = b + gt::B + (row >> 3) * 256 + (t & 1) * 128 + (row & 7) * 16;
+                *reinterpret_cast<uint4*>(rows) = od;
+                leave(rows + YPART, YPART, x[5]);
                 if (k < 7) request(u, k + 1);
                 else if (u + stride < units) request(u + stride, 0);
                 fence_async_smem();
@@ -374,86 +427,85 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             __syncwarp();
         }
     } else if (warp == (MAIN + CONV) / 32) {
-        constexpr uint32_t idF = make_idesc(128, 64, true, false), idE = make_idesc(128, 64, true, true), idA = make_idesc(64, 64, false, true),
-                           idL = make_idesc(64, 64, true, true), idQ = make_idesc(64, 64, false, false);
+        constexpr uint32_t id192 = make_idesc(128, 192, true, false), id128 = make_idesc(128, 128, true, false), id64 = make_idesc(128, 64, true, false),
+                           idH = make_idesc(128, 64, true, true), idA = make_idesc(64, 128, true, false), idL = make_idesc(64, 64, true, false);
         auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
             ok = ok && __all_sync(0xffffffffu, mbar_wait(bar, parity, p, what));
             tc_fence_after();
             return ok;
         };
-        int step = 0;
-        const uint32_t z = smem_u32(dyn + Z), x = smem_u32(dyn + X);
-        for (int u = blockIdx.x, it = 0; u < units && ok; u += stride, ++it) {
-            if (!wait(&tfull[it & 1], (it >> 1) & 1, 1 << 16) || (it > 0 && !wait(&accfree, (it - 1) & 1, 1 << 17))) break;
-            const uint32_t tile = smem_u32(dyn + (it & 1) * TILE);
-            for (int k = 0; k < 8 && ok; ++k, ++step) {
-                const int st = step % RING;
-                if (!wait(&full[st], (step / RING) & 1, 1 << 18)) break;
-                const uint32_t b = smem_u32(dyn + R0 + st * STAGE);
-                if (elect_one()) {
-                    const uint64_t dO = desc_rows(tile + DO, k);
-                    uint64_t S[3], D[3], W[3], G[3];
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) {
-                        S[i] = make_desc(b + S0 + i * SPART, 2048, 128);
-                        D[i] = make_desc(b + DS + i * SPART, 2048, 128);
-                        W[i] = make_desc(b + V + i * VPART, 1024, 128);
-                        G[i] = make_desc(b + Y + i * VPART, 1024, 128);
-                    }
-                    const bool acc = k > 0;
-#pragma unroll
-                    for (int i = 2; i >= 0; --i) {
-                        mma_ss(tmem0 + T_DA, dO, W[i], idA, acc || i < 2);
-                        mma_ss(tmem0 + T_F, S[i], dO, idF, acc || i < 2);
-                    }
-#pragma unroll
-                    for (int o = 2; o >= 0; --o)
-#pragma unroll
-                        for (int i = o; i >= 0; --i) {
-                            const bool more = acc || o < 2 || i < o;
-                            mma_ss(tmem0 + T_DL, G[i], W[o - i], idL, more);
-                            mma_ss(tmem0 + T_E, S[i], G[o - i], idE, more);
-                            mma_ss(tmem0 + T_H, D[i], W[o - i], idE, more);
-                        }
-                    mma_commit(&empty[st]);
-                }
-                __syncwarp();
-            }
-            if (!ok || (it > 0 && !wait(&dqfree, (it - 1) & 1, 1 << 19))) break;
+        // the last products of unit `it`.  Z^T and X^T are upper triangular: as [K = j][N = i] K-step s meets columns from its own block
+        // on, as [N = j][K = i] rows up to it.
+        auto finish = [&](int it) {
+            if ((it > 0 && !wait(&dqfree, (it - 1) & 1, 1 << 19)) || !wait(&zready, it & 1, 1 << 20)) return;
+            const uint32_t tile = smem_u32(dyn + (it & 1) * TILE), z = smem_u32(dyn + Z), x = smem_u32(dyn + X);
             if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    mma_ss(tmem0 + T_DQ, desc_rows(tile + Q, k), desc_rows(tile + KK, k), idQ, k > 0);
-                    mma_ss(tmem0 + T_DK, desc_rows(tile + KK, k), desc_rows(tile + KK, k), idQ, k > 0);
-                }
-                mma_commit(&accbar);
-            }
-            __syncwarp();
-            if (!wait(&zready, it & 1, 1 << 20)) break;
-            if (elect_one()) {  // Z and X are lower triangular: K-step s meets rows (or columns) from its own block on (or up to it)
 #pragma unroll
                 for (int i = 1; i >= 0; --i)
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
                         const uint64_t k_s = make_desc_sw128(tile + KK + s * 2048, 8192, 1024);
-                        const uint32_t id = make_idesc(128, 64 - 16 * s, true, false);
-                        mma_ss(tmem0 + T_DQ + 16 * s, k_s, make_desc(z + i * MAT + s * 256 + s * 2048, 128, 1024), id, i < 1 || s > 0);
-                        mma_ss(tmem0 + T_DK + 16 * s, k_s, make_desc(x + i * MAT + s * 256 + s * 2048, 128, 1024), id, i < 1 || s > 0);
+                        const uint32_t id = make_idesc(128, 64 - 16 * s, true, true);
+                        mma_ss(tmem0 + T_DQ + 16 * s, k_s, make_desc(z + i * MAT + s * 2048 + s * 256, 1024, 128), id, i < 1 || s > 0);
+                        mma_ss(tmem0 + T_DK + 16 * s, k_s, make_desc(x + i * MAT + s * 2048 + s * 256, 1024, 128), id, i < 1 || s > 0);
                     }
 #pragma unroll
                 for (int i = 1; i >= 0; --i)
 #pragma unroll
                     for (int s = 0; s < 4; ++s) {
-                        const uint32_t id = make_idesc(128, 16 * (s + 1), true, true);
-                        mma_ss(tmem0 + T_DK, make_desc_sw128(tile + KK + s * 2048, 8192, 1024), make_desc(x + i * MAT + s * 2048, 1024, 128), id, true);
-                        mma_ss(tmem0 + T_DK, make_desc_sw128(tile + Q + s * 2048, 8192, 1024), make_desc(z + i * MAT + s * 2048, 1024, 128), id, true);
+                        const uint32_t id = make_idesc(128, 16 * (s + 1), true, false);
+                        mma_ss(tmem0 + T_DK, make_desc_sw128(tile + KK + s * 2048, 8192, 1024), make_desc(x + i * MAT + s * 256, 128, 1024), id, true);
+                        mma_ss(tmem0 + T_DK, make_desc_sw128(tile + Q + s * 2048, 8192, 1024), make_desc(z + i * MAT + s * 256, 128, 1024), id, true);
                     }
                 mma_commit(&dqbar);
                 mma_commit(&tempty[it & 1]);
             }
             __syncwarp();
+        };
+        int step = 0, it = 0;
+        for (int u = blockIdx.x; u < units && ok; u += stride, ++it) {
+            if (it > 0 && !wait(&accfree, (it - 1) & 1, 1 << 17)) break;
+            for (int k = 0; k < 8 && ok; ++k, ++step) {
+                const int st = step % RING;
+                if (k == 3 && it > 0) finish(it - 1);  // by now its pairs are there
+                if (!wait(&full[st], (step / RING) & 1, 1 << 18)) break;
+                const uint32_t b = smem_u32(dyn + R0 + st * STAGE);
+                if (elect_one()) {
+                    uint64_t S[3], D[3], W[3];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        S[i] = make_desc(b + S0 + i * SPART, 2048, 128);
+                        D[i] = make_desc(b + DS + i * SPART, 2048, 128);
+                        W[i] = make_desc(b + V + i * 1024, 3072, 128);
+                    }
+                    const uint64_t dO = make_desc(b + gt::B, 128, 256), Y0 = make_desc(b + gt::B + YPART, 128, 256),
+                                   Y1 = make_desc(b + gt::B + 2 * YPART, 128, 256), Y2 = make_desc(b + gt::B + 3 * YPART, 128, 256);
+                    const bool acc = k > 0;
+                    // [do | Y0 | Y1] and [do | Y0] are read from dO on; products of the smallest parts first
+                    mma_ss(tmem0 + T_F, S[1], dO, id192, acc);
+                    mma_ss(tmem0 + T_F, S[2], dO, id128, true);
+                    mma_ss(tmem0 + T_E + 64, S[0], Y2, id64, true);
+                    mma_ss(tmem0 + T_F, S[0], dO, id192, true);
+                    mma_ss(tmem0 + T_H, D[2], W[0], idH, acc);
+                    mma_ss(tmem0 + T_H, D[1], W[1], idH, true);
+                    mma_ss(tmem0 + T_H, D[0], W[2], idH, true);
+                    mma_ss(tmem0 + T_H, D[1], W[0], idH, true);
+                    mma_ss(tmem0 + T_H, D[0], W[1], idH, true);
+                    mma_ss(tmem0 + T_H, D[0], W[0], idH, true);
+                    mma_ss(tmem0 + T_DA, W[2], dO, idA, acc);
+                    mma_ss(tmem0 + T_DL, W[1], Y1, idL, true);
+                    mma_ss(tmem0 + T_DL, W[0], Y2, idL, true);
+                    mma_ss(tmem0 + T_DA, W[1], dO, idA, true);
+                    mma_ss(tmem0 + T_DL, W[0], Y1, idL, true);
+                    mma_ss(tmem0 + T_DA, W[0], dO, idA, true);
+                    mma_commit(&empty[st]);
+                    if (k == 7) mma_commit(&accbar);
+                }
+                __syncwarp();
+            }
         }
-    } else {
+        if (ok && it > 0) finish(it - 1);
+    } else if (warp < (MAIN + CONV + 32 + ROWS) / 32) {
         const int rt = tid - MAIN - CONV - 32;
         for (int u = blockIdx.x, it = 0; u < units; u += stride, ++it) {
             const int tb = it & 1, c = u / p.HV, h = u - c * p.HV, kh = h / grp;
@@ -470,7 +522,6 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             }
             __syncwarp();
             const size_t qrow = ((size_t)ci.tok0 * p.H + kh) * K;
-            load_cm<K, ROWS, true>(reinterpret_cast<bf16*>(b + DO), static_cast<const bf16*>(p.grad_o) + ((size_t)ci.tok0 * p.HV + h) * 128, (size_t)p.HV * 128, ci.len, rt);
             load_cm<K, ROWS, true>(reinterpret_cast<bf16*>(b + Q), static_cast<const bf16*>(p.q) + qrow, (size_t)p.H * K, ci.len, rt);
             load_cm<K, ROWS, true>(reinterpret_cast<bf16*>(b + KK), static_cast<const bf16*>(p.k) + qrow, (size_t)p.H * K, ci.len, rt);
             load_words<ROWS>(reinterpret_cast<bf16*>(b + AU), reinterpret_cast<const bf16*>(ws + lay.aux + (size_t)u * AUX * 4), AUX * 4 / 16, rt);

@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ofree);
-            float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128;
+            float* Y = reinterpret_cast<float*>(sc + lay.Y) + unit * C * 128 + e;  // [64][128]
 #pragma unroll
             for (int g = 0; g < C / 16; ++g) {
                 float f[16];
@@ -555,8 +555,8 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                 for (int j = 0; j < 16; ++j) {
                     x[j] = __uint_as_float(y[g][j]);
                     tile[(16 * g + j) * 128 + e] = __float2bfloat16_rn(f[j] * x[j]);
+                    Y[(16 * g + j) * 128] = x[j];
                 }
-                store_record<16>(Y, e, 16 * g, C, x);
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[stage]);
