@@ -310,6 +310,8 @@ typedef struct KdaGdrParams {
     void *bwd_scratch;
     size_t bwd_scratch_bytes;
     int32_t *status, *status_host; /* as in KdaParams; may be NULL */
+    int32_t max_chunks;          /* with cu_seqlens: chunks of the longest sequence, 0: not known.  Decides whether long sequences
+                                    are cut into segments; the same value in all calls of one forward and backward */
 } KdaGdrParams;
 int kda_gdr_workspace_bytes(const KdaGdrParams *p, size_t *fwd_bytes, size_t *bwd_bytes);
 int kda_gdr_fwd(const KdaGdrParams *p, void *cuda_stream);

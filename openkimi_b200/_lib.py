@@ -55,7 +55,7 @@ class KdaGdrParams(C.Structure):
                                      "chunk_tab", "o", "ht", "workspace")] + [("workspace_bytes", C.c_size_t)]
         + [(n, C.c_void_p) for n in ("grad_o", "grad_ht", "grad_q", "grad_k", "grad_v", "grad_g", "grad_beta", "grad_A_log",
                                      "grad_dt_bias", "grad_h0", "bwd_scratch")] + [("bwd_scratch_bytes", C.c_size_t),
-                                                                                    ("status", C.c_void_p), ("status_host", C.c_void_p)])
+                                                                                    ("status", C.c_void_p), ("status_host", C.c_void_p), ("max_chunks", C.c_int32)])
 
 
 EXPORTS = {

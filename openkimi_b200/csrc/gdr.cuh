@@ -33,12 +33,38 @@ __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I *
 
 // per (chunk, value head) unit, byte offsets
 struct Layout {
-    size_t aux, T, A, total_nosave, S0, Vn, Tb, total;    // workspace
-    size_t dS, Y, part, dqk, bwd_total;                   // backward scratch
+    size_t aux, T, A, segE, segX, total_nosave, S0, Vn, Tb, total;  // workspace
+    size_t dS, Y, part, dqk, segF, bwd_total;                       // backward scratch
+    int segs, seg_len;                                              // segments of a sequence (1: none) and their chunks
 };
-__host__ __device__ inline Layout layout(const KdaGdrParams& p) {
+inline int longest(const KdaGdrParams& p) {  // chunks of the longest sequence, 0: not known
+    return p.cu_seqlens ? p.max_chunks : (p.T + C - 1) / C;
+}
+// Segments per sequence of the walks on tcgen05 (gdr_tc.cu).  A walk is a chain of chunks; with fewer walks than SMs a sequence is cut
+// into n segments that are walked twice: from zero (and from the identity, for what a segment does to the state that it is entered
+// with), and again from the states that follow.  Estimated with what a chunk (3.7 us without outputs, 4.3 us with), a border (1.5 us)
+// and the launches (8 us) cost; 8 walks of 512 chunks, the whole forward: 2312 -> 460 us.
+inline int segment_count(const KdaGdrParams& p) {
+    if (!on_tc(p)) return 1;
+    const int nc = longest(p), sms = sm_count();
+    const long long walks = (long long)p.N * p.HV;
+    if (nc < 4 || walks * 2 > sms) return 1;
+    double best = nc * 4.3;
+    int n = 1;
+    for (int s = 2; s <= nc / 2 && s <= 64; ++s) {
+        const int len = (nc + s - 1) / s;
+        const double waves1 = (double)((walks * (2 * s - 3) + sms - 1) / sms), waves2 = (double)((walks * s + sms - 1) / sms);
+        const double t = len * (3.7 * waves1 + 4.3 * waves2) + 1.5 * s + 8.0;
+        if (t < best) best = t, n = s;
+    }
+    return n;
+}
+inline Layout layout(const KdaGdrParams& p) {
     const size_t n = (size_t)p.NT * p.HV, mat = 3 * (on_tc(p) ? SQ : TRI) * 2;
     Layout l;
+    l.segs = segment_count(p);
+    l.seg_len = l.segs > 1 ? (longest(p) + l.segs - 1) / l.segs : 0x7fffffff;
+    const size_t seg_bytes = l.segs > 1 ? (size_t)p.N * p.HV * l.segs * p.dk * p.dv * 4 : 0;
     size_t off = 0;
     l.aux = off; off = align256(off + n * AUX * 4);
     // (I + diag(beta) L)^-1 and scale (q k^T) D as three BF16 parts: blocks of the lower triangle in blk() order, rows swizzled as
@@ -46,6 +72,8 @@ __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     // beta, and T itself for the backward
     l.T = off;   off = align256(off + n * mat);
     l.A = off;   off = align256(off + n * mat);
+    l.segE = off; off += seg_bytes;  // [sequence, head][segment][dk][dv]: state at the segment's end
+    l.segX = off; off += seg_bytes;  // the same of the identity: S_end = X S_begin + E
     l.total_nosave = off;
     // state at the chunk's start [dk][dv] and V' [64][dv], on_tc in the order of rec_idx()
     l.S0 = off;  off = align256(off + n * p.dk * p.dv * 4);
@@ -57,6 +85,7 @@ __host__ __device__ inline Layout layout(const KdaGdrParams& p) {
     l.Y = off;    off = align256(off + n * C * p.dv * 4);    // T^T dV' [64][dv]
     l.part = off; off = align256(off + n * 2 * 4);           // this unit's share of dA_log and ddt_bias
     l.dqk = off;  if (p.HV != p.H) off = align256(off + n * 2 * C * p.dk * 4);  // shared key heads: this value head's share of dq, dk
+    l.segF = off; off += seg_bytes;  // gradient of the state at the segment's start
     l.bwd_total = off;
     return l;
 }

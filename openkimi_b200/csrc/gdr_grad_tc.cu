@@ -6,13 +6,14 @@
 // with the key channels as the 128 lanes, so that products with the states run at M = 128.  What L2 norm's gradient needs of q . dq and
 // k . dk comes from the same sums as dG: q . F, k . E, k . H, and rows and columns of Z (q k^T) and X (k k^T).
 //
-// One CTA per SM walks the (chunk, value head) units.  Four warps read the records (FP32), take <S0, dS> and leave three BF16 parts in
-// a ring of two K-steps; one issues the products; two bring the next unit's rows; eight do the rest of a unit while the next unit's
-// accumulators fill.  What bounds it: 256 KB of records and rows per unit are 5.9 us of an SM's share of HBM, its products about as
-// much: an MMA whose A operand lies in shared memory takes N / 2 + 43 cycles here (M = 128; M = 64: N / 2 + 27), so do and the parts
-// of Y lie side by side and go through as one operand of up to 192 columns.  Loads from tensor memory wait for the MMAs issued before
-// them, so a unit's accumulators are read at once, before the next unit's first K-step, and the last products of a unit slip in
-// between two K-steps of the next.
+// One CTA per SM walks the (chunk, value head) units.  A warp copies the records' K-steps into shared memory, four warps take <S0, dS>
+// and leave three BF16 parts in a ring of two K-steps; one issues the products; one brings the next unit's rows; eight do the rest of
+// a unit while the next unit's accumulators fill; one the gradients of gate and beta.  (Code that
+// waits for its own results runs at one instruction in ten cycles a warp, so a unit is dealt to sixteen warps rather than eight: 358 -> us.)  What bounds it: 256 KB of records and rows per
+// unit are 5.9 us of an SM's share of HBM, its products about as much: an MMA whose A operand lies in shared memory takes N / 2 + 43
+// cycles here (M = 128; M = 64: N / 2 + 27), so do and the parts of Y lie side by side and go through as one operand of up to 192
+// columns.  Loads from tensor memory wait for the MMAs issued before them, so a unit's accumulators are read at once, before the next
+// unit's first K-step, and the last products of a unit slip in between two K-steps of the next.
 // Records of two BF16 parts take the same bytes and no conversion, but dg is a difference of larger sums: 2e-5 off for 15 tokens.
 #include "gdr.cuh"
 
@@ -20,9 +21,10 @@ namespace kda {
 namespace gdr {
 
 namespace gt {
-constexpr int MAIN = 256, CONV = 128, ROWS = 64, NTHR = 512, RING = 2, K = 128;  // and a warp for the products, one idle
-// registers of the main, converting and other warps: 8 x 168 + 4 x 104 + 4 x 72 = 16 x 128 a lane
-constexpr int REG_MAIN = 168, REG_CONV = 104, REG_REST = 72;
+constexpr int MAIN = 512, CONV = 256, NTHR = 896, RING = 2, K = 128;
+constexpr int W_CONV = MAIN / 32, W_MMA = W_CONV + CONV / 32, W_ROWS = W_MMA + 1, W_COPY = W_ROWS + 1;  // the other warps; the last is the gate's
+// registers of the main, converting and other warps; 16 x 80 + 8 x 56 + 4 x 72 = 28 x 72 a lane
+constexpr int REG_MAIN = 80, REG_CONV = 56, REG_REST = 72;
 constexpr uint32_t MAT = SQ * 2;
 // the rows of a unit: q, k as two halves of 64 columns with 128-byte swizzle
 constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;
@@ -30,53 +32,36 @@ constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;
 // [4 x 64][16], all in core-matrix order
 constexpr uint32_t SPART = 4096, YPART = 2048, S0 = 0, DS = 3 * SPART, V = 6 * SPART, B = V + 6144, STAGE = B + 4 * YPART;
 // Z^T, X^T: two parts each in core-matrix order, then dq and dk as rows
-constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 21 * C * 4, TOTAL = DOTS + 12 * C * 4;
-static_assert(TOTAL <= 231000 && TILE % 1024 == 0, "fits");
+constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 20 * C * 4,
+                   TOTAL = DOTS + 12 * C * 4;
+static_assert(TOTAL <= 232448 - 1024 && TILE % 1024 == 0, "fits");
 // tensor memory columns; E^T in two halves that are added up (products with the first and the second part of Y)
 constexpr uint32_t T_F = 0, T_E = 64, T_H = 192, T_DA = 256, T_DL = 320, T_DQ = 384, T_DK = 448;
-// sums over 64 x 64 matrices with rows i, columns j: of N over its columns j (two halves of i); by block of j, over rows i: N (4), Z qk^T (4), dL KKD
-// (4); diagonals of Z qk^T and of Y V'^T; the factors of q and k in the gradient of the L2 norm; sums over rows of N, Z qk^T, dL KKD
-enum { R_COL = 0, R_N = 2, R_ZQ = 6, R_B = 10, R_DZ = 14, R_DY = 15, R_CQ = 16, R_CK = 17 };
+// sums over 64 x 64 matrices with rows i, columns j: of N over columns j by block of i (4); over rows i by block of j: N (4), Z qk^T (4),
+// dL KKD (4); diagonals of Z qk^T and of Y V'^T; the factors of q and k in the gradient of the L2 norm
+enum { R_COL = 0, R_N = 4, R_ZQ = 8, R_B = 12, R_DZ = 16, R_DY = 17, R_CQ = 18, R_CK = 19 };
 }  // namespace gt
 
-// 16 lanes x 32 consecutive columns as fragments: registers 4 i .. 4 i + 3 are (row g, columns 8 i + 2 t, + 1), (row g + 8, the same)
-__device__ __forceinline__ void tmem_frag4(uint32_t at, float (&f)[4][4]) {
-    uint32_t r[16];
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+// 16 lanes x 16 consecutive columns as fragments: f[i] is (row g, columns 8 i + 2 t, + 1), (row g + 8, the same)
+__device__ __forceinline__ void tmem_frag2(uint32_t at, float (&f)[2][4]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=f"(f[0][0]), "=f"(f[0][1]), "=f"(f[0][2]), "=f"(f[0][3]), "=f"(f[1][0]), "=f"(f[1][1]), "=f"(f[1][2]), "=f"(f[1][3])
                  : "r"(at)
                  : "memory");
-    tmem_wait_ld();
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) f[i][j] = __uint_as_float(r[4 * i + j]);
 }
-// 32 consecutive columns of this thread's lane, from two places, or the sum of two
-__device__ __forceinline__ void tmem_row32(uint32_t at0, uint32_t at1, float (&x)[32], float (&y)[32]) {
-    uint32_t r[4][16];
-    tmem_ld16(at0, r[0]);
-    tmem_ld16(at0 + 16, r[1]);
-    tmem_ld16(at1, r[2]);
-    tmem_ld16(at1 + 16, r[3]);
-    tmem_wait_ld();
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-        x[j] = __uint_as_float(r[j >> 4][j & 15]);
-        y[j] = __uint_as_float(r[2 + (j >> 4)][j & 15]);
-    }
+// 16 consecutive columns of this thread's lane
+__device__ __forceinline__ void tmem_row16(uint32_t at, float (&x)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7]), "=f"(x[8]), "=f"(x[9]),
+                   "=f"(x[10]), "=f"(x[11]), "=f"(x[12]), "=f"(x[13]), "=f"(x[14]), "=f"(x[15])
+                 : "r"(at)
+                 : "memory");
 }
-__device__ __forceinline__ void tmem_row32(uint32_t at0, uint32_t at1, int t0, float (&x)[32]) {
-    float y[32];
-    tmem_row32(at0 + t0, at1 + t0, x, y);
-#pragma unroll
-    for (int j = 0; j < 32; ++j) x[j] += y[j];
-}
-// val[i] summed over the 32 lanes; lane l ends with value l in val[0]: the number of values a lane carries halves at every step
-template <int M, int O = 16>
+// val[i] summed over the 32 lanes; lanes 2 i and 2 i + 1 end with value i in val[0]: the number of values a lane carries halves at
+// every step
+template <int M = 16, int O = 16>
 __device__ __forceinline__ void lanes_total(float* val, int lane) {
-    if constexpr (O > 0) {
+    if constexpr (M > 1) {
         const bool up = lane & O;
 #pragma unroll
         for (int i = 0; i < M / 2; ++i) {
@@ -84,6 +69,8 @@ __device__ __forceinline__ void lanes_total(float* val, int lane) {
             val[i] = keep + __shfl_xor_sync(0xffffffffu, send, O);
         }
         lanes_total<M / 2, O / 2>(val, lane);
+    } else {
+        val[0] += __shfl_xor_sync(0xffffffffu, val[0], O);
     }
 }
 // A and B fragments of 16 rows from `row` on of a [64][128] tile with 128-byte swizzle, channels c..c + 15 (a_frag, b_frag)
@@ -99,7 +86,7 @@ template <int N> __device__ __forceinline__ void registers_down() { asm volatile
 __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrParams p, const Layout lay) {
     using namespace gt;
     extern __shared__ __align__(1024) unsigned char dyn[];
-    __shared__ uint64_t full[RING], empty[RING], tfull[2], tempty[2], accbar, accfree, zready, dqbar, dqfree;
+    __shared__ uint64_t full[RING], empty[RING], tfull[2], tempty[2], accbar, accfree, zready, dqbar, dqfree, sums, gatefree;
     __shared__ uint32_t tmem_s;
     __shared__ float ss[2][CONV / 32];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -115,14 +102,16 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&tfull[i], ROWS / 32);
-            mbar_init(&tempty[i], 1 + MAIN / 32);
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], 2 + MAIN / 32);
         }
         mbar_init(&accbar, 1 + CONV / 32);
         mbar_init(&accfree, MAIN / 32);
         mbar_init(&zready, MAIN / 32);
         mbar_init(&dqbar, 1);
         mbar_init(&dqfree, MAIN / 32);
+        mbar_init(&sums, MAIN / 32);
+        mbar_init(&gatefree, 1);
         mbar_fence_init();
     }
     pdl_wait();
@@ -133,16 +122,31 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
     const int units = p.NT * p.HV, stride = gridDim.x, grp = p.HV / p.H;
     const char* ws = static_cast<const char*>(p.workspace);
     char* sc = static_cast<char*>(p.bwd_scratch);
+    float* red = reinterpret_cast<float*>(dyn + RED);
+    float* dots = reinterpret_cast<float*>(dyn + DOTS);  // q.F, k.E, k.H: [3][4 blocks of channels][64]
+    auto dot = [&](int which, int r) {
+        const float* x = dots + which * 4 * C + r;
+        return (x[0] + x[C]) + (x[2 * C] + x[3 * C]);
+    };
+    auto rows = [&](int which, int r) {  // sum over row r, the blocks of columns up to its own
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s += j <= r >> 4 ? red[(which + j) * C + r] : 0.f;
+        return s;
+    };
+    auto cols = [&](int r) {  // sum over column r, the blocks of rows from its own on
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s += i >= r >> 4 ? red[(R_COL + i) * C + r] : 0.f;
+        return s;
+    };
     bool ok = true;
-    if (warp < MAIN / 32) registers_up<REG_MAIN>();  // (one instruction for the four warps of a group)
-    else if (warp < (MAIN + CONV) / 32) registers_down<REG_CONV>();
-    else registers_down<REG_REST>();
+    if (warp < W_CONV) registers_up<REG_MAIN>();  // (one instruction for the four warps of a group)
+    else if (warp < W_MMA) registers_down<REG_CONV>();
 
     if (warp < MAIN / 32) {
-        const int rb = warp & 3, half = warp >> 2, g = lane >> 2, t = lane & 3, d = tid & 127, t0 = 32 * half;
+        const int rb = warp & 3, ib = warp >> 2, g = lane >> 2, t = lane & 3, d = tid & 127, t0 = 16 * ib;
         const uint32_t tm = tmem0 + ((uint32_t)(rb * 32) << 16);
-        float* red = reinterpret_cast<float*>(dyn + RED);
-        float* dots = reinterpret_cast<float*>(dyn + DOTS);  // q.F, k.E, k.H: [3][4 blocks of channels][64]
         bf16 *sZ = reinterpret_cast<bf16*>(dyn + Z), *sX = reinterpret_cast<bf16*>(dyn + X);
         for (int u = blockIdx.x, it = 0; u < units; u += stride, ++it) {
             const int tb = it & 1, c = u / p.HV, h = u - c * p.HV, kh = h / grp;
@@ -155,11 +159,11 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             ok = bar_and(1, MAIN, ok);  // (also: the unit before is done with Z, X and the sums)
             if (!ok) break;
             // (a wait below that gives up finishes the unit with what there is, for the barriers' sake)
-            const bool any = 2 * half + 1 >= rb;  // rows j = 16 rb.. meet columns i = 32 half.. from the diagonal on
+            const bool any = ib >= rb;  // rows j = 16 rb.. meet columns i = 16 ib.. from the diagonal on
             const bool tiny = __any_sync(0xffffffffu, (2 * lane < ci.len && fabsf(be[2 * lane]) <= 1e-18f) || (2 * lane + 1 < ci.len && fabsf(be[2 * lane + 1]) <= 1e-18f));
-            float qk[4][4], kk[4][4];  // k_j . q_i, k_j . k_i
+            float qk[2][4], kk[2][4];  // k_j . q_i, k_j . k_i
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) qk[j][i] = kk[j][i] = 0.f;
             if (any)
@@ -167,35 +171,42 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 for (int k = 0; k < K; k += 16) {
                     uint32_t fk[4], bq[4], bk[4];
                     swz_a_frag(fk, smem_u32(sk), 16 * rb, k, lane);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        swz_b_frag(bq, smem_u32(sq), t0 + 16 * j, k, lane);
-                        swz_b_frag(bk, smem_u32(sk), t0 + 16 * j, k, lane);
-                        mma(qk[2 * j], fk, bq[0], bq[1]);
-                        mma(qk[2 * j + 1], fk, bq[2], bq[3]);
-                        mma(kk[2 * j], fk, bk[0], bk[1]);
-                        mma(kk[2 * j + 1], fk, bk[2], bk[3]);
-                    }
+                    swz_b_frag(bq, smem_u32(sq), t0, k, lane);
+                    swz_b_frag(bk, smem_u32(sk), t0, k, lane);
+                    mma(qk[0], fk, bq[0], bq[1]);
+                    mma(qk[1], fk, bq[2], bq[3]);
+                    mma(kk[0], fk, bk[0], bk[1]);
+                    mma(kk[1], fk, bk[2], bk[3]);
                 }
             ok = mbar_wait(&accbar, it & 1, p, 1 << 13) && ok;
             tc_fence_after();
             // ---- everything out of the accumulators
-            float fq[32], fk[32], hh[32], dA[4][4], dL[4][4];
-            tmem_row32(tm + T_E, tm + T_E + 64, t0, fk);
-            tmem_row32(tm + T_F + t0, tm + T_H + t0, fq, hh);
-            tmem_frag4(tm + T_DA + t0, dA);
-            tmem_frag4(tm + T_DL + t0, dL);
+            float fq[16], fk[16], hh[16], dA[2][4], dL[2][4];
+            {
+                float e1[16];
+                tmem_row16(tm + T_F + t0, fq);
+                tmem_row16(tm + T_E + t0, fk);
+                tmem_row16(tm + T_E + 64 + t0, e1);
+                tmem_row16(tm + T_H + t0, hh);
+                tmem_frag2(tm + T_DA + t0, dA);
+                tmem_frag2(tm + T_DL + t0, dL);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) fk[j] += e1[j];
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&accfree);
-            {   // ---- pairs of rows: 16 rows j x 32 columns i
+            if (it > 0) ok = mbar_wait(&gatefree, (it - 1) & 1, p, 1 << 11) && ok;  // the sums of the unit before have been used
+            if (any) {  // ---- pairs of rows: 16 rows j x 16 columns i
                 const int r0 = 16 * rb + g;
+                const float gj[2] = {ghi[r0], ghi[r0 + 8]}, lj[2] = {glo[r0], glo[r0 + 8]}, kj[2] = {rk[r0], rk[r0 + 8]};
                 float cn[2] = {0.f, 0.f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if (2 * half + j / 2 < rb) continue;
+                for (int j = 0; j < 2; ++j) {
                     float rn[2] = {0.f, 0.f}, rz[2] = {0.f, 0.f}, rl[2] = {0.f, 0.f};
                     const int i0 = t0 + 8 * j + 2 * t;
+                    const float2 gi = load2(ghi + i0), li = load2(glo + i0), qi = load2(rq + i0), ki = load2(rk + i0), bi = load2(be + i0);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int jj = r0 + 8 * i;
@@ -203,12 +214,14 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
 #pragma unroll
                         for (int y = 0; y < 2; ++y) {
                             const int ii = i0 + y;
-                            const float e = ii >= jj ? expf(ghi[ii] - ghi[jj] + (glo[ii] - glo[jj])) * rk[jj] : 0.f;
-                            z[y] = ii >= jj ? dA[j][2 * i + y] * p.scale * rq[ii] * e : 0.f;
-                            const float l = ii > jj ? -dL[j][2 * i + y] * rk[ii] * e : 0.f;
-                            x[y] = l * be[ii];
+                            // e^(G_i - G_j) / |k_j|
+                            const float e = ii >= jj ? expf((y ? gi.y : gi.x) - gj[i] + ((y ? li.y : li.x) - lj[i])) * kj[i] : 0.f;
+                            const float b = y ? bi.y : bi.x;
+                            z[y] = dA[j][2 * i + y] * (p.scale * (y ? qi.y : qi.x)) * e;
+                            const float l = ii > jj ? -dL[j][2 * i + y] * (y ? ki.y : ki.x) * e : 0.f;
+                            x[y] = l * b;
                             const float zq = z[y] * qk[j][2 * i + y], lk = l * kk[j][2 * i + y];
-                            const float nn = ii > jj ? fmaf(be[ii], lk, zq) : 0.f;
+                            const float nn = ii > jj ? fmaf(b, lk, zq) : 0.f;
                             rz[y] += zq;
                             rl[y] += lk;
                             rn[y] += nn;
@@ -239,106 +252,91 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                         }
                     }
                 }
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&zready);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int o = 1; o < 4; o <<= 1) cn[i] += __shfl_xor_sync(0xffffffffu, cn[i], o);
-                    if (t == 0) red[(R_COL + half) * C + r0 + 8 * i] = cn[i];
+                    if (t == 0) red[(R_COL + ib) * C + r0 + 8 * i] = cn[i];
                 }
+                fence_async_smem();
             }
-            // ---- the products with the states: lane d, 32 rows
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&zready);
+            // ---- the products with the states: lane d, 16 rows
+            uint32_t qk_d[16];  // q and k of this lane's channel
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int at = swz_bf16(t0 + j, d);
+                qk_d[j] = reinterpret_cast<const uint16_t*>(sq)[at] | (uint32_t)reinterpret_cast<const uint16_t*>(sk)[at] << 16;
+            }
             {
-                float s[32];
+                float s[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    fq[j] *= aux[A_OQ * C + t0 + j];
-                    s[j] = fq[j] * __bfloat162float(sq[swz_bf16(t0 + j, d)]);
-                }
-                lanes_total<32>(s, lane);
-                dots[rb * C + t0 + lane] = s[0];
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 oq = *reinterpret_cast<const float4*>(aux + A_OQ * C + t0 + j), gk = *reinterpret_cast<const float4*>(aux + A_GK * C + t0 + j),
+                                 fl = *reinterpret_cast<const float4*>(aux + A_FK * C + t0 + j), bb = *reinterpret_cast<const float4*>(be + t0 + j);
+                    const float *o = &oq.x, *e = &gk.x, *f = &fl.x, *b4 = &bb.x;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    const float k = __bfloat162float(sk[swz_bf16(t0 + j, d)]);
-                    fk[j] *= aux[A_GK * C + t0 + j];
-                    s[j] = fk[j] * k;
-                    hh[j] *= aux[A_FK * C + t0 + j];
-                    fk[j] = hh[j] - be[t0 + j] * fk[j];
-                    hh[j] *= k;
-                }
-                lanes_total<32>(s, lane);
-                dots[(4 + rb) * C + t0 + lane] = s[0];
-                lanes_total<32>(hh, lane);
-                dots[(8 + rb) * C + t0 + lane] = hh[0];
-            }
-            bar_sync(1, MAIN);
-            auto dot = [&](int which, int r) {
-                const float* x = dots + which * 4 * C + r;
-                return (x[0] + x[C]) + (x[2 * C] + x[3 * C]);
-            };
-            auto rows = [&](int which, int r) {  // sum over row r, the blocks of columns up to its own
-                float s = 0.f;
-                for (int j = 0; j <= r >> 4; ++j) s += red[(which + j) * C + r];
-                return s;
-            };
-            auto cols = [&](int r) { return red[R_COL * C + r] + red[(R_COL + 1) * C + r]; };
-            if (warp < 2) {  // a row shorter than 1e-6 is divided by that, whatever its length
-                const int r = tid;
-                const float n = rows(R_N, r), z = rows(R_ZQ, r), dz = red[R_DZ * C + r];
-                const bool l2 = p.flags & KDA_FLAG_QK_L2NORM;
-                red[R_CQ * C + r] = l2 && rq[r] < 1e6f ? rq[r] * rq[r] * (dot(0, r) + z) : 0.f;
-                red[R_CK * C + r] = l2 && rk[r] < 1e6f ? rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + (n - (z - dz)) + cols(r) + dz) : 0.f;
-            } else if (warp == 2) {  // the gate's and beta's gradients, two neighbouring rows per lane
-                const float last = aux[A_LAST * C], total = (ss[tb][0] + ss[tb][1]) + (ss[tb][2] + ss[tb][3]);
-                double dG[2], hsum = 0.0;
-                float db[2];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int r = 2 * lane + i;
-                    const float e = dot(1, r), h1 = dot(2, r);
-                    dG[i] = (double)rows(R_N, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
-                    hsum += h1;
-                    // Y_i . V'_i / beta_i; where beta_i is 0, or so small that the quotient means nothing, Y_i . v_i less what the chunk
-                    // predicts for v_i
-                    if (fabsf(be[r]) > 1e-18f) {
-                        db[i] = red[R_DY * C + r] / be[r];
-                    } else {
-                        const float* y = reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + r) * 128;
-                        float yv = 0.f;
-                        if (r < ci.len) {
-                            for (int x = 0; x < 128; ++x) yv = fmaf(y[x], ldf(static_cast<const bf16*>(p.v) + (((size_t)ci.tok0 + r) * p.HV + h) * 128 + x), yv);
-                            yv += rows(R_B, r) - e;
-                        }
-                        db[i] = yv;
+                    for (int x = 0; x < 4; ++x) {
+                        fq[j + x] *= o[x];
+                        s[j + x] = fk[j + x] * e[x];  // k.E
+                        hh[j + x] *= f[x];            // k.H
+                        fk[j + x] = hh[j + x] - b4[x] * s[j + x];
+                        const float k = __uint_as_float(qk_d[j + x] & 0xffff0000u);
+                        s[j + x] *= k;
+                        hh[j + x] *= k;
                     }
                 }
+                lanes_total(s, lane);
+                lanes_total(hh, lane);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
-                double run = dG[0] + dG[1];
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const double dn = __shfl_down_sync(0xffffffffu, run, o);
-                    if (lane + o < 32) run += dn;
+                for (int j = 15; j > 0; --j) hh[j] = fq[j] * __uint_as_float(qk_d[j] << 16);
+                const float kh = hh[0];
+                hh[0] = fq[0] * __uint_as_float(qk_d[0] << 16);
+                lanes_total(hh, lane);
+                if (!(lane & 1)) {
+                    float* to = dots + rb * C + t0 + (lane >> 1);
+                    to[0] = hh[0];
+                    to[4 * C] = s[0];
+                    to[8 * C] = kh;
                 }
-                run += (double)last * total + hsum;
-                gate_gradients(p, lay, ci, (size_t)u, h, (float)run, (float)(run - dG[0]), db[0], db[1], be[2 * lane], be[2 * lane + 1], lane);
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sums);
             bar_sync(1, MAIN);
+            {   // these rows' factors in the gradient of the L2 norm (a row shorter than 1e-6 is divided by that, whatever its length); the
+                // four warps of a block of rows write the same
+                const int r = t0 + (lane & 15);
+                float cq = 0.f, ck = 0.f;
+                if (p.flags & KDA_FLAG_QK_L2NORM) {
+                    const float z = rows(R_ZQ, r), dz = red[R_DZ * C + r];
+                    if (rq[r] < 1e6f) cq = rq[r] * rq[r] * (dot(0, r) + z);
+                    if (rk[r] < 1e6f) ck = rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + (rows(R_N, r) - (z - dz)) + cols(r) + dz);
+                }
+                red[R_CQ * C + r] = cq;
+                red[R_CK * C + r] = ck;
+                __syncwarp();
+            }
             // ---- the other products
             ok = mbar_wait(&dqbar, it & 1, p, 1 << 14) && ok;
             tc_fence_after();
             {
-                float s[32];
-                tmem_row32(tm + T_DQ + t0, tm + T_DK + t0, s, hh);
+                float s[16];
+                tmem_row16(tm + T_DQ + t0, s);
+                tmem_row16(tm + T_DK + t0, hh);
+                tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&dqfree);
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                    fq[j] += s[j] - red[R_CQ * C + t0 + j] * __bfloat162float(sq[swz_bf16(t0 + j, d)]);
-                    fk[j] += hh[j] - red[R_CK * C + t0 + j] * __bfloat162float(sk[swz_bf16(t0 + j, d)]);
+                for (int j = 0; j < 16; j += 4) {
+                    const float4 cq = *reinterpret_cast<const float4*>(red + R_CQ * C + t0 + j), ck = *reinterpret_cast<const float4*>(red + R_CK * C + t0 + j);
+                    const float *a = &cq.x, *e = &ck.x;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        fq[j + x] += s[j + x] - a[x] * __uint_as_float(qk_d[j + x] << 16);
+                        fk[j + x] += hh[j + x] - e[x] * __uint_as_float(qk_d[j + x] & 0xffff0000u);
+                    }
                 }
             }
             __syncwarp();
@@ -346,13 +344,13 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             if (grp > 1) {  // the group's value heads are added up, and the L2 norm follows, in gdr_heads_kernel (R_CQ, R_CK are 0 then)
                 float* out = reinterpret_cast<float*>(sc + lay.dqk) + (size_t)u * 2 * C * K + d;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = 0; j < 16; ++j) {
                     out[(t0 + j) * K] = fq[j];
                     out[C * K + (t0 + j) * K] = fk[j];
                 }
             } else {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
+                for (int j = 0; j < 16; ++j) {
                     sZ[(t0 + j) * K + d] = __float2bfloat16_rn(fq[j]);
                     sX[(t0 + j) * K + d] = __float2bfloat16_rn(fk[j]);
                 }
@@ -367,24 +365,24 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             }
         }
     } else if (warp < (MAIN + CONV) / 32) {
-        const int t = tid - MAIN, row = t >> 1, e8 = (t & 1) * 8;
-        float x[6][8];  // pieces of eight values: S0 and dS two each, V' and Y
-        uint4 od;       // do
+        const int t = tid - MAIN, t7 = t & 127, row = t7 >> 1, e8 = (t7 & 1) * 8;
+        const bool first = t < 128;  // of V' (the others: of Y and do)
+        float x[3][8];  // pieces of eight values: S0, dS, V' or Y
+        uint4 od;       // of do
         const bf16* dsrc = nullptr;
         auto request = [&](int u, int k) {
-            const float* a = reinterpret_cast<const float*>(ws + lay.S0) + (size_t)u * K * 128 + k * 16 * K + 8 * t;
-            const float* e = reinterpret_cast<const float*>(sc + lay.dS) + (size_t)u * K * 128 + k * 16 * K + 8 * t;
-            load8(a, x[0]);
-            load8(a + 8 * CONV, x[1]);
-            load8(e, x[2]);
-            load8(e + 8 * CONV, x[3]);
-            load8(reinterpret_cast<const float*>(ws + lay.Vn) + (size_t)u * C * 128 + k * 16 * C + 8 * t, x[4]);
-            load8(reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + row) * 128 + k * 16 + e8, x[5]);
-            if (k == 0) {
-                const ChunkInfo ci = chunk_info(p, u / p.HV);
-                dsrc = row < ci.len ? static_cast<const bf16*>(p.grad_o) + (((size_t)ci.tok0 + row) * p.HV + u % p.HV) * 128 + e8 : nullptr;
+            load8(reinterpret_cast<const float*>(ws + lay.S0) + (size_t)u * K * 128 + k * 16 * K + 8 * t, x[0]);
+            load8(reinterpret_cast<const float*>(sc + lay.dS) + (size_t)u * K * 128 + k * 16 * K + 8 * t, x[1]);
+            if (first) {
+                load8(reinterpret_cast<const float*>(ws + lay.Vn) + (size_t)u * C * 128 + k * 16 * C + 8 * t, x[2]);
+            } else {
+                load8(reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + row) * 128 + k * 16 + e8, x[2]);
+                if (k == 0) {
+                    const ChunkInfo ci = chunk_info(p, u / p.HV);
+                    dsrc = row < ci.len ? static_cast<const bf16*>(p.grad_o) + (((size_t)ci.tok0 + row) * p.HV + u % p.HV) * 128 + e8 : nullptr;
+                }
+                od = dsrc ? *reinterpret_cast<const uint4*>(dsrc + k * 16) : make_uint4(0, 0, 0, 0);
             }
-            od = dsrc ? *reinterpret_cast<const uint4*>(dsrc + k * 16) : make_uint4(0, 0, 0, 0);
         };
         auto leave = [&](unsigned char* at, uint32_t part, const float (&v)[8]) {
             uint32_t w[4][3];
@@ -403,16 +401,16 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 if (!ok) break;
                 unsigned char* b = dyn + R0 + st * STAGE;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) s = fmaf(x[j][i], x[2 + j][i], s);
-                    leave(b + S0 + 16 * (t + CONV * j), SPART, x[j]);
-                    leave(b + DS + 16 * (t + CONV * j), SPART, x[2 + j]);
+                for (int i = 0; i < 8; ++i) s = fmaf(x[0][i], x[1][i], s);
+                leave(b + S0 + 16 * t, SPART, x[0]);
+                leave(b + DS + 16 * t, SPART, x[1]);
+                if (first) {
+                    leave(b + V + (t >> 6) * 3072 + 16 * (t & 63), 1024, x[2]);
+                } else {
+                    unsigned char* rows = b + gt::B + (row >> 3) * 256 + (t & 1) * 128 + (row & 7) * 16;
+                    *reinterpret_cast<uint4*>(rows) = od;
+                    leave(rows + YPART, YPART, x[2]);
                 }
-                leave(b + V + (t >> 6) * 3072 + 16 * (t & 63), 1024, x[4]);
-                unsigned char* rows = b + gt::B + (row >> 3) * 256 + (t & 1) * 128 + (row & 7) * 16;
-                *reinterpret_cast<uint4*>(rows) = od;
-                leave(rows + YPART, YPART, x[5]);
                 if (k < 7) request(u, k + 1);
                 else if (u + stride < units) request(u + stride, 0);
                 fence_async_smem();
@@ -421,12 +419,12 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             }
             s = warp_sum(s);
             if (lane == 0) {
-                ss[it & 1][warp - MAIN / 32] = s;
+                ss[it & 1][warp - W_CONV] = s;
                 mbar_arrive(&accbar);
             }
             __syncwarp();
         }
-    } else if (warp == (MAIN + CONV) / 32) {
+    } else if (warp == W_MMA) {
         constexpr uint32_t id192 = make_idesc(128, 192, true, false), id128 = make_idesc(128, 128, true, false), id64 = make_idesc(128, 64, true, false),
                            idH = make_idesc(128, 64, true, true), idA = make_idesc(64, 128, true, false), idL = make_idesc(64, 64, true, false);
         auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
@@ -505,31 +503,78 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             }
         }
         if (ok && it > 0) finish(it - 1);
-    } else if (warp < (MAIN + CONV + 32 + ROWS) / 32) {
-        const int rt = tid - MAIN - CONV - 32;
+    } else if (warp == W_ROWS) {
         for (int u = blockIdx.x, it = 0; u < units; u += stride, ++it) {
             const int tb = it & 1, c = u / p.HV, h = u - c * p.HV, kh = h / grp;
             unsigned char* b = dyn + tb * TILE;
             const ChunkInfo ci = chunk_info(p, c);
             if (it > 1) ok = __all_sync(0xffffffffu, mbar_wait(&tempty[tb], ((it >> 1) & 1) ^ 1, p, 1 << 21));
             if (!ok) break;
-            if (rt == 0 && u + stride < units) {  // the next unit's records on their way into L2
+            const size_t qrow = ((size_t)ci.tok0 * p.H + kh) * K;
+            load_cm<K, 32, true>(reinterpret_cast<bf16*>(b + Q), static_cast<const bf16*>(p.q) + qrow, (size_t)p.H * K, ci.len, lane);
+            load_cm<K, 32, true>(reinterpret_cast<bf16*>(b + KK), static_cast<const bf16*>(p.k) + qrow, (size_t)p.H * K, ci.len, lane);
+            load_words<32>(reinterpret_cast<bf16*>(b + AU), reinterpret_cast<const bf16*>(ws + lay.aux + (size_t)u * AUX * 4), AUX * 4 / 16, lane);
+            cp_async_commit();
+            cp_async_wait<0>();
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&tfull[tb]);
+        }
+    } else if (warp == W_COPY) {  // (nothing waits for it: hints only, a unit ahead of the converters)
+        if (lane == 0)
+            for (int u = blockIdx.x, it = 0; u + stride < units && ok; u += stride, ++it) {
+                ok = mbar_wait(&tfull[it & 1], (it >> 1) & 1, p, 1 << 9);
                 const size_t n = (size_t)u + stride;
                 l2_prefetch_bulk(ws + lay.S0 + n * K * 512, K * 512);
                 l2_prefetch_bulk(sc + lay.dS + n * K * 512, K * 512);
                 l2_prefetch_bulk(ws + lay.Vn + n * C * 512, C * 512);
                 l2_prefetch_bulk(sc + lay.Y + n * C * 512, C * 512);
             }
+    } else {  // gradients of the gate and of beta, two neighbouring rows per lane
+        for (int u = blockIdx.x, it = 0; u < units; u += stride, ++it) {
+            const int tb = it & 1, c = u / p.HV, h = u - c * p.HV;
+            const float *aux = reinterpret_cast<const float*>(dyn + tb * TILE + AU), *be = aux + A_BETA * C;
+            const ChunkInfo ci = chunk_info(p, c);
+            ok = __all_sync(0xffffffffu, mbar_wait(&sums, it & 1, p, 1 << 8));
+            if (!ok) break;
+            const float last = aux[A_LAST * C], total = ((ss[tb][0] + ss[tb][1]) + (ss[tb][2] + ss[tb][3])) + ((ss[tb][4] + ss[tb][5]) + (ss[tb][6] + ss[tb][7]));
+            double dG[2], hsum = 0.0;
+            float db[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int r = 2 * lane + i;
+                const float e = dot(1, r), h1 = dot(2, r);
+                dG[i] = (double)rows(R_N, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
+                hsum += h1;
+                // Y_i . V'_i / beta_i; where beta_i is 0, or so small that the quotient means nothing, Y_i . v_i less what the chunk
+                // predicts for v_i
+                if (fabsf(be[r]) > 1e-18f) {
+                    db[i] = red[R_DY * C + r] / be[r];
+                } else {
+                    const float* y = reinterpret_cast<const float*>(sc + lay.Y) + ((size_t)u * C + r) * 128;
+                    float yv = 0.f;
+                    if (r < ci.len) {
+                        for (int x = 0; x < 128; ++x) yv = fmaf(y[x], ldf(static_cast<const bf16*>(p.v) + (((size_t)ci.tok0 + r) * p.HV + h) * 128 + x), yv);
+                        yv += rows(R_B, r) - e;
+                    }
+                    db[i] = yv;
+                }
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
+            double run = dG[0] + dG[1];
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const double dn = __shfl_down_sync(0xffffffffu, run, o);
+                if (lane + o < 32) run += dn;
+            }
+            run += (double)last * total + hsum;
+            gate_gradients(p, lay, ci, (size_t)u, h, (float)run, (float)(run - dG[0]), db[0], db[1], be[2 * lane], be[2 * lane + 1], lane);
             __syncwarp();
-            const size_t qrow = ((size_t)ci.tok0 * p.H + kh) * K;
-            load_cm<K, ROWS, true>(reinterpret_cast<bf16*>(b + Q), static_cast<const bf16*>(p.q) + qrow, (size_t)p.H * K, ci.len, rt);
-            load_cm<K, ROWS, true>(reinterpret_cast<bf16*>(b + KK), static_cast<const bf16*>(p.k) + qrow, (size_t)p.H * K, ci.len, rt);
-            load_words<ROWS>(reinterpret_cast<bf16*>(b + AU), reinterpret_cast<const bf16*>(ws + lay.aux + (size_t)u * AUX * 4), AUX * 4 / 16, rt);
-            cp_async_commit();
-            cp_async_wait<0>();
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&tfull[tb]);
+            if (lane == 0) {
+                mbar_arrive(&gatefree);
+                mbar_arrive(&tempty[tb]);
+            }
         }
     }
     tc_fence_before();

@@ -47,6 +47,25 @@ __device__ __forceinline__ void store_record(float* rec, int e, int col, int col
 #pragma unroll
     for (int j = 0; j < N; j += 8) store8(rec + rec_idx(e, col + j, cols), x + j);
 }
+// DH key channels from d0 on of column e: states [dk][dv], or [dv][dk] (rows); src NULL: zero
+__device__ __forceinline__ void load_state(const float* src, bool rows, int e, int d0, float (&S)[ft::DH]) {
+#pragma unroll
+    for (int j = 0; j < ft::DH; j += 4) {
+        if (!src) {
+            S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
+        } else if (rows) {
+            const float4 x = *reinterpret_cast<const float4*>(src + (size_t)e * ft::K + d0 + j);
+            S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) S[j + i] = src[(d0 + j + i) * 128 + e];
+        }
+    }
+}
+__device__ __forceinline__ void store_state(float* dst, bool rows, int e, int d0, const float (&S)[ft::DH]) {
+#pragma unroll
+    for (int j = 0; j < ft::DH; ++j) dst[rows ? e * ft::K + d0 + j : (d0 + j) * 128 + e] = S[j];
+}
 __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
 #pragma unroll
     for (int j = 0; j < 16; j += 4) {
@@ -54,21 +73,49 @@ __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
         x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
     }
 }
+// What a CTA walks: chunks cb..ce of a sequence for one value head.
+//   pass 0  whole sequences
+//   pass 1  segments of sequences, for the state they end in: blockIdx.y 0, from zero (the first: from the sequence's own start),
+//           1: from the identity and without values, what the segment makes of the state that it is entered with
+//   pass 2  segments from the states that gdr_borders_kernel has made of that
+// The backward's segments run from their ends to their starts; its pass 1 takes the transitions of the forward.
 struct Walk {
-    int n, h, kh, c0, nc;
+    int n, h, kh, c0, cb, ce, seg;
     long long tok_begin, tok_end;
+    // index of the segment: blockIdx.x is (sequence, head, segment) with `count` segments from `first` on
+    __device__ __forceinline__ void init(const KdaGdrParams& p, const Layout& l, int first, int count) {
+        const int w = blockIdx.x / count;
+        seg = first + blockIdx.x % count;
+        h = w % p.HV; n = w / p.HV; kh = h / (p.HV / p.H);
+        int nc;
+        seq_chunks(p, n, c0, nc);
+        seq_tokens(p, n, tok_begin, tok_end);
+        cb = min((long long)seg * l.seg_len, (long long)nc);
+        ce = seg == l.segs - 1 ? nc : min((long long)(seg + 1) * l.seg_len, (long long)nc);  // (however long the sequence is)
+    }
+    // the segment's matrix in a segment buffer
+    __device__ __forceinline__ size_t slot(const KdaGdrParams& p, const Layout& l, int s) const { return (((size_t)n * p.HV + h) * l.segs + s) * 16384; }
     __device__ __forceinline__ long long tok(int c) const { return tok_begin + (long long)c * C; }
     __device__ __forceinline__ int rows(int c) const { return (int)min((long long)C, tok_end - tok(c)); }
 };
 
-template <bool SAVE>
-__global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
-    using namespace ft;
-    using M = Map;
+// SAVE: records for the backward; OUT: outputs (pass 1 has none)
+template <bool SAVE, bool OUT>
+__global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrParams p, const Layout lay, const int pass) {
+    using ft::MAIN;
+    using ft::PROD;
+    using ft::K;
+    using ft::DH;
+    using M = ft::Map;
+    constexpr int OUTW = ft::OUT;
     extern __shared__ __align__(1024) unsigned char dyn[];
     __shared__ uint64_t full[2], empty[2], sready, ksbar, rready, vbar, wready, sibar, obar, ofree;
     __shared__ uint32_t tmem_s;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    if (pass == 1 && blockIdx.y == 1 && (p.flags & KDA_FLAG_NO_SAVE) && blockIdx.x % (lay.segs - 1) == lay.segs - 2) {
+        pdl_wait();
+        return;  // the last segment's transition is for the backward
+    }
     if (warp == 0) {
         tmem_alloc(&tmem_s, 512);
         tmem_relinquish();
@@ -77,7 +124,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mbar_init(&full[i], 1 + PROD / 32);
-            mbar_init(&empty[i], OUT / 32);
+            mbar_init(&empty[i], OUT ? OUTW / 32 : MAIN / 32);
         }
         mbar_init(&sready, MAIN / 32);
         mbar_init(&rready, MAIN / 32);
@@ -86,14 +133,16 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         mbar_init(&vbar, 1);
         mbar_init(&sibar, 1);
         mbar_init(&obar, 1);
-        mbar_init(&ofree, OUT / 32);
+        mbar_init(&ofree, OUTW / 32);
         mbar_fence_init();
     }
     pdl_wait();
     Walk wk;
-    wk.h = blockIdx.x % p.HV; wk.n = blockIdx.x / p.HV; wk.kh = wk.h / (p.HV / p.H);
-    seq_chunks(p, wk.n, wk.c0, wk.nc);
-    seq_tokens(p, wk.n, wk.tok_begin, wk.tok_end);
+    wk.init(p, lay, pass == 1 && blockIdx.y, pass == 1 ? lay.segs - 1 : lay.segs);
+    const int nc = wk.ce - wk.cb;
+    const bool values = pass != 1 || blockIdx.y == 0;
+    wk.c0 += wk.cb;
+    wk.tok_begin += (long long)wk.cb * C;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -106,20 +155,17 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         const size_t sbase = (size_t)(wk.n * (size_t)p.HV + wk.h) * K * 128;
         const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST;
+        float* const ends = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.segE);
         float S[DH];
+        {   // the state that the walk starts from
+            const bool begin = wk.seg == 0, own = begin || pass != 1;
+            const float* src = !values || !own ? nullptr : begin ? p.h0 ? p.h0 + sbase : nullptr : ends + wk.slot(p, lay, wk.seg - 1);
+            load_state(src, begin && vf, e, d0, S);
+            if (!values)
 #pragma unroll
-        for (int j = 0; j < DH; j += 4) {
-            if (!p.h0) {
-                S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
-            } else if (vf) {
-                const float4 x = *reinterpret_cast<const float4*>(p.h0 + sbase + (size_t)e * K + d0 + j);
-                S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[j + i] = p.h0[sbase + (size_t)(d0 + j + i) * 128 + e];
-            }
+                for (int j = 0; j < DH; ++j) S[j] = d0 + j == e ? 1.f : 0.f;
         }
-        for (int c = 0; c < wk.nc; ++c) {
+        for (int c = 0; c < nc; ++c) {
             const int stage = c & 1, ph = c & 1;
             const unsigned char* b = dyn + stage * M::STAGE;
             const float* aux = reinterpret_cast<const float*>(b + M::AU);
@@ -176,7 +222,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                     f[j] *= x[g][j];
                 }
                 st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, f);
-                st_parts<2>(tm + M::VA + half * 32 + 8 * g, 16, x[g]);
+                if (OUT) st_parts<2>(tm + M::VA + half * 32 + 8 * g, 16, x[g]);
             }
             tmem_wait_st();
             tc_fence_before();
@@ -191,6 +237,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             ok = mbar_wait(&sibar, ph, p, 1 << 15) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
+            if (!OUT && lane == 0) mbar_arrive(&empty[stage]);
 #pragma unroll
             for (int g = 0; g < DH / 16; g += 2) {
                 tmem_ld16(tm + M::SP + half * M::HB + 16 * g, r[0]);
@@ -202,19 +249,19 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                     for (int j = 0; j < 16; ++j) S[16 * (g + i) + j] = fmaf(last, S[16 * (g + i) + j], __uint_as_float(r[i][j]));
             }
         }
-        if (p.ht && ok) {
-#pragma unroll
-            for (int j = 0; j < DH; ++j) p.ht[sbase + (vf ? (size_t)e * K + d0 + j : (size_t)(d0 + j) * 128 + e)] = S[j];
+        if (ok) {
+            if (pass == 1) store_state((values ? ends : reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.segX)) + wk.slot(p, lay, wk.seg), false, e, d0, S);
+            else if (p.ht && wk.seg == lay.segs - 1) store_state(p.ht + sbase, vf, e, d0, S);
         }
-    } else if (warp < (MAIN + OUT) / 32) {
+    } else if (warp < (MAIN + OUTW) / 32) {
         const int e = tid & 127;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
-        for (int c = 0; c < wk.nc; ++c) {
+        for (int c = 0; c < (OUT ? nc : 0); ++c) {
             const int stage = c & 1;
             const float* oq = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_OQ * C;
             ok = mbar_wait(&obar, c & 1, p, 1 << 16) && ok;
-            ok = bar_and(2, OUT, ok);  // (also: the tile of the previous chunk has been stored)
+            ok = bar_and(2, OUTW, ok);  // (also: the tile of the previous chunk has been stored)
             if (!ok) break;
             tc_fence_after();
             uint32_t o[C / 2];
@@ -242,19 +289,19 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                 reinterpret_cast<uint16_t*>(tile)[(2 * j) * 128 + e] = (uint16_t)o[j];
                 reinterpret_cast<uint16_t*>(tile)[(2 * j + 1) * 128 + e] = (uint16_t)(o[j] >> 16);
             }
-            bar_sync(2, OUT);
+            bar_sync(2, OUTW);
             const int rows = wk.rows(c);
             bf16* dst = static_cast<bf16*>(p.o) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
 #pragma unroll
-            for (int i = e; i < C * 16; i += OUT) {
+            for (int i = e; i < C * 16; i += OUTW) {
                 const int rr = i >> 4, cc = (i & 15) * 8;
                 if (rr < rows) *reinterpret_cast<uint4*>(dst + (size_t)rr * p.HV * 128 + cc) = *reinterpret_cast<const uint4*>(tile + rr * 128 + cc);
             }
         }
-    } else if (warp < (MAIN + OUT + PROD) / 32) {
-        const int pt = tid - MAIN - OUT;
+    } else if (warp < (MAIN + OUTW + PROD) / 32) {
+        const int pt = tid - MAIN - OUTW;
         int c = 0;
-        for (; c < wk.nc; ++c) {
+        for (; c < nc; ++c) {
             const int stage = c & 1;
             unsigned char* b = dyn + stage * M::STAGE;
             if (c > 1) ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((c >> 1) & 1) ^ 1, p, 1 << 17));
@@ -262,16 +309,16 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
             const int rows = wk.rows(c);
             if (pt == 0) {
-                mbar_expect_tx(&full[stage], 5 * M::MAT + AUX * 4);
+                mbar_expect_tx(&full[stage], (OUT ? 5 : 3) * M::MAT + AUX * 4);
                 tma_load_1d(b + M::TM, ws + lay.T + unit * 3 * M::MAT, 3 * M::MAT, &full[stage]);
                 tma_load_1d(b + M::AU, ws + lay.aux + unit * AUX * 4, AUX * 4, &full[stage]);
-                tma_load_1d(b + M::AM, ws + lay.A + unit * 3 * M::MAT, 2 * M::MAT, &full[stage]);
+                if (OUT) tma_load_1d(b + M::AM, ws + lay.A + unit * 3 * M::MAT, 2 * M::MAT, &full[stage]);
             }
             __syncwarp();
             const size_t krow = ((size_t)wk.tok(c) * p.H + wk.kh) * K;
             load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::KK), static_cast<const bf16*>(p.k) + krow, (size_t)p.H * K, rows, pt);
-            load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
-            load_cm<128, PROD>(reinterpret_cast<bf16*>(b + M::V), static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
+            if (OUT) load_cm<K, PROD>(reinterpret_cast<bf16*>(b + M::Q), static_cast<const bf16*>(p.q) + krow, (size_t)p.H * K, rows, pt);
+            if (values) load_cm<128, PROD>(reinterpret_cast<bf16*>(b + M::V), static_cast<const bf16*>(p.v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128,
                                (size_t)p.HV * 128, rows, pt);
             cp_async_commit();
             cp_async_wait<0>();
@@ -283,7 +330,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         for (int i = max(c - 2, 0); !ok && i < c; ++i) mbar_wait(&full[i & 1], (i >> 1) & 1, p, 1 << 17);
     } else {
         constexpr uint32_t id64 = make_idesc(128, 64, false, false), idu = make_idesc(128, DH, false, true);
-        for (int c = 0; c < wk.nc && ok; ++c) {
+        for (int c = 0; c < nc && ok; ++c) {
             const int stage = c & 1, ph = c & 1;
             const uint32_t b = smem_u32(dyn + stage * M::STAGE);
             auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
@@ -313,23 +360,24 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                         first = false;
                     }
             };
-            if (!wait(&sready, ph, 1 << 19) || (c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
+            if (!wait(&sready, ph, 1 << 19) || (OUT && c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
             if (elect_one()) {
                 with_rows(M::KS, M::KK, 3);
                 mma_commit(&ksbar);
                 // v^T T'^T (the parts of V' that were here have been used: their products' outputs have been read)
+                if (values)
 #pragma unroll
                 for (int i = 2; i >= 0; --i)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
                         mma_ss(tmem0 + M::VA + 16 * s, make_desc(b + M::V + s * 4096, 2048, 128), make_desc(b + M::TM + i * M::MAT + s * 256 + s * 2048, 128, 1024),
                                make_idesc(128, 64 - 16 * s, true, false), i < 2 || s > 0);
-                with_rows(M::QS, M::Q, 2);
+                if (OUT) with_rows(M::QS, M::Q, 2);
             }
             __syncwarp();
             if (!wait(&rready, ph, 1 << 21)) break;
             if (elect_one()) {
-                with_matrix(M::VA, [](int i, int s) { return M::R + i * 32 + s * 8; }, M::TM, 3, false);
+                with_matrix(M::VA, [](int i, int s) { return M::R + i * 32 + s * 8; }, M::TM, 3, !values);
                 mma_commit(&vbar);
             }
             __syncwarp();
@@ -344,8 +392,10 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                             mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + M::R + i * 32 + s * 8,
                                    make_desc(b + M::KK + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu, i < 2 || s > 0);
                 mma_commit(&sibar);
+                if (OUT) {
                 with_matrix(M::AV, [](int i, int s) { return M::VA + (s >> 1) * 32 + i * 16 + (s & 1) * 8; }, M::AM, 2, true);
                 mma_commit(&obar);
+                }
             }
             __syncwarp();
         }
@@ -360,10 +410,6 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
 //   dS^T <- e^G_last dS^T + (scale e^G / |q| do)^T q + X^T k
 // The products with do only are issued beside the chain dS - dS k - dV' - dV' T - X - X k - dS.
 namespace bt {
-using ft::MAIN;
-using ft::OUT;
-using ft::PROD;
-using ft::NTHR;
 using ft::K;
 using ft::DH;
 struct Map {
@@ -376,9 +422,15 @@ struct Map {
 };
 }  // namespace bt
 
-__global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrParams p, const Layout lay) {
-    using namespace bt;
-    using M = Map;
+// OUT: dv and the records (pass 1 has none)
+template <bool OUT>
+__global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrParams p, const Layout lay, const int pass) {
+    using ft::MAIN;
+    using ft::PROD;
+    using ft::K;
+    using ft::DH;
+    using M = bt::Map;
+    constexpr int OUTW = ft::OUT;
     extern __shared__ __align__(1024) unsigned char dyn[];
     __shared__ uint64_t full[2], empty[2], sready, kdbar, dosready, dvready, ybar, xready, sibar, ofree;
     __shared__ uint32_t tmem_s;
@@ -391,7 +443,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mbar_init(&full[i], 1 + PROD / 32);
-            mbar_init(&empty[i], (MAIN + OUT) / 32);
+            mbar_init(&empty[i], (MAIN + (OUT ? OUTW : 0)) / 32);
         }
         mbar_init(&sready, MAIN / 32);
         mbar_init(&dosready, MAIN / 32);
@@ -400,14 +452,15 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         mbar_init(&kdbar, 1);
         mbar_init(&ybar, 1);
         mbar_init(&sibar, 1);
-        mbar_init(&ofree, OUT / 32);
+        mbar_init(&ofree, OUTW / 32);
         mbar_fence_init();
     }
     pdl_wait();
     Walk wk;
-    wk.h = blockIdx.x % p.HV; wk.n = blockIdx.x / p.HV; wk.kh = wk.h / (p.HV / p.H);
-    seq_chunks(p, wk.n, wk.c0, wk.nc);
-    seq_tokens(p, wk.n, wk.tok_begin, wk.tok_end);
+    wk.init(p, lay, pass == 1, pass == 1 ? lay.segs - 1 : lay.segs);
+    const int nc = wk.ce - wk.cb;
+    wk.c0 += wk.cb;
+    wk.tok_begin += (long long)wk.cb * C;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -421,22 +474,12 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         const int e = tid & 127, half = warp >> 2, d0 = half * DH, t0 = half * 32;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         const size_t sbase = (size_t)(wk.n * (size_t)p.HV + wk.h) * K * 128;
-        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST;
+        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST, end = wk.seg == lay.segs - 1;
+        float* const starts = reinterpret_cast<float*>(sc + lay.segF);
         float S[DH];
-#pragma unroll
-        for (int j = 0; j < DH; j += 4) {
-            if (!p.grad_ht) {
-                S[j] = S[j + 1] = S[j + 2] = S[j + 3] = 0.f;
-            } else if (vf) {
-                const float4 x = *reinterpret_cast<const float4*>(p.grad_ht + sbase + (size_t)e * K + d0 + j);
-                S[j] = x.x; S[j + 1] = x.y; S[j + 2] = x.z; S[j + 3] = x.w;
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) S[j + i] = p.grad_ht[sbase + (size_t)(d0 + j + i) * 128 + e];
-            }
-        }
-        for (int i = 0; i < wk.nc; ++i) {
-            const int c = wk.nc - 1 - i, stage = i & 1, ph = i & 1;
+        load_state(end ? p.grad_ht ? p.grad_ht + sbase : nullptr : pass == 1 ? nullptr : starts + wk.slot(p, lay, wk.seg + 1), end && vf, e, d0, S);
+        for (int i = 0; i < nc; ++i) {
+            const int c = nc - 1 - i, stage = i & 1, ph = i & 1;
             const unsigned char* b = dyn + stage * M::STAGE;
             const float* aux = reinterpret_cast<const float*>(b + M::AU);
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
@@ -466,7 +509,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&dosready);
-            store_record<DH>(reinterpret_cast<float*>(sc + lay.dS) + unit * K * 128, e, d0, K, S);
+            if (OUT) store_record<DH>(reinterpret_cast<float*>(sc + lay.dS) + unit * K * 128, e, d0, K, S);
             // ---- dV'
             ok = mbar_wait(&kdbar, ph, p, 1 << 13) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
@@ -522,20 +565,20 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                     for (int j = 0; j < 16; ++j) S[16 * (g + x) + j] = fmaf(last, S[16 * (g + x) + j], __uint_as_float(r[x][j]));
             }
         }
-        if (p.grad_h0 && ok) {
-#pragma unroll
-            for (int j = 0; j < DH; ++j) p.grad_h0[sbase + (vf ? (size_t)e * K + d0 + j : (size_t)(d0 + j) * 128 + e)] = S[j];
+        if (ok) {
+            if (pass == 1) store_state(starts + wk.slot(p, lay, wk.seg), false, e, d0, S);
+            else if (p.grad_h0 && wk.seg == 0) store_state(p.grad_h0 + sbase, vf, e, d0, S);
         }
-    } else if (warp < (MAIN + OUT) / 32) {
+    } else if (warp < (MAIN + OUTW) / 32) {
         const int e = tid & 127;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         bf16* tile = reinterpret_cast<bf16*>(dyn + M::OT);
-        for (int i = 0; i < wk.nc; ++i) {
-            const int c = wk.nc - 1 - i, stage = i & 1;
+        for (int i = 0; i < (OUT ? nc : 0); ++i) {
+            const int c = nc - 1 - i, stage = i & 1;
             const float* be = reinterpret_cast<const float*>(dyn + stage * M::STAGE + M::AU) + A_BETA * C;
             const size_t unit = (size_t)(wk.c0 + c) * p.HV + wk.h;
             ok = mbar_wait(&ybar, i & 1, p, 1 << 16) && ok;
-            ok = bar_and(2, OUT, ok);
+            ok = bar_and(2, OUTW, ok);
             if (!ok) break;
             tc_fence_after();
             uint32_t y[C / 16][16];
@@ -560,20 +603,20 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&empty[stage]);
-            bar_sync(2, OUT);
+            bar_sync(2, OUTW);
             const int rows = wk.rows(c);
             bf16* dst = static_cast<bf16*>(p.grad_v) + ((size_t)wk.tok(c) * p.HV + wk.h) * 128;
 #pragma unroll
-            for (int x = e; x < C * 16; x += OUT) {
+            for (int x = e; x < C * 16; x += OUTW) {
                 const int rr = x >> 4, cc = (x & 15) * 8;
                 if (rr < rows) *reinterpret_cast<uint4*>(dst + (size_t)rr * p.HV * 128 + cc) = *reinterpret_cast<const uint4*>(tile + rr * 128 + cc);
             }
         }
-    } else if (warp < (MAIN + OUT + PROD) / 32) {
-        const int pt = tid - MAIN - OUT;
+    } else if (warp < (MAIN + OUTW + PROD) / 32) {
+        const int pt = tid - MAIN - OUTW;
         int i = 0;
-        for (; i < wk.nc; ++i) {
-            const int c = wk.nc - 1 - i, stage = i & 1;
+        for (; i < nc; ++i) {
+            const int c = nc - 1 - i, stage = i & 1;
             unsigned char* b = dyn + stage * M::STAGE;
             if (i > 1) ok = __all_sync(0xffffffffu, mbar_wait(&empty[stage], ((i >> 1) & 1) ^ 1, p, 1 << 17));
             if (!ok) break;
@@ -600,7 +643,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         for (int x = max(i - 2, 0); !ok && x < i; ++x) mbar_wait(&full[x & 1], (x >> 1) & 1, p, 1 << 17);
     } else {
         constexpr uint32_t id64 = make_idesc(128, 64, false, false), idu = make_idesc(128, DH, false, true);
-        for (int i = 0; i < wk.nc && ok; ++i) {
+        for (int i = 0; i < nc && ok; ++i) {
             const int stage = i & 1, ph = i & 1;
             const uint32_t b = smem_u32(dyn + stage * M::STAGE);
             auto wait = [&](uint64_t* bar, uint32_t parity, int what) {
@@ -630,7 +673,7 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                                make_desc(b + M::AM + x * M::MAT + s * 2048, 1024, 128), make_idesc(128, 16 * (s + 1), true, true), x < 2 || s < 3);
             }
             __syncwarp();
-            if (!wait(&sready, ph, 1 << 19) || (i > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
+            if (!wait(&sready, ph, 1 << 19) || (OUT && i > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
             if (elect_one()) {
 #pragma unroll
                 for (int x = 2; x >= 0; --x)
@@ -673,21 +716,93 @@ __global__ void __launch_bounds__(bt::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
     if (warp == 0) tmem_dealloc(tmem0, 512);
 }
 
-template <bool SAVE>
-static cudaError_t launch_fwd(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    cudaError_t e = allow_smem(gdr_fwd_tc_kernel<SAVE>, ft::Map::TOTAL);
-    if (e != cudaSuccess) return e;
-    return launch_dependent(gdr_fwd_tc_kernel<SAVE>, p.N * p.HV, ft::NTHR, ft::Map::TOTAL, s, p, l);
+// States at the segments' borders, 8 columns of one (sequence, head) per CTA: forward, E_j <- X_j E_{j-1} + E_j for j = 1, 2, ..; backward
+// (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  FP32 multiply-adds; the next segment's X arrives meanwhile.
+constexpr int LDX = 132;  // floats per row of X
+template <bool TR>
+__global__ void __launch_bounds__(256) gdr_borders_kernel(const Layout lay, float* M, const float* X) {
+    extern __shared__ __align__(16) float sm[];  // X twice, then the columns [128][8]
+    float* cols = sm + 2 * 128 * LDX;
+    const int tid = threadIdx.x, d = tid >> 1, c4 = (tid & 1) * 4, c0 = (blockIdx.x & 15) * 8;
+    const size_t base = (size_t)(blockIdx.x >> 4) * lay.segs * 16384;
+    const int steps = lay.segs - 2;  // (segment 0 of the forward, the last of the backward are done)
+    pdl_wait();
+    auto seg = [&](int i) { return TR ? lay.segs - 2 - i : 1 + i; };
+    auto request = [&](int i) {
+        const float* x = X + base + (size_t)seg(i) * 16384;
+        for (int q = tid; q < 4096; q += 256) cp_async16_z(sm + (i & 1) * 128 * LDX + (q >> 5) * LDX + (q & 31) * 4, x + 4 * q, true);
+        cp_async_commit();
+    };
+    auto at = [&](int s) { return reinterpret_cast<float4*>(M + base + (size_t)s * 16384 + d * 128 + c0 + c4); };
+    if (steps > 0) request(0);
+    *reinterpret_cast<float4*>(cols + d * 8 + c4) = *at(TR ? lay.segs - 1 : 0);
+    for (int i = 0; i < steps; ++i) {
+        if (i + 1 < steps) request(i + 1);
+        else cp_async_commit();
+        float4 acc = *at(seg(i));
+        cp_async_wait<1>();
+        __syncthreads();
+        const float* x = sm + (i & 1) * 128 * LDX;
+#pragma unroll 8
+        for (int k = 0; k < 128; k += 4) {
+            float w[4];
+            if (TR) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = x[(k + j) * LDX + d];
+            } else {
+                const float4 v = *reinterpret_cast<const float4*>(x + d * LDX + k);
+                w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float4 s = *reinterpret_cast<const float4*>(cols + (k + j) * 8 + c4);
+                acc.x = fmaf(w[j], s.x, acc.x); acc.y = fmaf(w[j], s.y, acc.y); acc.z = fmaf(w[j], s.z, acc.z); acc.w = fmaf(w[j], s.w, acc.w);
+            }
+        }
+        __syncthreads();
+        *reinterpret_cast<float4*>(cols + d * 8 + c4) = acc;
+        *at(seg(i)) = acc;
+    }
+}
+
+template <class Kernel>
+static cudaError_t walk(Kernel* k, dim3 grid, int bytes, const KdaGdrParams& p, const Layout& l, int pass, cudaStream_t s) {
+    const cudaError_t e = allow_smem(k, bytes);
+    return e == cudaSuccess ? launch_dependent(k, grid, ft::NTHR, bytes, s, p, l, pass) : e;
+}
+template <bool TR>
+static cudaError_t borders(const KdaGdrParams& p, const Layout& l, float* m, cudaStream_t s) {
+    constexpr int bytes = (2 * 128 * LDX + 128 * 8) * 4;
+    if (l.segs < 3) return cudaSuccess;
+    const cudaError_t e = allow_smem(gdr_borders_kernel<TR>, bytes);
+    const float* x = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + l.segX);
+    return e == cudaSuccess ? launch_dependent(gdr_borders_kernel<TR>, p.N * p.HV * 16, 256, bytes, s, l, m, x) : e;
 }
 
 cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    return p.flags & KDA_FLAG_NO_SAVE ? launch_fwd<false>(p, l, s) : launch_fwd<true>(p, l, s);
+    const unsigned walks = (unsigned)(p.N * p.HV);
+    const bool save = !(p.flags & KDA_FLAG_NO_SAVE);
+    cudaError_t e = cudaSuccess;
+    if (l.segs > 1) {
+        // (two segments need no transition in the forward)
+        e = walk(gdr_fwd_tc_kernel<false, false>, dim3(walks * (l.segs - 1), save || l.segs > 2 ? 2 : 1), ft::Map::TOTAL, p, l, 1, s);
+        if (e == cudaSuccess) e = borders<false>(p, l, reinterpret_cast<float*>(static_cast<char*>(p.workspace) + l.segE), s);
+    }
+    if (e != cudaSuccess) return e;
+    const dim3 grid(walks * l.segs);
+    const int pass = l.segs > 1 ? 2 : 0;
+    return save ? walk(gdr_fwd_tc_kernel<true, true>, grid, ft::Map::TOTAL, p, l, pass, s) : walk(gdr_fwd_tc_kernel<false, true>, grid, ft::Map::TOTAL, p, l, pass, s);
 }
 
 cudaError_t bwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
-    cudaError_t e = allow_smem(gdr_bwd_tc_kernel, bt::Map::TOTAL);
+    const unsigned walks = (unsigned)(p.N * p.HV);
+    cudaError_t e = cudaSuccess;
+    if (l.segs > 1) {
+        e = walk(gdr_bwd_tc_kernel<false>, dim3(walks * (l.segs - 1)), bt::Map::TOTAL, p, l, 1, s);
+        if (e == cudaSuccess) e = borders<true>(p, l, reinterpret_cast<float*>(static_cast<char*>(p.bwd_scratch) + l.segF), s);
+    }
     if (e != cudaSuccess) return e;
-    return launch_dependent(gdr_bwd_tc_kernel, p.N * p.HV, bt::NTHR, bt::Map::TOTAL, s, p, l);
+    return walk(gdr_bwd_tc_kernel<true>, dim3(walks * l.segs), bt::Map::TOTAL, p, l, l.segs > 1 ? 2 : 0, s);
 }
 
 }  // namespace gdr

@@ -31,6 +31,7 @@ struct Spec {
     bool want_state = false;
     bool covered = true;  // every row belongs to a sequence
     int64_t N = 0, NT = 0;
+    int64_t longest = 0;  // chunks of the longest packed document
 };
 
 // sizes and types of one call; multi: q [B, T, H, K], else [N, H, K].  Returns {B, T, H, HV, K, V}.
@@ -80,7 +81,7 @@ KdaGdrParams params(const Inputs& in, const Spec& sp, int flags) {
     KdaGdrParams p{};
     p.B = (int)in.q.size(0); p.T = (int)in.q.size(1); p.H = (int)in.q.size(2); p.dk = (int)in.q.size(3);
     p.HV = (int)in.v.size(2); p.dv = (int)in.v.size(3);
-    p.N = (int)sp.N; p.NT = (int)sp.NT;
+    p.N = (int)sp.N; p.NT = (int)sp.NT; p.max_chunks = (int)sp.longest;
     p.dtype = code(in.q.scalar_type()); p.g_dtype = code(in.g.scalar_type());
     p.flags = flags;
     p.scale = (float)sp.scale;
@@ -182,6 +183,7 @@ struct ChunkGdr : torch::autograd::Function<ChunkGdr> {
         ctx->saved_data["flags"] = (int64_t)sp.flags;
         ctx->saved_data["N"] = sp.N;
         ctx->saved_data["NT"] = sp.NT;
+        ctx->saved_data["longest"] = sp.longest;
         ctx->saved_data["covered"] = sp.covered;
         if (f.ht.defined()) return {f.o, f.ht};
         return {f.o};
@@ -194,6 +196,7 @@ struct ChunkGdr : torch::autograd::Function<ChunkGdr> {
         sp.flags = (int)ctx->saved_data["flags"].toInt();
         sp.N = ctx->saved_data["N"].toInt();
         sp.NT = ctx->saved_data["NT"].toInt();
+        sp.longest = ctx->saved_data["longest"].toInt();
         sp.covered = ctx->saved_data["covered"].toBool();
         c10::cuda::CUDAGuard guard(in.q.device());
         const Grads r = run_bwd(in, sp, s[12], grads[0], grads.size() > 1 ? grads[1] : Tensor());
@@ -205,7 +208,7 @@ struct ChunkGdr : torch::autograd::Function<ChunkGdr> {
 std::tuple<Tensor, OptTensor> chunk_gdr(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
                                         OptTensor A_log, OptTensor dt_bias, OptTensor h0, std::optional<double> scale, int64_t flags,
                                         bool want_state, OptTensor cu, OptTensor chunk_seq, OptTensor seq_off, OptTensor chunk_tab,
-                                        int64_t NT, bool covered) {
+                                        int64_t NT, int64_t longest, bool covered) {
     const auto [B, T, H, HV, K, V] = check_shapes("chunk_gated_delta_rule", q, k, v, g, beta, true);
     Spec sp;
     Inputs tables;
@@ -216,6 +219,7 @@ std::tuple<Tensor, OptTensor> chunk_gdr(const Tensor& q, const Tensor& k, const 
         tables.cu = *cu; tables.chunk_seq = *chunk_seq; tables.seq_off = *seq_off; tables.chunk_tab = *chunk_tab;
         sp.N = cu->numel() - 1;
         sp.NT = NT;
+        sp.longest = longest;
         sp.covered = covered;
     }
     check_gate(flags, A_log, dt_bias, HV);

@@ -46,7 +46,7 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
     state or a gradient in FP32 is one to FP32 accuracy.  Differentiated calls keep about (4 K V + 256 V + 33000) bytes per 64 tokens
     and value head for the backward.  Returns ``(o [B, T, HV, V], final_state or None)``.
     """
-    tables = (None, None, None, None, 0, True)
+    tables = (None, None, None, None, 0, 0, True)
     if cu_seqlens is not None or cu_seqlens_cpu is not None:
         host = cu_seqlens_cpu if cu_seqlens_cpu is not None else cu_seqlens.cpu()
         if host.dim() != 1 or host.numel() < 2:
@@ -58,9 +58,9 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
         if q.shape[0] != 1:
             raise ValueError(f"The batch size is expected to be 1 rather than {q.shape[0]} when using `cu_seqlens`.")
         tokens = q.shape[0] * q.shape[1]
-        seq, off, nt, tab, _ = _chunk_tables(None, host, q.device, tokens)
+        seq, off, nt, tab, longest = _chunk_tables(None, host, q.device, tokens)
         cu = tuple(int(x) for x in host.tolist())
-        tables = (_offsets(cu, q.device.index or 0), seq, off, tab, nt, cu[0] == 0 and cu[-1] == tokens)
+        tables = (_offsets(cu, q.device.index or 0), seq, off, tab, nt, longest, cu[0] == 0 and cu[-1] == tokens)
     return _lib.host().chunk_gdr(q, k, v, g, beta, A_log, dt_bias, initial_state, scale,
                                  _flags(use_qk_l2norm_in_kernel, use_gate_in_kernel, use_beta_sigmoid_in_kernel, state_v_first),
                                  bool(output_final_state), *tables)
