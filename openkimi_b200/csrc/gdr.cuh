@@ -40,24 +40,28 @@ struct Layout {
 inline int longest(const KdaGdrParams& p) {  // chunks of the longest sequence, 0: not known
     return p.cu_seqlens ? p.max_chunks : (p.T + C - 1) / C;
 }
-// Segments per sequence of the walks on tcgen05 (gdr_tc.cu).  A walk is a chain of chunks; with fewer walks than SMs a sequence is cut
-// into n segments that are walked twice: from zero (and from the identity, for what a segment does to the state that it is entered
-// with), and again from the states that follow.  Estimated with what a chunk (3.7 us without outputs, 4.3 us with), a border (1.5 us)
-// and the launches (8 us) cost; 8 walks of 512 chunks, the whole forward: 2312 -> 460 us.
+// Segments of the longest sequence in the walks on tcgen05 (gdr_tc.cu).  A walk is a chain of chunks; where walks are few, or one is
+// much longer than its share, sequences are cut into segments of equal length that are walked twice: from zero (and from the identity,
+// for what a segment does to the state that it is entered with), and again from the states that follow.  Estimated with what a chunk
+// costs (3.2 us without outputs, 3.7 us with), a border (3.3 us) and the launches (12 us): equal sequences go in waves, packed ones
+// fill the SMs up to half a segment.  8 walks of 512 chunks, forward: 2312 -> 553 us.
 inline int segment_count(const KdaGdrParams& p) {
     if (!on_tc(p)) return 1;
     const int nc = longest(p), sms = sm_count();
-    const long long walks = (long long)p.N * p.HV;
-    if (nc < 4 || walks * 2 > sms) return 1;
-    double best = nc * 4.3;
+    if (nc < 4) return 1;
+    const double walks = (double)p.N * p.HV, all = (double)p.NT * p.HV;
+    auto waves = [&](double ctas, double len) { return (double)(long long)((ctas + sms - 1) / sms) * len; };
+    auto fill = [&](double chunks, double len) { return chunks <= 0 ? 0.0 : chunks / sms + len / 2 > len ? chunks / sms + len / 2 : len; };
+    double best = 3.7 * (p.cu_seqlens ? fill(all, nc) : waves(walks, nc));
     int n = 1;
     for (int s = 2; s <= nc / 2 && s <= 64; ++s) {
         const int len = (nc + s - 1) / s;
-        const double waves1 = (double)((walks * (2 * s - 3) + sms - 1) / sms), waves2 = (double)((walks * s + sms - 1) / sms);
-        const double t = len * (3.7 * waves1 + 4.3 * waves2) + 1.5 * s + 8.0;
+        const double t1 = p.cu_seqlens ? fill(2 * (all - 0.75 * walks * len), len) : waves(walks * (2 * s - 3), len),
+                     t2 = p.cu_seqlens ? fill(all, len) : waves(walks * s, len), t = 3.2 * t1 + 3.7 * t2 + 3.3 * (s - 2) + 12.0;
         if (t < best) best = t, n = s;
     }
-    return n;
+    // (segment buffers of 64 KB a segment and head)
+    return walks * n > 8192 ? 1 : n;
 }
 inline Layout layout(const KdaGdrParams& p) {
     const size_t n = (size_t)p.NT * p.HV, mat = 3 * (on_tc(p) ? SQ : TRI) * 2;

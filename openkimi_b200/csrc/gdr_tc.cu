@@ -21,8 +21,8 @@ struct Map {
     static constexpr uint32_t KK = 0, Q = ROWS, V = 2 * ROWS, TM = V + C * 256, AM = TM + 3 * MAT, AU = AM + 2 * MAT, STAGE = AU + AUX * 4;
     static constexpr uint32_t OT = 2 * STAGE, TOTAL = OT + C * 256;
     // tensor memory columns.  S parts: per half three blocks of DH / 2; over them, once S k and S q are done, the update (DH columns).
-    // V' A^T over S k, W over R, the parts of V' over V' itself, each half of the rows over its own columns.
-    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, KS = 2 * HB, AV = KS, QS = KS + 64, VA = QS + 64, R = VA + 64, COLS = R + 96;
+    // W and then V' A^T over R, the parts of V' over V' itself, each half of the rows over its own columns.
+    static constexpr uint32_t SP = 0, HB = 3 * DH / 2, KS = 2 * HB, QS = KS + 64, VA = QS + 64, R = VA + 64, AV = R, COLS = R + 96;
     static_assert(COLS <= 512 && TOTAL <= 232448, "fits");
 };
 }  // namespace ft
@@ -73,6 +73,17 @@ __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
         x[j] = v.x; x[j + 1] = v.y; x[j + 2] = v.z; x[j + 3] = v.w;
     }
 }
+// this warp has read what the products waiting for `bar` may not hold up: loads from tensor memory wait for the MMAs issued before them,
+// so products that are not on the chain are issued behind a load, beside the conversion that follows it
+__device__ __forceinline__ void signal(uint64_t* bar, int lane) {
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar);
+}
+
+// last segment that a sequence of nc chunks reaches (however long it is: the count is a hint's)
+__device__ __forceinline__ int last_segment(int nc, const Layout& l) { return l.segs == 1 ? 0 : max(0, min(l.segs, (nc + l.seg_len - 1) / l.seg_len) - 1); }
+
 // What a CTA walks: chunks cb..ce of a sequence for one value head.
 //   pass 0  whole sequences
 //   pass 1  segments of sequences, for the state they end in: blockIdx.y 0, from zero (the first: from the sequence's own start),
@@ -80,7 +91,7 @@ __device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
 //   pass 2  segments from the states that gdr_borders_kernel has made of that
 // The backward's segments run from their ends to their starts; its pass 1 takes the transitions of the forward.
 struct Walk {
-    int n, h, kh, c0, cb, ce, seg;
+    int n, h, kh, c0, cb, ce, seg, last;  // last: the sequence's last segment, of those that it reaches
     long long tok_begin, tok_end;
     // index of the segment: blockIdx.x is (sequence, head, segment) with `count` segments from `first` on
     __device__ __forceinline__ void init(const KdaGdrParams& p, const Layout& l, int first, int count) {
@@ -90,8 +101,9 @@ struct Walk {
         int nc;
         seq_chunks(p, n, c0, nc);
         seq_tokens(p, n, tok_begin, tok_end);
+        last = last_segment(nc, l);
         cb = min((long long)seg * l.seg_len, (long long)nc);
-        ce = seg == l.segs - 1 ? nc : min((long long)(seg + 1) * l.seg_len, (long long)nc);  // (however long the sequence is)
+        ce = seg == last ? nc : min((long long)(seg + 1) * l.seg_len, (long long)nc);
     }
     // the segment's matrix in a segment buffer
     __device__ __forceinline__ size_t slot(const KdaGdrParams& p, const Layout& l, int s) const { return (((size_t)n * p.HV + h) * l.segs + s) * 16384; }
@@ -109,13 +121,18 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
     using M = ft::Map;
     constexpr int OUTW = ft::OUT;
     extern __shared__ __align__(1024) unsigned char dyn[];
-    __shared__ uint64_t full[2], empty[2], sready, ksbar, rready, vbar, wready, sibar, obar, ofree;
+    __shared__ uint64_t full[2], empty[2], sready, ksbar, rready, vbar, wready, sibar, obar, ofree, ksread, vread, siread;
     __shared__ uint32_t tmem_s;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    if (pass == 1 && blockIdx.y == 1 && (p.flags & KDA_FLAG_NO_SAVE) && blockIdx.x % (lay.segs - 1) == lay.segs - 2) {
-        pdl_wait();
-        return;  // the last segment's transition is for the backward
-    }
+    pdl_wait();
+    Walk wk;
+    wk.init(p, lay, pass == 1 && blockIdx.y, pass == 1 ? lay.segs - 1 : lay.segs);
+    const int nc = wk.ce - wk.cb;
+    const bool values = pass != 1 || blockIdx.y == 0;
+    // segments that the sequence does not reach; the last one ends in pass 2, and its transition is for the backward
+    if (wk.seg > wk.last || (pass == 1 && wk.seg == wk.last && (values || (p.flags & KDA_FLAG_NO_SAVE)))) return;
+    wk.c0 += wk.cb;
+    wk.tok_begin += (long long)wk.cb * C;
     if (warp == 0) {
         tmem_alloc(&tmem_s, 512);
         tmem_relinquish();
@@ -129,6 +146,9 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         mbar_init(&sready, MAIN / 32);
         mbar_init(&rready, MAIN / 32);
         mbar_init(&wready, MAIN / 32);
+        mbar_init(&ksread, MAIN / 32);
+        mbar_init(&vread, MAIN / 32);
+        mbar_init(&siread, MAIN / 32);
         mbar_init(&ksbar, 1);
         mbar_init(&vbar, 1);
         mbar_init(&sibar, 1);
@@ -136,13 +156,6 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         mbar_init(&ofree, OUTW / 32);
         mbar_fence_init();
     }
-    pdl_wait();
-    Walk wk;
-    wk.init(p, lay, pass == 1 && blockIdx.y, pass == 1 ? lay.segs - 1 : lay.segs);
-    const int nc = wk.ce - wk.cb;
-    const bool values = pass != 1 || blockIdx.y == 0;
-    wk.c0 += wk.cb;
-    wk.tok_begin += (long long)wk.cb * C;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -192,6 +205,8 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             tmem_ld16(tm + M::KS + t0, r[0]);
             tmem_ld16(tm + M::KS + t0 + 16, r[1]);
             tmem_wait_ld();
+            signal(&ksread, lane);
+            if (OUT && c > 0) ok = mbar_wait(&ofree, ph ^ 1, p, 1 << 11) && ok;  // V' A^T of the chunk before has left R's place
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 float f[16];
@@ -211,6 +226,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
             tmem_ld16(tm + M::VA + t0, r[0]);
             tmem_ld16(tm + M::VA + t0 + 16, r[1]);
             tmem_wait_ld();
+            signal(&vread, lane);
             float x[2][16];
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
@@ -243,6 +259,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                 tmem_ld16(tm + M::SP + half * M::HB + 16 * g, r[0]);
                 tmem_ld16(tm + M::SP + half * M::HB + 16 * g + 16, r[1]);
                 tmem_wait_ld();
+                if (g == DH / 16 - 2) signal(&siread, lane);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -251,7 +268,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
         }
         if (ok) {
             if (pass == 1) store_state((values ? ends : reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.segX)) + wk.slot(p, lay, wk.seg), false, e, d0, S);
-            else if (p.ht && wk.seg == lay.segs - 1) store_state(p.ht + sbase, vf, e, d0, S);
+            else if (p.ht && wk.seg == wk.last) store_state(p.ht + sbase, vf, e, d0, S);
         }
     } else if (warp < (MAIN + OUTW) / 32) {
         const int e = tid & 127;
@@ -360,20 +377,21 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                         first = false;
                     }
             };
-            if (!wait(&sready, ph, 1 << 19) || (OUT && c > 0 && !wait(&ofree, ph ^ 1, 1 << 20))) break;
+            if (!wait(&sready, ph, 1 << 19)) break;
             if (elect_one()) {
                 with_rows(M::KS, M::KK, 3);
                 mma_commit(&ksbar);
-                // v^T T'^T (the parts of V' that were here have been used: their products' outputs have been read)
-                if (values)
+            }
+            __syncwarp();
+            if (!wait(&ksread, ph, 1 << 20)) break;
+            // v^T T'^T (the parts of V' that were here have been used: their products are done)
+            if (values && elect_one())
 #pragma unroll
                 for (int i = 2; i >= 0; --i)
 #pragma unroll
                     for (int s = 0; s < 4; ++s)
                         mma_ss(tmem0 + M::VA + 16 * s, make_desc(b + M::V + s * 4096, 2048, 128), make_desc(b + M::TM + i * M::MAT + s * 256 + s * 2048, 128, 1024),
                                make_idesc(128, 64 - 16 * s, true, false), i < 2 || s > 0);
-                if (OUT) with_rows(M::QS, M::Q, 2);
-            }
             __syncwarp();
             if (!wait(&rready, ph, 1 << 21)) break;
             if (elect_one()) {
@@ -381,6 +399,11 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                 mma_commit(&vbar);
             }
             __syncwarp();
+            if (OUT) {  // (the accumulator of the chunk before has been read: R could not have been stored)
+                if (!wait(&vread, ph, 1 << 10)) break;
+                if (elect_one()) with_rows(M::QS, M::Q, 2);
+                __syncwarp();
+            }
             if (!wait(&wready, ph, 1 << 22)) break;
             if (elect_one()) {
 #pragma unroll
@@ -392,12 +415,16 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                             mma_ts(tmem0 + M::SP + h * M::HB, tmem0 + M::R + i * 32 + s * 8,
                                    make_desc(b + M::KK + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu, i < 2 || s > 0);
                 mma_commit(&sibar);
-                if (OUT) {
-                with_matrix(M::AV, [](int i, int s) { return M::VA + (s >> 1) * 32 + i * 16 + (s & 1) * 8; }, M::AM, 2, true);
-                mma_commit(&obar);
-                }
             }
             __syncwarp();
+            if (OUT) {
+                if (!wait(&siread, ph, 1 << 9)) break;
+                if (elect_one()) {
+                    with_matrix(M::AV, [](int i, int s) { return M::VA + (s >> 1) * 32 + i * 16 + (s & 1) * 8; }, M::AM, 2, true);
+                    mma_commit(&obar);
+                }
+                __syncwarp();
+            }
         }
     }
     tc_fence_before();
@@ -432,9 +459,16 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
     using M = bt::Map;
     constexpr int OUTW = ft::OUT;
     extern __shared__ __align__(1024) unsigned char dyn[];
-    __shared__ uint64_t full[2], empty[2], sready, kdbar, dosready, dvready, ybar, xready, sibar, ofree;
+    __shared__ uint64_t full[2], empty[2], sready, kdbar, dosready, dvready, ybar, xready, sibar, ofree, kdread, siread;
     __shared__ uint32_t tmem_s;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    pdl_wait();
+    Walk wk;
+    wk.init(p, lay, pass == 1, pass == 1 ? lay.segs - 1 : lay.segs);
+    const int nc = wk.ce - wk.cb;
+    if (wk.seg > wk.last) return;  // (a segment that the sequence does not reach)
+    wk.c0 += wk.cb;
+    wk.tok_begin += (long long)wk.cb * C;
     if (warp == 0) {
         tmem_alloc(&tmem_s, 512);
         tmem_relinquish();
@@ -449,18 +483,14 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         mbar_init(&dosready, MAIN / 32);
         mbar_init(&dvready, MAIN / 32);
         mbar_init(&xready, MAIN / 32);
+        mbar_init(&kdread, MAIN / 32);
+        mbar_init(&siread, MAIN / 32);
         mbar_init(&kdbar, 1);
         mbar_init(&ybar, 1);
         mbar_init(&sibar, 1);
         mbar_init(&ofree, OUTW / 32);
         mbar_fence_init();
     }
-    pdl_wait();
-    Walk wk;
-    wk.init(p, lay, pass == 1, pass == 1 ? lay.segs - 1 : lay.segs);
-    const int nc = wk.ce - wk.cb;
-    wk.c0 += wk.cb;
-    wk.tok_begin += (long long)wk.cb * C;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -474,7 +504,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
         const int e = tid & 127, half = warp >> 2, d0 = half * DH, t0 = half * 32;
         const uint32_t tm = tmem0 + ((uint32_t)((warp & 3) * 32) << 16);
         const size_t sbase = (size_t)(wk.n * (size_t)p.HV + wk.h) * K * 128;
-        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST, end = wk.seg == lay.segs - 1;
+        const bool vf = p.flags & KDA_FLAG_STATE_V_FIRST, end = wk.seg == wk.last;
         float* const starts = reinterpret_cast<float*>(sc + lay.segF);
         float S[DH];
         load_state(end ? p.grad_ht ? p.grad_ht + sbase : nullptr : pass == 1 ? nullptr : starts + wk.slot(p, lay, wk.seg + 1), end && vf, e, d0, S);
@@ -514,16 +544,19 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
             ok = mbar_wait(&kdbar, ph, p, 1 << 13) && ok;
             if (!__all_sync(0xffffffffu, ok)) break;
             tc_fence_after();
-            uint32_t r[2][16];
+            uint32_t r[2][16], ad[2][16];
+            tmem_ld16(tm + M::KD + t0, r[0]);
+            tmem_ld16(tm + M::KD + t0 + 16, r[1]);
+            tmem_ld16(tm + M::AD + t0, ad[0]);
+            tmem_ld16(tm + M::AD + t0 + 16, ad[1]);
+            tmem_wait_ld();
+            signal(&kdread, lane);
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 float f[16];
-                tmem_ld16(tm + M::KD + t0 + 16 * g, r[0]);
-                tmem_ld16(tm + M::AD + t0 + 16 * g, r[1]);
                 load16(aux + A_FK * C + t0 + 16 * g, f);
-                tmem_wait_ld();
 #pragma unroll
-                for (int j = 0; j < 16; ++j) f[j] = fmaf(f[j], __uint_as_float(r[0][j]), __uint_as_float(r[1][j]));
+                for (int j = 0; j < 16; ++j) f[j] = fmaf(f[j], __uint_as_float(r[g][j]), __uint_as_float(ad[g][j]));
                 st_parts<3>(tm + M::DV + half * 16 + 8 * g, 32, f);
             }
             tmem_wait_st();
@@ -559,6 +592,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                 tmem_ld16(tm + M::SP + half * M::HB + 16 * g, r[0]);
                 tmem_ld16(tm + M::SP + half * M::HB + 16 * g + 16, r[1]);
                 tmem_wait_ld();
+                if (g == DH / 16 - 2) signal(&siread, lane);
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -663,8 +697,8 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                                    make_desc(b + rows_at + h * (DH / 8) * 128 + s * 2 * (K / 8) * 128, (K / 8) * 128, 128), idu,
                                    !first || x < 2 || s > 0);
             };
-            if (!wait(&full[stage], (i >> 1) & 1, 1 << 18)) break;
-            if (elect_one()) {  // (the accumulator's last reader has arrived at dvready of the chunk before)
+            if (!wait(&full[stage], (i >> 1) & 1, 1 << 18) || (i > 0 && !wait(&siread, ph ^ 1, 1 << 9))) break;
+            if (elect_one()) {
 #pragma unroll
                 for (int x = 2; x >= 0; --x)
 #pragma unroll
@@ -684,7 +718,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
                 mma_commit(&kdbar);
             }
             __syncwarp();
-            if (!wait(&dosready, ph, 1 << 21) || !wait(&kdbar, ph, 1 << 22)) break;
+            if (!wait(&dosready, ph, 1 << 21) || !wait(&kdread, ph, 1 << 22)) break;  // (the parts of dS have been used)
             if (elect_one()) update(M::DOS, M::Q, true);
             __syncwarp();
             if (!wait(&dvready, ph, 1 << 23)) break;
@@ -720,22 +754,25 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
 // (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  FP32 multiply-adds; the next segment's X arrives meanwhile.
 constexpr int LDX = 132;  // floats per row of X
 template <bool TR>
-__global__ void __launch_bounds__(256) gdr_borders_kernel(const Layout lay, float* M, const float* X) {
+__global__ void __launch_bounds__(256) gdr_borders_kernel(const KdaGdrParams p, const Layout lay, float* M, const float* X) {
     extern __shared__ __align__(16) float sm[];  // X twice, then the columns [128][8]
     float* cols = sm + 2 * 128 * LDX;
     const int tid = threadIdx.x, d = tid >> 1, c4 = (tid & 1) * 4, c0 = (blockIdx.x & 15) * 8;
     const size_t base = (size_t)(blockIdx.x >> 4) * lay.segs * 16384;
-    const int steps = lay.segs - 2;  // (segment 0 of the forward, the last of the backward are done)
     pdl_wait();
-    auto seg = [&](int i) { return TR ? lay.segs - 2 - i : 1 + i; };
+    int first_chunk, nc;
+    seq_chunks(p, (blockIdx.x >> 4) / p.HV, first_chunk, nc);
+    const int last = last_segment(nc, lay), steps = last - 1;  // (segment 0 of the forward, the last of the backward are done)
+    if (steps < 1) return;
+    auto seg = [&](int i) { return TR ? last - 1 - i : 1 + i; };
     auto request = [&](int i) {
         const float* x = X + base + (size_t)seg(i) * 16384;
         for (int q = tid; q < 4096; q += 256) cp_async16_z(sm + (i & 1) * 128 * LDX + (q >> 5) * LDX + (q & 31) * 4, x + 4 * q, true);
         cp_async_commit();
     };
     auto at = [&](int s) { return reinterpret_cast<float4*>(M + base + (size_t)s * 16384 + d * 128 + c0 + c4); };
-    if (steps > 0) request(0);
-    *reinterpret_cast<float4*>(cols + d * 8 + c4) = *at(TR ? lay.segs - 1 : 0);
+    request(0);
+    *reinterpret_cast<float4*>(cols + d * 8 + c4) = *at(TR ? last : 0);
     for (int i = 0; i < steps; ++i) {
         if (i + 1 < steps) request(i + 1);
         else cp_async_commit();
@@ -776,7 +813,7 @@ static cudaError_t borders(const KdaGdrParams& p, const Layout& l, float* m, cud
     if (l.segs < 3) return cudaSuccess;
     const cudaError_t e = allow_smem(gdr_borders_kernel<TR>, bytes);
     const float* x = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + l.segX);
-    return e == cudaSuccess ? launch_dependent(gdr_borders_kernel<TR>, p.N * p.HV * 16, 256, bytes, s, l, m, x) : e;
+    return e == cudaSuccess ? launch_dependent(gdr_borders_kernel<TR>, p.N * p.HV * 16, 256, bytes, s, p, l, m, x) : e;
 }
 
 cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
