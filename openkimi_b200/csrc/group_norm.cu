@@ -5,11 +5,12 @@
 //
 // HBM-bound: forward one read and one write, backward two reads and one write per value.
 //   * S = 1 (every token by itself, groups of up to 1024 channels): L lanes hold a group of one row in registers, so that one pass
-//     does it all; the lanes keep their group over the rows they walk and with it w, b and their shares of dw, db.
+//     does it all, the next row on its way meanwhile; the lanes keep their group over the rows they walk and with it w, b and their
+//     shares of dw, db.
 //   * else: a thread keeps VEC channels and walks rows of a slice of a sample.  Forward: sums of x and x^2 about the slice's first
-//     row, joined over slices and channels as (count, mean, sum of squared deviations), then a second pass that applies.  Backward:
-//     per sample and channel the sums of dz and dz x^, which give dw, db and, weighted with w, m1 and m2; then dx.  The second pass
-//     reads from L2 what fits there.
+//     row, joined over the slice's channels to (mean, sum of squared deviations) of a group, and over the slices at the start of the
+//     second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which give dw, db and, weighted with w,
+//     m1 and m2; then dx.  The second pass reads from L2 what fits there.
 // Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
 #include "kda_common.cuh"
 
@@ -18,8 +19,10 @@ namespace gn {
 
 using bf16 = __nv_bfloat16;
 constexpr int NTHR = 256;
+constexpr int SLICE_THR = 384;    // at most, in the kernels over slices
 constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
 constexpr int MAX_SLICES = 256;
+constexpr int GROUPS_MAX = 24576; // groups whose numbers fit shared memory where they are not taken row by row
 
 struct Args {
     const void *x, *dy;
@@ -28,7 +31,7 @@ struct Args {
     float *mean, *rstd;           // [N, G]
     float *dw, *db;               // [Ch], may be NULL
     float* part;                  // scratch
-    long long N, S;
+    long long N, S, len;          // len: rows of a slice
     int Ch, G, act, slices;
     float eps;
 };
@@ -47,6 +50,12 @@ __device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
                 v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
             }
         }
+    } else if constexpr (VEC == 2 && sizeof(T) == 4) {
+        const float2 r = *reinterpret_cast<const float2*>(p);
+        v[0] = r.x; v[1] = r.y;
+    } else if constexpr (VEC == 2) {
+        const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
+        v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[i] = ldf(p + i);
@@ -66,15 +75,22 @@ __device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
             }
         }
         *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    } else if constexpr (VEC == 2 && sizeof(T) == 4) {
+        *reinterpret_cast<float2*>(p) = make_float2(v[0], v[1]);
+    } else if constexpr (VEC == 2) {
+        *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(v[0], v[1]);
     } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) stf(p + i, v[i]);
     }
 }
 
-// FP32 values go through expf, BF16 ones through the hardware's 2^x (2 ulp, and |z| 2^-24 from its argument)
+// FP32 values go through expf and a division, BF16 ones through the hardware's 2^x and 1 / x (2 ulp and 1, and |z| 2^-24 from the
+// argument)
 template <typename T>
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + (sizeof(T) == 4 ? expf(-z) : __expf(-z))); }
+__device__ __forceinline__ float sigmoid(float z) {
+    return sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : rcp_ftz(1.f + ex2_ftz(-LOG2E * z));
+}
 template <typename T>
 __device__ __forceinline__ float act(float z, bool silu) { return silu ? z * sigmoid<T>(z) : z; }
 // dy act'(z)
@@ -84,10 +100,15 @@ __device__ __forceinline__ float act_grad(float z, float dy, bool silu) {
     const float s = sigmoid<T>(z);
     return dy * s * fmaf(z, 1.f - s, 1.f);
 }
+// over L = 2^i lanes
 __device__ __forceinline__ float lanes_sum(float v, int L) {
-    for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < L) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+template <typename T>
+__device__ __forceinline__ float inv_sqrt(float v) { return sizeof(T) == 4 ? 1.f / sqrtf(v) : rsqrtf(v); }
 
 // ---- one row at a time ------------------------------------------------------------------------------------------------
 // Slots of L lanes; slot s has group s mod G and rows s / G, s / G + step, ...  Every lane of a warp makes the same number of turns.
@@ -114,32 +135,37 @@ __global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int
             dw[j][i] = db[j][i] = 0.f;
         }
     const long long turns = (a.N + step - 1) / step;
+    float nx[NV][VEC], ndy[NV][VEC];               // the next row
+    auto request = [&](long long k) {
+        const long long n = slot / a.G + k * step;
+        const bool on = !idle && n < a.N;
+        const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
+#pragma unroll
+        for (int j = 0; j < NV; ++j) {
+            const int c = (j * L + lane) * VEC;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) nx[j][i] = ndy[j][i] = 0.f;
+            if (on && c < Cg) {
+                load<T, VEC>(X + base + c, nx[j]);
+                if (BWD) load<T, VEC>(static_cast<const T*>(a.dy) + base + c, ndy[j]);
+            }
+        }
+    };
+    request(0);
     for (long long k = 0; k < turns; ++k) {
         const long long n = slot / a.G + k * step;
         const bool on = !idle && n < a.N;
         const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
-        float x[NV][VEC], s = 0.f;
+        float x[NV][VEC], dy[NV][VEC], s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * VEC;
-            if (on && c < Cg) load<T, VEC>(X + base + c, x[j]);
-            else
+        for (int j = 0; j < NV; ++j)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) x[j][i] = 0.f;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) s += x[j][i];
-        }
-        float dy[NV][VEC];
-        if (BWD) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = (j * L + lane) * VEC;
-                if (on && c < Cg) load<T, VEC>(static_cast<const T*>(a.dy) + base + c, dy[j]);
-                else
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) dy[j][i] = 0.f;
+            for (int i = 0; i < VEC; ++i) {
+                x[j][i] = nx[j][i];
+                dy[j][i] = ndy[j][i];
+                s += x[j][i];
             }
-        }
+        if (k + 1 < turns) request(k + 1);
         const float mean = lanes_sum(s, L) * inv;
         float q = 0.f;
 #pragma unroll
@@ -149,7 +175,7 @@ __global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int
                 x[j][i] = (j * L + lane) * VEC < Cg ? x[j][i] - mean : 0.f;
                 q = fmaf(x[j][i], x[j][i], q);
             }
-        const float rstd = 1.f / sqrtf(lanes_sum(q, L) * inv + a.eps);
+        const float rstd = inv_sqrt<T>(lanes_sum(q, L) * inv + a.eps);
         if (!BWD) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
@@ -217,23 +243,26 @@ __global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* pa
 }
 
 // ---- samples of several positions -------------------------------------------------------------------------------------
-// A CTA has one slice of one sample; thread = (row of TR, VEC channels), channels in blocks of NTHR * VEC where a row is wider than
+// A CTA has one slice of one sample; thread = (row of TR, VEC channels), channels in blocks of SLICE_THR * VEC where a row is wider than
 // the CTA.
 struct Slice {
     long long n, s0, s1;
     __device__ __forceinline__ Slice(const Args& a) {
         n = blockIdx.x / a.slices;
         const long long i = blockIdx.x % a.slices;
-        s0 = a.S * i / a.slices;
-        s1 = a.S * (i + 1) / a.slices;
+        s0 = i * a.len;
+        s1 = min(a.S, s0 + a.len);
     }
 };
+// scratch: [N * slices][2][Ch] sums of the channels, then [N * slices][G][2] numbers of the groups
+__device__ __forceinline__ float* group_part(const Args& a) { return a.part + (size_t)a.N * a.slices * 2 * a.Ch; }
 
-// MODE 0: count-free sums of x - x0 and (x - x0)^2 about the slice's first row x0; 1: sums of dz x^ and dz
+// MODE 0: sums of x - x0 and (x - x0)^2 about the slice's first row x0, and from them a group's mean and sum of squared deviations;
+// 1: sums of dz x^ and dz, and over a group's channels w times those
 template <typename T, int VEC, int MODE>
-__global__ void __launch_bounds__(NTHR) group_norm_sums_kernel(const Args a) {
+__global__ void __launch_bounds__(SLICE_THR) group_norm_sums_kernel(const Args a) {
     extern __shared__ float sm[];                  // [2][TR][TC * VEC]
-    const int cols = a.Ch / VEC, TC = min(cols, NTHR), TR = NTHR / TC;
+    const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
     const Slice sl(a);
     const long long n = sl.n;
@@ -295,7 +324,7 @@ __global__ void __launch_bounds__(NTHR) group_norm_sums_kernel(const Args a) {
                 sm[(TR + tr) * TC * VEC + tc * VEC + i] = s2[i];
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * TC * VEC; i += NTHR) {
+        for (int i = threadIdx.x; i < 2 * TC * VEC; i += blockDim.x) {
             const int which = i / (TC * VEC), cc = i % (TC * VEC);
             if (v0 * VEC + cc >= a.Ch) continue;
             float s = 0.f;
@@ -303,92 +332,87 @@ __global__ void __launch_bounds__(NTHR) group_norm_sums_kernel(const Args a) {
             out[(size_t)which * a.Ch + v0 * VEC + cc] = s;
         }
     }
-}
-
-// mean and rstd of (sample, group) from the slices' sums: two passes over slices and channels, in 64 bits (channels and slices are
-// few).  A CTA per (group, sample).
-template <typename T>
-__global__ void __launch_bounds__(128) group_norm_stats_kernel(const Args a) {
-    __shared__ double s[128];
-    const int Cg = a.Ch / a.G, g = blockIdx.x % a.G;
-    const long long n = blockIdx.x / a.G;
-    pdl_wait();
-    const float* part = a.part + (size_t)n * a.slices * 2 * a.Ch;
-    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
-    auto sum = [&](double v) {
-        s[threadIdx.x] = v;
-        for (int o = 64; o > 0; o >>= 1) {
-            __syncthreads();
-            if (threadIdx.x < o) s[threadIdx.x] += s[threadIdx.x + o];
+    __syncthreads();  // (the sums are read back by the CTA that wrote them)
+    float* groups = group_part(a) + (size_t)blockIdx.x * a.G * 2;
+    const int lane = threadIdx.x & 31;
+    const float m = (float)(sl.s1 - sl.s0);
+    for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
+        float u = 0.f, v = 0.f;
+        if (MODE == 0) {
+            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) u += fmaf(m, ldf(X + (size_t)sl.s0 * a.Ch + c), out[c]);
+            u = warp_sum(u) / (m * Cg);
+            // sum (x - mean)^2 = sum (x - x0)^2 + 2 (x0 - mean) sum (x - x0) + m (x0 - mean)^2
+            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
+                const float d = ldf(X + (size_t)sl.s0 * a.Ch + c) - u;
+                v += fmaf(d, fmaf(m, d, 2.f * out[c]), out[a.Ch + c]);
+            }
+            v = warp_sum(v);
+        } else {
+            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
+                const float w = a.w ? a.w[c] : 1.f;
+                v = fmaf(w, out[c], v);
+                u = fmaf(w, out[a.Ch + c], u);
+            }
+            u = warp_sum(u);
+            v = warp_sum(v);
         }
-        __syncthreads();
-        const double r = s[0];
-        __syncthreads();
-        return r;
-    };
-    auto each = [&](auto f) {
-        double v = 0.0;
-        for (int i = threadIdx.x; i < a.slices * Cg; i += 128) {
-            const int sl = i / Cg, c = g * Cg + i % Cg;
-            const long long s0 = a.S * sl / a.slices, s1 = a.S * (sl + 1) / a.slices;
-            v += f((double)(s1 - s0), (double)ldf(X + (size_t)s0 * a.Ch + c), (double)part[(size_t)sl * 2 * a.Ch + c],
-                   (double)part[((size_t)sl * 2 + 1) * a.Ch + c]);
-        }
-        return sum(v);
-    };
-    const double count = (double)a.S * Cg;
-    const double mean = each([](double m, double x0, double d1, double) { return m * x0 + d1; }) / count;
-    // sum (x - mean)^2 = sum (x - x0)^2 + 2 (x0 - mean) sum (x - x0) + m (x0 - mean)^2
-    const double var = each([mean](double m, double x0, double d1, double d2) { return d2 + (x0 - mean) * (2.0 * d1 + m * (x0 - mean)); }) / count;
-    if (threadIdx.x == 0) {
-        a.mean[n * a.G + g] = (float)mean;
-        a.rstd[n * a.G + g] = (float)(1.0 / sqrt((var > 0.0 || !(var <= 0.0) ? var : 0.0) + (double)a.eps));
-    }
-}
-
-// m1, m2 of (sample, group) from the sums over its slices, [N, G, 2] behind them
-__global__ void __launch_bounds__(128) group_norm_means_kernel(const Args a) {
-    __shared__ double s[2][128];
-    const int Cg = a.Ch / a.G, g = blockIdx.x % a.G;
-    const long long n = blockIdx.x / a.G;
-    pdl_wait();
-    const float* part = a.part + (size_t)n * a.slices * 2 * a.Ch;
-    double m1 = 0.0, m2 = 0.0;
-    for (int i = threadIdx.x; i < a.slices * Cg; i += 128) {
-        const int sl = i / Cg, c = g * Cg + i % Cg;
-        const double w = a.w ? a.w[c] : 1.f;
-        m2 += w * part[(size_t)sl * 2 * a.Ch + c];
-        m1 += w * part[((size_t)sl * 2 + 1) * a.Ch + c];
-    }
-    s[0][threadIdx.x] = m1;
-    s[1][threadIdx.x] = m2;
-    for (int o = 64; o > 0; o >>= 1) {
-        __syncthreads();
-        if (threadIdx.x < o) {
-            s[0][threadIdx.x] += s[0][threadIdx.x + o];
-            s[1][threadIdx.x] += s[1][threadIdx.x + o];
-        }
-    }
-    if (threadIdx.x == 0) {
-        const double count = (double)a.S * Cg;
-        float* out = a.part + (size_t)a.N * a.slices * 2 * a.Ch + (n * a.G + g) * 2;
-        out[0] = (float)(s[0][0] / count);
-        out[1] = (float)(s[1][0] / count);
+        if (lane == 0) *reinterpret_cast<float2*>(groups + 2 * g) = make_float2(u, v);
     }
 }
 
 template <typename T, int VEC, bool BWD>
-__global__ void __launch_bounds__(NTHR) group_norm_apply_kernel(const Args a) {
-    const int cols = a.Ch / VEC, TC = min(cols, NTHR), TR = NTHR / TC;
+__global__ void __launch_bounds__(SLICE_THR) group_norm_apply_kernel(const Args a) {
+    const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
     const Slice sl(a);
     const long long n = sl.n;
+    extern __shared__ float stat[];                // [G][2]: mean, rstd; backward: m1, m2
     pdl_wait();
+    {   // the sample's slices, a warp per group; means about the first slice's
+        const float2* groups = reinterpret_cast<const float2*>(group_part(a)) + (size_t)n * a.slices * a.G;
+        const int lane = threadIdx.x & 31;
+        const float rows = (float)a.len, tail = (float)(a.S - (a.slices - 1) * a.len), count = (float)a.S * Cg;
+        for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
+            float2 p[MAX_SLICES / 32];
+            const float u0 = BWD ? 0.f : groups[g].x;
+            float u = 0.f, v = 0.f;
+#pragma unroll
+            for (int j = 0; j < MAX_SLICES / 32; ++j)
+                if (j * 32 < a.slices) {
+                    const int i = j * 32 + lane;
+                    p[j] = i < a.slices ? groups[(size_t)i * a.G + g] : make_float2(u0, 0.f);
+                    p[j].x -= u0;
+                    u += BWD ? p[j].x : p[j].x * (i == a.slices - 1 ? tail : rows);
+                    v += p[j].y;
+                }
+            u = warp_sum(u);
+            if (!BWD) {
+                u /= (float)a.S;
+#pragma unroll
+                for (int j = 0; j < MAX_SLICES / 32; ++j)
+                    if (j * 32 + lane < a.slices) {
+                        const float d = p[j].x - u;
+                        v = fmaf(d * d, (j * 32 + lane == a.slices - 1 ? tail : rows) * Cg, v);
+                    }
+            }
+            v = warp_sum(v);
+            const float s0 = BWD ? u / count : u0 + u, s1 = BWD ? v / count : 1.f / sqrtf(fmaxf(v, 0.f) / count + a.eps);
+            if (lane == 0) {
+                // (fmaxf drops a NaN: one among the values is one in their mean)
+                stat[2 * g] = s0;
+                stat[2 * g + 1] = !BWD && s0 != s0 ? s0 : s1;
+                if (!BWD && sl.s0 == 0) {
+                    a.mean[n * a.G + g] = stat[2 * g];
+                    a.rstd[n * a.G + g] = stat[2 * g + 1];
+                }
+            }
+        }
+        __syncthreads();
+    }
     if (tr >= TR) return;
     const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
     const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
     T* Y = static_cast<T*>(BWD ? a.dx : a.y) + (size_t)n * a.S * a.Ch;
-    const float* m = a.part + (size_t)a.N * a.slices * 2 * a.Ch + n * a.G * 2;
     const bool silu = a.act;
     for (int v = tc; v < cols; v += TC) {
         const int c = v * VEC;
@@ -396,12 +420,12 @@ __global__ void __launch_bounds__(NTHR) group_norm_apply_kernel(const Args a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             const int g = (c + i) / Cg;
-            mu[i] = a.mean[n * a.G + g];
-            rs[i] = a.rstd[n * a.G + g];
+            mu[i] = BWD ? a.mean[n * a.G + g] : stat[2 * g];
+            rs[i] = BWD ? a.rstd[n * a.G + g] : stat[2 * g + 1];
             w[i] = a.w ? a.w[c + i] : 1.f;
             b[i] = a.b ? a.b[c + i] : 0.f;
-            m1[i] = BWD ? m[2 * g] : 0.f;
-            m2[i] = BWD ? m[2 * g + 1] : 0.f;
+            m1[i] = BWD ? stat[2 * g] : 0.f;
+            m2[i] = BWD ? stat[2 * g + 1] : 0.f;
         }
 #pragma unroll 4
         for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
@@ -421,11 +445,14 @@ __global__ void __launch_bounds__(NTHR) group_norm_apply_kernel(const Args a) {
 // ---- launches -----------------------------------------------------------------------------------------------------------
 static bool by_rows(long long S, int Ch, int G) { return S == 1 && Ch / G <= ROWS_MAX; }
 
-// slices of a sample: about four CTAs per SM over all samples, of at least 16 rows
-static int slice_count(long long N, long long S) {
-    long long want = (4LL * sm_count() + N - 1) / N, most = (S + 15) / 16;
+// slices of a sample: about four CTAs per SM over all samples, of at least 8 rows, all but the last of the same length
+static void cut(Args& a) {
+    long long want = (4LL * sm_count() + a.N - 1) / a.N, most = (a.S + 7) / 8;
     if (want > most) want = most;
-    return (int)(want < 1 ? 1 : want > MAX_SLICES ? MAX_SLICES : want);
+    if (want > MAX_SLICES) want = MAX_SLICES;
+    if (want < 1) want = 1;
+    a.len = (a.S + want - 1) / want;
+    a.slices = (int)((a.S + a.len - 1) / a.len);
 }
 
 struct RowsGrid { int L; long long ctas, step; };
@@ -442,10 +469,11 @@ static RowsGrid rows_grid(long long N, int Ch, int G, int vec, bool bwd) {
     r.step = r.ctas * per / G;
     return r;
 }
-// elements per access: 16 bytes where every group (or, for `rows_only`, every row) starts on 16 bytes
+// elements per access: 16 bytes where every unit (a group, or a row of slices) starts on 16 bytes, else two or one
 static int vec_of(int unit, int es, const void* x, const void* y, const void* z) {
     const int full = 16 / es;
-    return unit % full == 0 && (((uintptr_t)x | (uintptr_t)y | (uintptr_t)z) & 15) == 0 ? full : 1;
+    const uintptr_t at = (uintptr_t)x | (uintptr_t)y | (uintptr_t)z;
+    return unit % full == 0 && (at & 15) == 0 ? full : unit % 2 == 0 && (at & (2 * es - 1)) == 0 ? 2 : 1;
 }
 
 template <typename T, int VEC, bool BWD>
@@ -464,12 +492,12 @@ static cudaError_t rows_launch(const Args& a, cudaStream_t s) {
 
 template <typename T, int VEC, bool BWD>
 static cudaError_t slices_launch(const Args& a, cudaStream_t s) {
-    const dim3 grid((unsigned)(a.N * a.slices)), groups((unsigned)(a.N * a.G));
-    const int cols = a.Ch / VEC, TC = cols < NTHR ? cols : NTHR, TR = NTHR / TC;
-    const size_t smem = (size_t)2 * TR * TC * VEC * sizeof(float);
-    cudaError_t e = launch_dependent(group_norm_sums_kernel<T, VEC, BWD ? 1 : 0>, grid, NTHR, smem, s, a);
-    if (e == cudaSuccess) e = BWD ? launch_dependent(group_norm_means_kernel, groups, 128, 0, s, a) : launch_dependent(group_norm_stats_kernel<T>, groups, 128, 0, s, a);
-    if (e == cudaSuccess) e = launch_dependent(group_norm_apply_kernel<T, VEC, BWD>, grid, NTHR, 0, s, a);
+    const dim3 grid((unsigned)(a.N * a.slices));
+    const int cols = a.Ch / VEC, TC = cols < SLICE_THR ? cols : SLICE_THR, TR = SLICE_THR / TC, threads = (TC * TR + 31) / 32 * 32;
+    const size_t smem = (size_t)2 * TR * TC * VEC * sizeof(float), stat = (size_t)2 * a.G * sizeof(float);
+    cudaError_t e = stat > 48 * 1024 ? allow_smem(group_norm_apply_kernel<T, VEC, BWD>, GROUPS_MAX * 8) : cudaSuccess;
+    if (e == cudaSuccess) e = launch_dependent(group_norm_sums_kernel<T, VEC, BWD ? 1 : 0>, grid, threads, smem, s, a);
+    if (e == cudaSuccess) e = launch_dependent(group_norm_apply_kernel<T, VEC, BWD>, grid, threads, stat, s, a);
     if (e == cudaSuccess && BWD && a.dw)
         e = launch_dependent(group_norm_params_kernel, dim3((a.Ch + 31) / 32, 2), dim3(32, 32), 0, s, (const float*)a.part, a.N * a.slices, a.Ch, a.dw, a.db);
     return e;
@@ -480,27 +508,33 @@ static cudaError_t dispatch(const Args& a, cudaStream_t s) {
     constexpr int FULL = 16 / sizeof(T);
     const bool rows = by_rows(a.S, a.Ch, a.G);
     const int vec = vec_of(rows ? a.Ch / a.G : a.Ch, sizeof(T), a.x, BWD ? a.dx : a.y, a.dy);
-    if (rows) return vec == FULL ? rows_launch<T, FULL, BWD>(a, s) : rows_launch<T, 1, BWD>(a, s);
-    return vec == FULL ? slices_launch<T, FULL, BWD>(a, s) : slices_launch<T, 1, BWD>(a, s);
+    if (rows) return vec == FULL ? rows_launch<T, FULL, BWD>(a, s) : vec == 2 ? rows_launch<T, 2, BWD>(a, s) : rows_launch<T, 1, BWD>(a, s);
+    return vec == FULL ? slices_launch<T, FULL, BWD>(a, s) : vec == 2 ? slices_launch<T, 2, BWD>(a, s) : slices_launch<T, 1, BWD>(a, s);
 }
 
 static int check(const Args& a, int dtype) {
     if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
     if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.G <= 0 || a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
-    // grids of samples x slices and samples x groups
-    if (!by_rows(a.S, a.Ch, a.G) && (a.N > 0x7fffffffLL / MAX_SLICES || a.N > 0x7fffffffLL / a.G)) return KDA_ERR_SHAPE;
+    // a grid of samples x slices, and the groups' numbers in shared memory
+    if (!by_rows(a.S, a.Ch, a.G) && (a.N > 0x7fffffffLL / MAX_SLICES || a.G > GROUPS_MAX)) return KDA_ERR_SHAPE;
     if (by_rows(a.S, a.Ch, a.G) && a.N > (1LL << 40) / a.G) return KDA_ERR_SHAPE;
     return KDA_OK;
 }
 static size_t scratch(long long N, long long S, int Ch, int G, int es, bool bwd) {
     if (by_rows(S, Ch, G)) {
         if (!bwd) return 0;
-        long long step = rows_grid(N, Ch, G, 1, true).step;  // (the element width is known only with the pointers)
-        const long long wide = (Ch / G) % (16 / es) ? 0 : rows_grid(N, Ch, G, 16 / es, true).step;
-        if (wide > step) step = wide;
+        long long step = 0;  // (the element width is known only with the pointers)
+        for (int vec : {1, 2, 16 / es})
+            if ((Ch / G) % vec == 0) {
+                const long long n = rows_grid(N, Ch, G, vec, true).step;
+                if (n > step) step = n;
+            }
         return (size_t)step * 2 * Ch * sizeof(float);
     }
-    return ((size_t)N * slice_count(N, S) * 2 * Ch + (size_t)N * G * 2) * sizeof(float);
+    Args a = {};
+    a.N = N; a.S = S;
+    cut(a);
+    return (size_t)N * a.slices * 2 * (Ch + G) * sizeof(float);
 }
 
 }  // namespace gn
@@ -527,7 +561,7 @@ extern "C" int kda_group_norm_fwd(const void* x, const float* weight, const floa
     a.N = N; a.S = S; a.Ch = channels; a.G = groups; a.act = silu; a.eps = eps;
     if (const int rc = gn::check(a, dtype)) return rc;
     if (!x || !y || (!gn::by_rows(S, channels, groups) && (!mean || !rstd || !scratch))) return KDA_ERR_NULL;
-    a.slices = gn::slice_count(N, S);
+    gn::cut(a);
     const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, false>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, false>(a, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }
@@ -542,7 +576,7 @@ extern "C" int kda_group_norm_bwd(const void* x, const float* weight, const floa
     if (const int rc = gn::check(a, dtype)) return rc;
     const bool rows = gn::by_rows(S, channels, groups);
     if (!x || !dy || !dx || (!rows && (!mean || !rstd || !scratch)) || (dweight && (!dbias || !scratch)) || (!dweight && dbias)) return KDA_ERR_NULL;
-    a.slices = gn::slice_count(N, S);
+    gn::cut(a);
     const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, true>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, true>(a, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }
