@@ -36,31 +36,31 @@ struct Args {
     float eps;
 };
 
+// VEC elements as they lie in memory: 16 bytes, two elements or one
+template <typename T, int VEC> struct Raw { T v[VEC]; };
+template <> struct Raw<float, 4> { uint4 v; };
+template <> struct Raw<bf16, 8> { uint4 v; };
+template <> struct Raw<float, 2> { float2 v; };
+template <> struct Raw<bf16, 2> { uint32_t v; };
 template <typename T, int VEC>
-__device__ __forceinline__ void load(const T* p, float (&v)[VEC]) {
-    if constexpr (sizeof(T) * VEC == 16) {
-        const uint4 r = *reinterpret_cast<const uint4*>(p);
-        const uint32_t u[4] = {r.x, r.y, r.z, r.w};
+__device__ __forceinline__ Raw<T, VEC> load_raw(const T* p) { return *reinterpret_cast<const Raw<T, VEC>*>(p); }
+__device__ __forceinline__ void unpack(const Raw<float, 1>& r, float (&x)[1]) { x[0] = r.v[0]; }
+__device__ __forceinline__ void unpack(const Raw<bf16, 1>& r, float (&x)[1]) { x[0] = __bfloat162float(r.v[0]); }
+__device__ __forceinline__ void unpack(const Raw<float, 2>& r, float (&x)[2]) { x[0] = r.v.x; x[1] = r.v.y; }
+__device__ __forceinline__ void unpack(const Raw<bf16, 2>& r, float (&x)[2]) { x[0] = __uint_as_float(r.v << 16); x[1] = __uint_as_float(r.v & 0xffff0000u); }
+__device__ __forceinline__ void unpack(const Raw<float, 4>& r, float (&x)[4]) {
+    x[0] = __uint_as_float(r.v.x); x[1] = __uint_as_float(r.v.y); x[2] = __uint_as_float(r.v.z); x[3] = __uint_as_float(r.v.w);
+}
+__device__ __forceinline__ void unpack(const Raw<bf16, 8>& r, float (&x)[8]) {
+    const uint32_t u[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if constexpr (sizeof(T) == 4) {
-                v[i] = __uint_as_float(u[i]);
-            } else {
-                v[2 * i] = __uint_as_float(u[i] << 16);
-                v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
-            }
-        }
-    } else if constexpr (VEC == 2 && sizeof(T) == 4) {
-        const float2 r = *reinterpret_cast<const float2*>(p);
-        v[0] = r.x; v[1] = r.y;
-    } else if constexpr (VEC == 2) {
-        const uint32_t r = *reinterpret_cast<const uint32_t*>(p);
-        v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u);
-    } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[i] = ldf(p + i);
+    for (int i = 0; i < 4; ++i) {
+        x[2 * i] = __uint_as_float(u[i] << 16);
+        x[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
     }
 }
+template <typename T, int VEC>
+__device__ __forceinline__ void load(const T* p, float (&v)[VEC]) { unpack(load_raw<T, VEC>(p), v); }
 template <typename T, int VEC>
 __device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
     if constexpr (sizeof(T) * VEC == 16) {
@@ -113,7 +113,7 @@ __device__ __forceinline__ float inv_sqrt(float v) { return sizeof(T) == 4 ? 1.f
 // ---- one row at a time ------------------------------------------------------------------------------------------------
 // Slots of L lanes; slot s has group s mod G and rows s / G, s / G + step, ...  Every lane of a warp makes the same number of turns.
 template <typename T, int VEC, int NV, bool BWD>
-__global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int L) {
+__global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 2 : 1) group_norm_rows_kernel(const Args a, int L) {
     const int lane = threadIdx.x & (L - 1), Cg = a.Ch / a.G;
     const long long slot = ((long long)blockIdx.x * NTHR + threadIdx.x) / L, slots = (long long)gridDim.x * NTHR / L;
     const long long step = slots / a.G;            // rows between a slot's rows; slots beyond step * G have none
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int
             dw[j][i] = db[j][i] = 0.f;
         }
     const long long turns = (a.N + step - 1) / step;
-    float nx[NV][VEC], ndy[NV][VEC];               // the next row
+    Raw<T, VEC> nx[NV], ndy[NV];                   // the next row
     auto request = [&](long long k) {
         const long long n = slot / a.G + k * step;
         const bool on = !idle && n < a.N;
@@ -143,11 +143,10 @@ __global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int c = (j * L + lane) * VEC;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) nx[j][i] = ndy[j][i] = 0.f;
+            nx[j] = ndy[j] = Raw<T, VEC>{};
             if (on && c < Cg) {
-                load<T, VEC>(X + base + c, nx[j]);
-                if (BWD) load<T, VEC>(static_cast<const T*>(a.dy) + base + c, ndy[j]);
+                nx[j] = load_raw<T, VEC>(X + base + c);
+                if (BWD) ndy[j] = load_raw<T, VEC>(static_cast<const T*>(a.dy) + base + c);
             }
         }
     };
@@ -158,13 +157,12 @@ __global__ void __launch_bounds__(NTHR) group_norm_rows_kernel(const Args a, int
         const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
         float x[NV][VEC], dy[NV][VEC], s = 0.f;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
+        for (int j = 0; j < NV; ++j) {
+            unpack(nx[j], x[j]);
+            if (BWD) unpack(ndy[j], dy[j]);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                x[j][i] = nx[j][i];
-                dy[j][i] = ndy[j][i];
-                s += x[j][i];
-            }
+            for (int i = 0; i < VEC; ++i) s += x[j][i];
+        }
         if (k + 1 < turns) request(k + 1);
         const float mean = lanes_sum(s, L) * inv;
         float q = 0.f;
@@ -233,6 +231,7 @@ __global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* pa
     pdl_wait();
     double v = 0.0;
     if (c < Ch)
+#pragma unroll 8
         for (long long i = threadIdx.y; i < count; i += 32) v += part[(i * 2 + which) * Ch + c];
     s[threadIdx.y][threadIdx.x] = v;
     __syncthreads();
@@ -260,7 +259,7 @@ __device__ __forceinline__ float* group_part(const Args& a) { return a.part + (s
 // MODE 0: sums of x - x0 and (x - x0)^2 about the slice's first row x0, and from them a group's mean and sum of squared deviations;
 // 1: sums of dz x^ and dz, and over a group's channels w times those
 template <typename T, int VEC, int MODE>
-__global__ void __launch_bounds__(SLICE_THR) group_norm_sums_kernel(const Args a) {
+__global__ void __launch_bounds__(SLICE_THR, VEC <= 8 ? 3 : 1) group_norm_sums_kernel(const Args a) {
     extern __shared__ float sm[];                  // [2][TR][TC * VEC]
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
@@ -274,18 +273,15 @@ __global__ void __launch_bounds__(SLICE_THR) group_norm_sums_kernel(const Args a
     for (int v0 = 0; v0 < cols; v0 += TC) {
         const int v = v0 + tc, c = v * VEC;
         const bool on = tr < TR && v < cols;
-        float p[VEC], q[VEC], s1[VEC], s2[VEC];
+        float p[VEC], s1[VEC], s2[VEC], mu = 0.f, rs = 0.f;  // (a thread's channels are of one group)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.f;
         if (on) {
             if (MODE == 0) {
                 load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, p);
             } else {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    p[i] = a.mean[n * a.G + (c + i) / Cg];
-                    q[i] = a.rstd[n * a.G + (c + i) / Cg];
-                }
+                mu = a.mean[n * a.G + c / Cg];
+                rs = a.rstd[n * a.G + c / Cg];
             }
             float w[VEC], b[VEC];
 #pragma unroll
@@ -309,7 +305,7 @@ __global__ void __launch_bounds__(SLICE_THR) group_norm_sums_kernel(const Args a
                     load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) {
-                        const float xh = (x[i] - p[i]) * q[i], dz = act_grad<T>(fmaf(xh, w[i], b[i]), dy[i], silu);
+                        const float xh = (x[i] - mu) * rs, dz = act_grad<T>(fmaf(xh, w[i], b[i]), dy[i], silu);
                         s1[i] = fmaf(dz, xh, s1[i]);
                         s2[i] += dz;
                     }
@@ -361,7 +357,7 @@ __global__ void __launch_bounds__(SLICE_THR) group_norm_sums_kernel(const Args a
 }
 
 template <typename T, int VEC, bool BWD>
-__global__ void __launch_bounds__(SLICE_THR) group_norm_apply_kernel(const Args a) {
+__global__ void __launch_bounds__(SLICE_THR, 3) group_norm_apply_kernel(const Args a) {
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
     const Slice sl(a);
@@ -416,26 +412,25 @@ __global__ void __launch_bounds__(SLICE_THR) group_norm_apply_kernel(const Args 
     const bool silu = a.act;
     for (int v = tc; v < cols; v += TC) {
         const int c = v * VEC;
-        float mu[VEC], rs[VEC], w[VEC], b[VEC], m1[VEC], m2[VEC];
+        const int g = c / Cg;  // (a thread's channels are of one group)
+        const float mu = BWD ? a.mean[n * a.G + g] : stat[2 * g], rs = BWD ? a.rstd[n * a.G + g] : stat[2 * g + 1];
+        // dx = (rstd w) dz + (x - mean) (-rstd^2 m2) - rstd m1
+        const float k1 = BWD ? -rs * stat[2 * g] : 0.f, k2 = BWD ? -rs * rs * stat[2 * g + 1] : 0.f;
+        float w[VEC], b[VEC];
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const int g = (c + i) / Cg;
-            mu[i] = BWD ? a.mean[n * a.G + g] : stat[2 * g];
-            rs[i] = BWD ? a.rstd[n * a.G + g] : stat[2 * g + 1];
-            w[i] = a.w ? a.w[c + i] : 1.f;
+            w[i] = rs * (a.w ? a.w[c + i] : 1.f);
             b[i] = a.b ? a.b[c + i] : 0.f;
-            m1[i] = BWD ? stat[2 * g] : 0.f;
-            m2[i] = BWD ? stat[2 * g + 1] : 0.f;
         }
-#pragma unroll 4
+#pragma unroll(BWD ? 2 : 4)
         for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
             float x[VEC], dy[VEC], y[VEC];
             load<T, VEC>(X + (size_t)s * a.Ch + c, x);
             if (BWD) load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                const float xh = (x[i] - mu[i]) * rs[i], z = fmaf(xh, w[i], b[i]);
-                y[i] = BWD ? rs[i] * (act_grad<T>(z, dy[i], silu) * w[i] - m1[i] - xh * m2[i]) : act<T>(z, silu);
+                const float d = x[i] - mu, z = fmaf(d, w[i], b[i]);
+                y[i] = BWD ? fmaf(act_grad<T>(z, dy[i], silu), w[i], fmaf(d, k2, k1)) : act<T>(z, silu);
             }
             store<T, VEC>(Y + (size_t)s * a.Ch + c, y);
         }
@@ -445,9 +440,9 @@ __global__ void __launch_bounds__(SLICE_THR) group_norm_apply_kernel(const Args 
 // ---- launches -----------------------------------------------------------------------------------------------------------
 static bool by_rows(long long S, int Ch, int G) { return S == 1 && Ch / G <= ROWS_MAX; }
 
-// slices of a sample: about four CTAs per SM over all samples, of at least 8 rows, all but the last of the same length
+// slices of a sample: three CTAs per SM (what their registers allow) over all samples, of at least 8 rows, all but the last of the same length
 static void cut(Args& a) {
-    long long want = (4LL * sm_count() + a.N - 1) / a.N, most = (a.S + 7) / 8;
+    long long want = 3LL * sm_count() / a.N, most = (a.S + 7) / 8;
     if (want > most) want = most;
     if (want > MAX_SLICES) want = MAX_SLICES;
     if (want < 1) want = 1;
@@ -469,7 +464,7 @@ static RowsGrid rows_grid(long long N, int Ch, int G, int vec, bool bwd) {
     r.step = r.ctas * per / G;
     return r;
 }
-// elements per access: 16 bytes where every unit (a group, or a row of slices) starts on 16 bytes, else two or one
+// elements per access: 16 bytes where every group starts on 16 bytes, else two or one
 static int vec_of(int unit, int es, const void* x, const void* y, const void* z) {
     const int full = 16 / es;
     const uintptr_t at = (uintptr_t)x | (uintptr_t)y | (uintptr_t)z;
@@ -507,7 +502,7 @@ template <typename T, bool BWD>
 static cudaError_t dispatch(const Args& a, cudaStream_t s) {
     constexpr int FULL = 16 / sizeof(T);
     const bool rows = by_rows(a.S, a.Ch, a.G);
-    const int vec = vec_of(rows ? a.Ch / a.G : a.Ch, sizeof(T), a.x, BWD ? a.dx : a.y, a.dy);
+    const int vec = vec_of(a.Ch / a.G, sizeof(T), a.x, BWD ? a.dx : a.y, a.dy);
     if (rows) return vec == FULL ? rows_launch<T, FULL, BWD>(a, s) : vec == 2 ? rows_launch<T, 2, BWD>(a, s) : rows_launch<T, 1, BWD>(a, s);
     return vec == FULL ? slices_launch<T, FULL, BWD>(a, s) : vec == 2 ? slices_launch<T, 2, BWD>(a, s) : slices_launch<T, 1, BWD>(a, s);
 }
