@@ -22,6 +22,7 @@ constexpr int NTHR = 256;
 constexpr int SLICE_THR = 384;    // at most, in the kernels over slices
 constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
 constexpr int MAX_SLICES = 256;
+
 constexpr int GROUPS_MAX = 24576; // groups whose numbers fit shared memory where they are not taken row by row
 
 struct Args {
@@ -85,20 +86,94 @@ __device__ __forceinline__ void store(T* p, const float (&v)[VEC]) {
     }
 }
 
+// d = a b + c, a b, a + b over VEC elements, two an instruction
+template <int VEC, typename A, typename B, typename X>
+__device__ __forceinline__ void vfma(float (&d)[VEC], const A& a, const B& b, const X& c) {
+#pragma unroll
+    for (int i = 0; i + 1 < VEC; i += 2) {
+        const float2 r = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), make_float2(c[i], c[i + 1]));
+        d[i] = r.x;
+        d[i + 1] = r.y;
+    }
+    if (VEC & 1) d[VEC - 1] = fmaf(a[VEC - 1], b[VEC - 1], c[VEC - 1]);
+}
+template <int VEC, typename A, typename B>
+__device__ __forceinline__ void vmul(float (&d)[VEC], const A& a, const B& b) {
+#pragma unroll
+    for (int i = 0; i + 1 < VEC; i += 2) {
+        const float2 r = __fmul2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+        d[i] = r.x;
+        d[i + 1] = r.y;
+    }
+    if (VEC & 1) d[VEC - 1] = a[VEC - 1] * b[VEC - 1];
+}
+template <int VEC, typename A, typename B>
+__device__ __forceinline__ void vadd(float (&d)[VEC], const A& a, const B& b) {
+#pragma unroll
+    for (int i = 0; i + 1 < VEC; i += 2) {
+        const float2 r = __fadd2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]));
+        d[i] = r.x;
+        d[i + 1] = r.y;
+    }
+    if (VEC & 1) d[VEC - 1] = a[VEC - 1] + b[VEC - 1];
+}
+struct Same { float v; __device__ __forceinline__ float operator[](int) const { return v; } };  // one number for all of them
+// sums over a thread's elements, in two halves
+template <int VEC>
+__device__ __forceinline__ float2 sum2(float2 s, const float (&a)[VEC]) {
+#pragma unroll
+    for (int i = 0; i + 1 < VEC; i += 2) s = __fadd2_rn(make_float2(a[i], a[i + 1]), s);
+    if (VEC & 1) s.x += a[VEC - 1];
+    return s;
+}
+template <int VEC>
+__device__ __forceinline__ float2 dot2(float2 s, const float (&a)[VEC], const float (&b)[VEC]) {
+#pragma unroll
+    for (int i = 0; i + 1 < VEC; i += 2) s = __ffma2_rn(make_float2(a[i], a[i + 1]), make_float2(b[i], b[i + 1]), s);
+    if (VEC & 1) s.x = fmaf(a[VEC - 1], b[VEC - 1], s.x);
+    return s;
+}
+
 // FP32 values go through expf and a division, BF16 ones through the hardware's 2^x and 1 / x (2 ulp and 1, and |z| 2^-24 from the
 // argument)
-template <typename T>
-__device__ __forceinline__ float sigmoid(float z) {
-    return sizeof(T) == 4 ? 1.f / (1.f + expf(-z)) : rcp_ftz(1.f + ex2_ftz(-LOG2E * z));
+template <typename T, int VEC>
+__device__ __forceinline__ void sigmoid(float (&s)[VEC], const float (&z)[VEC]) {
+    if (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = 1.f / (1.f + expf(-z[i]));
+    } else {
+        vmul(s, z, Same{-LOG2E});
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = ex2_ftz(s[i]);
+        vadd(s, s, Same{1.f});
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) s[i] = rcp_ftz(s[i]);
+    }
 }
-template <typename T>
-__device__ __forceinline__ float act(float z, bool silu) { return silu ? z * sigmoid<T>(z) : z; }
-// dy act'(z)
-template <typename T>
-__device__ __forceinline__ float act_grad(float z, float dy, bool silu) {
-    if (!silu) return dy;
-    const float s = sigmoid<T>(z);
-    return dy * s * fmaf(z, 1.f - s, 1.f);
+template <typename T, int VEC>
+__device__ __forceinline__ void act(float (&y)[VEC], const float (&z)[VEC], bool silu) {
+    if (silu) {
+        sigmoid<T>(y, z);
+        vmul(y, y, z);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) y[i] = z[i];
+    }
+}
+// dz = dy act'(z), act'(z) = s + s z (1 - s)
+template <typename T, int VEC>
+__device__ __forceinline__ void act_grad(float (&dz)[VEC], const float (&z)[VEC], const float (&dy)[VEC], bool silu) {
+    if (silu) {
+        float s[VEC], u[VEC];
+        sigmoid<T>(s, z);
+        vfma(u, s, Same{-1.f}, Same{1.f});
+        vfma(u, u, z, Same{1.f});
+        vmul(s, s, dy);
+        vmul(dz, s, u);
+    } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) dz[i] = dy[i];
+    }
 }
 // over L = 2^i lanes
 __device__ __forceinline__ float lanes_sum(float v, int L) {
@@ -113,7 +188,7 @@ __device__ __forceinline__ float inv_sqrt(float v) { return sizeof(T) == 4 ? 1.f
 // ---- one row at a time ------------------------------------------------------------------------------------------------
 // Slots of L lanes; slot s has group s mod G and rows s / G, s / G + step, ...  Every lane of a warp makes the same number of turns.
 template <typename T, int VEC, int NV, bool BWD>
-__global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 2 : 1) group_norm_rows_kernel(const Args a, int L) {
+__global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? (BWD ? 3 : 4) : NV * VEC <= 16 ? 2 : 1) group_norm_rows_kernel(const Args a, int L) {
     const int lane = threadIdx.x & (L - 1), Cg = a.Ch / a.G;
     const long long slot = ((long long)blockIdx.x * NTHR + threadIdx.x) / L, slots = (long long)gridDim.x * NTHR / L;
     const long long step = slots / a.G;            // rows between a slot's rows; slots beyond step * G have none
@@ -155,56 +230,54 @@ __global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? 4 : NV * VEC <= 16 ? 2 :
         const long long n = slot / a.G + k * step;
         const bool on = !idle && n < a.N;
         const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
-        float x[NV][VEC], dy[NV][VEC], s = 0.f;
+        float x[NV][VEC], dy[NV][VEC];
+        float2 s = make_float2(0.f, 0.f), q = s;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             unpack(nx[j], x[j]);
             if (BWD) unpack(ndy[j], dy[j]);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) s += x[j][i];
+            s = sum2(s, x[j]);
         }
         if (k + 1 < turns) request(k + 1);
-        const float mean = lanes_sum(s, L) * inv;
-        float q = 0.f;
+        const float mean = lanes_sum(s.x + s.y, L) * inv;
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                x[j][i] = (j * L + lane) * VEC < Cg ? x[j][i] - mean : 0.f;
-                q = fmaf(x[j][i], x[j][i], q);
-            }
-        const float rstd = inv_sqrt<T>(lanes_sum(q, L) * inv + a.eps);
+        for (int j = 0; j < NV; ++j) {
+            vadd(x[j], x[j], Same{-mean});
+            if ((j * L + lane) * VEC < Cg) q = dot2(q, x[j], x[j]);
+        }
+        const float var = lanes_sum(q.x + q.y, L) * inv, rstd = on ? inv_sqrt<T>(var + a.eps) : 0.f;  // (no row: no infinity into dw, db)
         if (!BWD) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * L + lane) * VEC;
                 float y[VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) y[i] = act<T>(fmaf(x[j][i] * rstd, w[j][i], b[j][i]), silu);
+                vmul(x[j], x[j], Same{rstd});
+                vfma(x[j], x[j], w[j], b[j]);
+                act<T>(y, x[j], silu);
                 if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.y) + base + c, y);
             }
         } else {
-            float m1 = 0.f, m2 = 0.f;
+            float2 t1 = make_float2(0.f, 0.f), t2 = t1;
 #pragma unroll
-            for (int j = 0; j < NV; ++j)
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    x[j][i] *= rstd;
-                    const float dz = act_grad<T>(fmaf(x[j][i], w[j][i], b[j][i]), dy[j][i], silu);
-                    db[j][i] += dz;
-                    dw[j][i] = fmaf(dz, x[j][i], dw[j][i]);
-                    dy[j][i] = dz * w[j][i];
-                    m1 += dy[j][i];
-                    m2 = fmaf(dy[j][i], x[j][i], m2);
-                }
-            m1 = lanes_sum(m1, L) * inv;
-            m2 = lanes_sum(m2, L) * inv;
+            for (int j = 0; j < NV; ++j) {  // (beyond the group's end dy = 0)
+                float z[VEC];
+                vmul(x[j], x[j], Same{rstd});
+                vfma(z, x[j], w[j], b[j]);
+                act_grad<T>(dy[j], z, dy[j], silu);
+                vadd(db[j], db[j], dy[j]);
+                vfma(dw[j], dy[j], x[j], dw[j]);
+                vmul(dy[j], dy[j], w[j]);
+                t1 = sum2(t1, dy[j]);
+                t2 = dot2(t2, dy[j], x[j]);
+            }
+            const float m1 = -lanes_sum(t1.x + t1.y, L) * inv, m2 = -lanes_sum(t2.x + t2.y, L) * inv;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
                 const int c = (j * L + lane) * VEC;
                 float dx[VEC];
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) dx[i] = rstd * (dy[j][i] - m1 - x[j][i] * m2);
+                vadd(dx, dy[j], Same{m1});  // (before rstd: a group of one channel has exactly 0)
+                vfma(dx, x[j], Same{m2}, dx);
+                vmul(dx, dx, Same{rstd});
                 if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.dx) + base + c, dx);
             }
         }
@@ -244,6 +317,8 @@ __global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* pa
 // ---- samples of several positions -------------------------------------------------------------------------------------
 // A CTA has one slice of one sample; thread = (row of TR, VEC channels), channels in blocks of SLICE_THR * VEC where a row is wider than
 // the CTA.
+// CTAs per SM that registers allow without spilling
+__host__ __device__ constexpr int slice_ctas(bool bwd) { return bwd ? 2 : 3; }
 struct Slice {
     long long n, s0, s1;
     __device__ __forceinline__ Slice(const Args& a) {
@@ -259,7 +334,7 @@ __device__ __forceinline__ float* group_part(const Args& a) { return a.part + (s
 // MODE 0: sums of x - x0 and (x - x0)^2 about the slice's first row x0, and from them a group's mean and sum of squared deviations;
 // 1: sums of dz x^ and dz, and over a group's channels w times those
 template <typename T, int VEC, int MODE>
-__global__ void __launch_bounds__(SLICE_THR, VEC <= 8 ? 3 : 1) group_norm_sums_kernel(const Args a) {
+__global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_kernel(const Args a) {
     extern __shared__ float sm[];                  // [2][TR][TC * VEC]
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
@@ -279,6 +354,7 @@ __global__ void __launch_bounds__(SLICE_THR, VEC <= 8 ? 3 : 1) group_norm_sums_k
         if (on) {
             if (MODE == 0) {
                 load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, p);
+                vmul(p, p, Same{-1.f});
             } else {
                 mu = a.mean[n * a.G + c / Cg];
                 rs = a.rstd[n * a.G + c / Cg];
@@ -294,21 +370,18 @@ __global__ void __launch_bounds__(SLICE_THR, VEC <= 8 ? 3 : 1) group_norm_sums_k
                 float x[VEC];
                 load<T, VEC>(X + (size_t)s * a.Ch + c, x);
                 if (MODE == 0) {
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        const float d = x[i] - p[i];
-                        s1[i] += d;
-                        s2[i] = fmaf(d, d, s2[i]);
-                    }
+                    vadd(x, x, p);
+                    vadd(s1, s1, x);
+                    vfma(s2, x, x, s2);
                 } else {
-                    float dy[VEC];
+                    float dy[VEC], z[VEC];
                     load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) {
-                        const float xh = (x[i] - mu) * rs, dz = act_grad<T>(fmaf(xh, w[i], b[i]), dy[i], silu);
-                        s1[i] = fmaf(dz, xh, s1[i]);
-                        s2[i] += dz;
-                    }
+                    vadd(x, x, Same{-mu});
+                    vmul(x, x, Same{rs});
+                    vfma(z, x, w, b);
+                    act_grad<T>(dy, z, dy, silu);
+                    vfma(s1, dy, x, s1);
+                    vadd(s2, s2, dy);
                 }
             }
         }
@@ -357,7 +430,7 @@ __global__ void __launch_bounds__(SLICE_THR, VEC <= 8 ? 3 : 1) group_norm_sums_k
 }
 
 template <typename T, int VEC, bool BWD>
-__global__ void __launch_bounds__(SLICE_THR, 3) group_norm_apply_kernel(const Args a) {
+__global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_kernel(const Args a) {
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
     const Slice sl(a);
@@ -406,6 +479,7 @@ __global__ void __launch_bounds__(SLICE_THR, 3) group_norm_apply_kernel(const Ar
         __syncthreads();
     }
     if (tr >= TR) return;
+    constexpr int UNROLL = BWD ? 2 : 4;
     const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
     const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
     T* Y = static_cast<T*>(BWD ? a.dx : a.y) + (size_t)n * a.S * a.Ch;
@@ -422,15 +496,20 @@ __global__ void __launch_bounds__(SLICE_THR, 3) group_norm_apply_kernel(const Ar
             w[i] = rs * (a.w ? a.w[c + i] : 1.f);
             b[i] = a.b ? a.b[c + i] : 0.f;
         }
-#pragma unroll(BWD ? 2 : 4)
+#pragma unroll UNROLL
         for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
             float x[VEC], dy[VEC], y[VEC];
             load<T, VEC>(X + (size_t)s * a.Ch + c, x);
             if (BWD) load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float d = x[i] - mu, z = fmaf(d, w[i], b[i]);
-                y[i] = BWD ? fmaf(act_grad<T>(z, dy[i], silu), w[i], fmaf(d, k2, k1)) : act<T>(z, silu);
+            float d[VEC], z[VEC];
+            vadd(d, x, Same{-mu});
+            vfma(z, d, w, b);
+            if (BWD) {
+                act_grad<T>(y, z, dy, silu);
+                vfma(d, d, Same{k2}, Same{k1});
+                vfma(y, y, w, d);
+            } else {
+                act<T>(y, z, silu);
             }
             store<T, VEC>(Y + (size_t)s * a.Ch + c, y);
         }
@@ -440,9 +519,9 @@ __global__ void __launch_bounds__(SLICE_THR, 3) group_norm_apply_kernel(const Ar
 // ---- launches -----------------------------------------------------------------------------------------------------------
 static bool by_rows(long long S, int Ch, int G) { return S == 1 && Ch / G <= ROWS_MAX; }
 
-// slices of a sample: three CTAs per SM (what their registers allow) over all samples, of at least 8 rows, all but the last of the same length
-static void cut(Args& a) {
-    long long want = 3LL * sm_count() / a.N, most = (a.S + 7) / 8;
+// slices of a sample: as many as are resident over all samples, of at least 8 rows, all but the last of the same length
+static void cut(Args& a, bool bwd) {
+    long long want = (long long)slice_ctas(bwd) * sm_count() / a.N, most = (a.S + 7) / 8;
     if (want > most) want = most;
     if (want > MAX_SLICES) want = MAX_SLICES;
     if (want < 1) want = 1;
@@ -457,7 +536,7 @@ static RowsGrid rows_grid(long long N, int Ch, int G, int vec, bool bwd) {
     r.L = 1;
     while (r.L < 32 && r.L * vec < Cg) r.L *= 2;
     const long long per = NTHR / r.L, need = (N * G + per - 1) / per;
-    long long most = (bwd ? 4LL : 8LL) * sm_count();
+    long long most = (bwd ? 3 : 4) * (long long)sm_count();
     const long long least = (G + per - 1) / per;   // every group has a slot
     if (most < least) most = least;
     r.ctas = need < least ? least : need < most ? need : most;
@@ -528,7 +607,7 @@ static size_t scratch(long long N, long long S, int Ch, int G, int es, bool bwd)
     }
     Args a = {};
     a.N = N; a.S = S;
-    cut(a);
+    cut(a, bwd);
     return (size_t)N * a.slices * 2 * (Ch + G) * sizeof(float);
 }
 
@@ -556,7 +635,7 @@ extern "C" int kda_group_norm_fwd(const void* x, const float* weight, const floa
     a.N = N; a.S = S; a.Ch = channels; a.G = groups; a.act = silu; a.eps = eps;
     if (const int rc = gn::check(a, dtype)) return rc;
     if (!x || !y || (!gn::by_rows(S, channels, groups) && (!mean || !rstd || !scratch))) return KDA_ERR_NULL;
-    gn::cut(a);
+    gn::cut(a, false);
     const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, false>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, false>(a, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }
@@ -571,7 +650,7 @@ extern "C" int kda_group_norm_bwd(const void* x, const float* weight, const floa
     if (const int rc = gn::check(a, dtype)) return rc;
     const bool rows = gn::by_rows(S, channels, groups);
     if (!x || !dy || !dx || (!rows && (!mean || !rstd || !scratch)) || (dweight && (!dbias || !scratch)) || (!dweight && dbias)) return KDA_ERR_NULL;
-    gn::cut(a);
+    gn::cut(a, true);
     const cudaError_t e = dtype == KDA_DTYPE_F32 ? gn::dispatch<float, true>(a, (cudaStream_t)stream) : gn::dispatch<gn::bf16, true>(a, (cudaStream_t)stream);
     return e == cudaSuccess ? KDA_OK : fail_cuda(e);
 }

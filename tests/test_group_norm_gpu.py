@@ -90,6 +90,15 @@ def test_offsets_far_above_the_spread(shape):
         assert float((a.double() - r).abs().max()) <= 4 * 1000 * 2.0 ** -24 * float(r.abs().max())
 
 
+@pytest.mark.parametrize("shape,G", [((7, 768), 6), ((333, 96), 3), ((2, 33, 96), 3)])
+def test_without_an_epsilon(shape, G):
+    """Lanes that have no row in a turn add nothing to the parameters' gradients, where 1 / sqrt(0) would be infinite."""
+    gen = torch.Generator().manual_seed(6)
+    x, dy = torch.randn(*shape, generator=gen).cuda(), torch.randn(*shape, generator=gen).cuda()
+    w, b = torch.rand(shape[-1], generator=gen).cuda(), torch.randn(shape[-1], generator=gen).cuda()
+    check(run(x, G, w, b, 0.0, True, dy), reference(x, G, w, b, 0.0, True, dy), terms=4 * dy.double().abs().reshape(-1, shape[-1]).sum(0).max())
+
+
 def test_constant_input_and_large_values():
     from openkimi_b200 import group_norm
 
