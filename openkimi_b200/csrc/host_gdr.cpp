@@ -2,6 +2,8 @@
 // memory, autograd and launches.  Nothing is kept from one call for the next.
 #include "host_util.h"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 using namespace kda_host;
 
 namespace {
@@ -18,6 +20,20 @@ int code(at::ScalarType t) { return t == at::kBFloat16 ? KDA_DTYPE_BF16 : KDA_DT
 // type in which the kernels read g and beta: theirs where they share one that the kernels have, else FP32
 at::ScalarType gate_type(const Tensor& g, const Tensor& beta) {
     return g.scalar_type() == at::kBFloat16 && beta.scalar_type() == at::kBFloat16 ? at::kBFloat16 : at::kFloat;
+}
+
+// Gradients whose own derivative is asked for (create_graph) raise when it is taken: the backward kernels have none.
+variable_list differentiable_once(const char* what, variable_list r) {
+    if (!at::GradMode::is_enabled()) return r;
+    variable_list have;
+    for (const Tensor& t : r)
+        if (t.defined()) have.push_back(t.detach().requires_grad_());
+    const std::string msg = std::string("the gradient of ") + what + " is not differentiable: its backward has no derivative";
+    const variable_list out = (*std::make_shared<torch::autograd::DelayedError>(msg, (int64_t)have.size()))(std::move(have));
+    size_t i = 0;
+    for (Tensor& t : r)
+        if (t.defined()) t = out[i++];
+    return r;
 }
 
 // ---- gated delta rule ------------------------------------------------------------------------------------------------
@@ -201,7 +217,7 @@ struct ChunkGdr : torch::autograd::Function<ChunkGdr> {
         c10::cuda::CUDAGuard guard(in.q.device());
         const Grads r = run_bwd(in, sp, s[12], grads[0], grads.size() > 1 ? grads[1] : Tensor());
         // (the engine casts every gradient to its input's dtype)
-        return {r.q, r.k, r.v, r.g, r.beta, r.A_log, r.dt_bias, r.h0, Tensor(), Tensor()};
+        return differentiable_once("chunk_gated_delta_rule", {r.q, r.k, r.v, r.g, r.beta, r.A_log, r.dt_bias, r.h0, Tensor(), Tensor()});
     }
 };
 
@@ -357,7 +373,7 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
                                         (float)ctx->saved_data["eps"].toDouble(), (int)z[4], dt, stream_of(x)),
                      "kda_group_norm_bwd");
         }
-        return {dx, w.defined() ? dw : Tensor(), b.defined() ? db : Tensor(), Tensor()};
+        return differentiable_once("group_norm", {dx, w.defined() ? dw : Tensor(), b.defined() ? db : Tensor(), Tensor()});
     }
 };
 

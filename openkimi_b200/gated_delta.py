@@ -26,6 +26,9 @@ def _offsets(cu: tuple, device_index: int):
     return torch.tensor(cu, dtype=torch.int64, device=torch.device("cuda", device_index))
 
 
+_in_graphs: dict = {}  # tables that captured graphs read: a graph outlives what the caches above keep
+
+
 @torch.compiler.disable
 def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, output_final_state=False,
                            use_qk_l2norm_in_kernel=False, use_gate_in_kernel=False, use_beta_sigmoid_in_kernel=False,
@@ -43,8 +46,9 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
     outputs and gradients.
 
     Sums, states and pairwise decays are in FP32; BF16 inputs are multiplied exactly and computed operands in 24 bits, so a final
-    state or a gradient in FP32 is one to FP32 accuracy.  Differentiated calls keep about (4 K V + 256 V + 33000) bytes per 64 tokens
-    and value head for the backward.  Returns ``(o [B, T, HV, V], final_state or None)``.
+    state or a gradient in FP32 is one to FP32 accuracy.  Differentiated calls keep about (4 K V + 256 V + 34000) bytes per 64 tokens
+    and value head for the backward (BF16 with K = V = 128: 173 KB), and where few long sequences are cut into segments 8 K V per
+    segment.  A gradient is not differentiable again.  Returns ``(o [B, T, HV, V], final_state or None)``.
     """
     tables = (None, None, None, None, 0, 0, True)
     if cu_seqlens is not None or cu_seqlens_cpu is not None:
@@ -61,6 +65,8 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
         seq, off, nt, tab, longest = _chunk_tables(None, host, q.device, tokens)
         cu = tuple(int(x) for x in host.tolist())
         tables = (_offsets(cu, q.device.index or 0), seq, off, tab, nt, longest, cu[0] == 0 and cu[-1] == tokens)
+        if torch.cuda.is_current_stream_capturing():
+            _in_graphs.setdefault((cu, q.device.index or 0), tables)
     return _lib.host().chunk_gdr(q, k, v, g, beta, A_log, dt_bias, initial_state, scale,
                                  _flags(use_qk_l2norm_in_kernel, use_gate_in_kernel, use_beta_sigmoid_in_kernel, state_v_first),
                                  bool(output_final_state), *tables)
