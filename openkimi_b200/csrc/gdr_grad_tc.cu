@@ -8,7 +8,7 @@
 //
 // One CTA per SM walks the (chunk, value head) units.  A warp copies the records' K-steps into shared memory, eight warps take <S0, dS>
 // and leave three BF16 parts in a ring of two K-steps; one issues the products; one brings the next unit's rows; sixteen do the rest
-// of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  3072 units take 360 us: 256 KB of records
+// of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  3072 units take 365 us (732 on mma.sync): 256 KB of records
 // and rows per unit, 2.2 TB/s, a third of the copy's rate.  What bounds it is shared memory's pipe: the copy of the records in, their
 // conversion (read once, written in 1.5 times the bytes), the MMAs' operands and the exchange of rows and columns come to about
 // 28000 of the 33000 cycles of a unit, and twice the warps for either part gained nothing.  An MMA whose A operand lies in shared
@@ -25,7 +25,7 @@ namespace gt {
 constexpr int MAIN = 512, CONV = 256, NTHR = 896, RING = 2, K = 128;
 constexpr int W_CONV = MAIN / 32, W_MMA = W_CONV + CONV / 32, W_ROWS = W_MMA + 1, W_COPY = W_ROWS + 1;  // the other warps; the last is the gate's
 // registers of the main, converting and other warps; 16 x 80 + 8 x 56 + 4 x 72 = 28 x 72 a lane
-constexpr int REG_MAIN = 80, REG_CONV = 56, REG_REST = 72;
+constexpr int REG_MAIN = 80, REG_CONV = 56;  // the rest keep the 72 of the launch
 constexpr uint32_t MAT = SQ * 2;
 // the rows of a unit: q, k as two halves of 64 columns with 128-byte swizzle
 constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;

@@ -11,6 +11,10 @@
 //     row, joined over the slice's channels to (mean, sum of squared deviations) of a group, and over the slices at the start of the
 //     second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which give dw, db and, weighted with w,
 //     m1 and m2; then dx.  The second pass reads from L2 what fits there.
+// Bound by issue slots (70 % of them used in the first form) and by the latency of small slices: [32768, 768] in groups of 128, BF16
+// with SiLU, takes 29 us forward (3.5 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups GNF and GNB.  Two values an
+// instruction (three for the sigmoid's), a thread's channels all of one group and a grid of what is resident made 209 us of the latter's
+// two directions GNT.
 // Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
 #include "kda_common.cuh"
 
@@ -328,7 +332,7 @@ struct Slice {
         s1 = min(a.S, s0 + a.len);
     }
 };
-// scratch: [N * slices][2][Ch] sums of the channels, then [N * slices][G][2] numbers of the groups
+// scratch: [N * slices][2][Ch] sums of the channels, then [N][G][slices][2] numbers of the groups
 __device__ __forceinline__ float* group_part(const Args& a) { return a.part + (size_t)a.N * a.slices * 2 * a.Ch; }
 
 // MODE 0: sums of x - x0 and (x - x0)^2 about the slice's first row x0, and from them a group's mean and sum of squared deviations;
@@ -399,33 +403,36 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
             float s = 0.f;
             for (int r = 0; r < TR; ++r) s += sm[(which * TR + r) * TC * VEC + cc];
             out[(size_t)which * a.Ch + v0 * VEC + cc] = s;
+            sm[which * TR * TC * VEC + cc] = s;
         }
     }
-    __syncthreads();  // (the sums are read back by the CTA that wrote them)
-    float* groups = group_part(a) + (size_t)blockIdx.x * a.G * 2;
+    __syncthreads();
+    // a row as wide as one block of channels is still in shared memory; else the CTA reads back what it wrote
+    const float *sum1 = cols <= TC ? sm : out, *sum2 = cols <= TC ? sm + TR * TC * VEC : out + a.Ch;
+    float* groups = group_part(a) + ((size_t)n * a.G * a.slices + blockIdx.x % a.slices) * 2;
     const int lane = threadIdx.x & 31;
     const float m = (float)(sl.s1 - sl.s0);
     for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
         float u = 0.f, v = 0.f;
         if (MODE == 0) {
-            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) u += fmaf(m, ldf(X + (size_t)sl.s0 * a.Ch + c), out[c]);
+            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) u += fmaf(m, ldf(X + (size_t)sl.s0 * a.Ch + c), sum1[c]);
             u = warp_sum(u) / (m * Cg);
             // sum (x - mean)^2 = sum (x - x0)^2 + 2 (x0 - mean) sum (x - x0) + m (x0 - mean)^2
             for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
                 const float d = ldf(X + (size_t)sl.s0 * a.Ch + c) - u;
-                v += fmaf(d, fmaf(m, d, 2.f * out[c]), out[a.Ch + c]);
+                v += fmaf(d, fmaf(m, d, 2.f * sum1[c]), sum2[c]);
             }
             v = warp_sum(v);
         } else {
             for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
                 const float w = a.w ? a.w[c] : 1.f;
-                v = fmaf(w, out[c], v);
-                u = fmaf(w, out[a.Ch + c], u);
+                v = fmaf(w, sum1[c], v);
+                u = fmaf(w, sum2[c], u);
             }
             u = warp_sum(u);
             v = warp_sum(v);
         }
-        if (lane == 0) *reinterpret_cast<float2*>(groups + 2 * g) = make_float2(u, v);
+        if (lane == 0) *reinterpret_cast<float2*>(groups + (size_t)g * a.slices * 2) = make_float2(u, v);
     }
 }
 
@@ -438,18 +445,19 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
     extern __shared__ float stat[];                // [G][2]: mean, rstd; backward: m1, m2
     pdl_wait();
     {   // the sample's slices, a warp per group; means about the first slice's
-        const float2* groups = reinterpret_cast<const float2*>(group_part(a)) + (size_t)n * a.slices * a.G;
+        const float2* groups = reinterpret_cast<const float2*>(group_part(a)) + (size_t)n * a.slices * a.G;  // [G][slices]
         const int lane = threadIdx.x & 31;
         const float rows = (float)a.len, tail = (float)(a.S - (a.slices - 1) * a.len), count = (float)a.S * Cg;
         for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
             float2 p[MAX_SLICES / 32];
-            const float u0 = BWD ? 0.f : groups[g].x;
+            const float2* of = groups + (size_t)g * a.slices;
+            const float u0 = BWD ? 0.f : of[0].x;
             float u = 0.f, v = 0.f;
 #pragma unroll
             for (int j = 0; j < MAX_SLICES / 32; ++j)
                 if (j * 32 < a.slices) {
                     const int i = j * 32 + lane;
-                    p[j] = i < a.slices ? groups[(size_t)i * a.G + g] : make_float2(u0, 0.f);
+                    p[j] = i < a.slices ? of[i] : make_float2(u0, 0.f);
                     p[j].x -= u0;
                     u += BWD ? p[j].x : p[j].x * (i == a.slices - 1 ? tail : rows);
                     v += p[j].y;
