@@ -12,9 +12,9 @@
 //     second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which give dw, db and, weighted with w,
 //     m1 and m2; then dx.  The second pass reads from L2 what fits there.
 // Bound by issue slots (70 % of them used in the first form) and by the latency of small slices: [32768, 768] in groups of 128, BF16
-// with SiLU, takes 29 us forward (3.5 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups GNF and GNB.  Two values an
-// instruction (three for the sigmoid's), a thread's channels all of one group and a grid of what is resident made 209 us of the latter's
-// two directions GNT.
+// with SiLU, takes 29 us forward (3.5 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups 47 and 64 (3.2 and 4.3 TB/s of
+// what its passes read and write).  In the first form the two took 172 and 291 us; what made them faster is two values an instruction, a
+// thread's channels all of one group, rows kept as they lie in memory until they are used, and a grid of what is resident.
 // Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
 #include "kda_common.cuh"
 
@@ -26,7 +26,6 @@ constexpr int NTHR = 256;
 constexpr int SLICE_THR = 384;    // at most, in the kernels over slices
 constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
 constexpr int MAX_SLICES = 256;
-
 constexpr int GROUPS_MAX = 24576; // groups whose numbers fit shared memory where they are not taken row by row
 
 struct Args {
@@ -332,6 +331,47 @@ struct Slice {
         s1 = min(a.S, s0 + a.len);
     }
 };
+// A thread's rows of a slice, every TR-th, VEC channels each: f(row, x, dy).  The next U rows are on their way while U are used (a load
+// of x would not pass a store to y by itself), the first ones from the constructor on.
+template <typename T, int VEC, bool TWO, int U>
+struct Rows {
+    const T *X, *D;
+    long long s, s1;
+    int TR, Ch;
+    Raw<T, VEC> nx[U], nd[U];
+    __device__ __forceinline__ Rows(const T* X, const T* D, const Slice& sl, int tr, int TR, int Ch) : X(X), D(D), s(sl.s0 + tr), s1(sl.s1), TR(TR), Ch(Ch) { request(s); }
+    __device__ __forceinline__ void request(long long at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (at + u * TR < s1) {
+                nx[u] = load_raw<T, VEC>(X + (size_t)(at + u * TR) * Ch);
+                if (TWO) nd[u] = load_raw<T, VEC>(D + (size_t)(at + u * TR) * Ch);
+            }
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        for (; s < s1; s += U * TR) {
+            Raw<T, VEC> rx[U], rd[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                rx[u] = nx[u];
+                if (TWO) rd[u] = nd[u];
+            }
+            request(s + U * TR);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (s + u * TR < s1) {
+                    float x[VEC], dy[VEC];
+                    unpack(rx[u], x);
+                    if (TWO) unpack(rd[u], dy);
+                    f(s + u * TR, x, dy);
+                }
+        }
+    }
+};
+// rows in flight, what registers allow: [4, 8191, 768] BF16 in 32 groups, sums of the backward 29 us with one and 37 with two; its second
+// pass 31 with two and 33 with one
+template <int VEC> constexpr int rows_ahead(bool two) { return VEC <= 2 ? 4 : VEC == 4 || !two ? 2 : 1; }
 // scratch: [N * slices][2][Ch] sums of the channels, then [N][G][slices][2] numbers of the groups
 __device__ __forceinline__ float* group_part(const Args& a) { return a.part + (size_t)a.N * a.slices * 2 * a.Ch; }
 
@@ -356,6 +396,7 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
 #pragma unroll
         for (int i = 0; i < VEC; ++i) s1[i] = s2[i] = 0.f;
         if (on) {
+            Rows<T, VEC, MODE, rows_ahead<VEC>(MODE)> rows(X + c, D + c, sl, tr, TR, a.Ch);
             if (MODE == 0) {
                 load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, p);
                 vmul(p, p, Same{-1.f});
@@ -369,17 +410,13 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
                 w[i] = MODE && a.w ? a.w[c + i] : 1.f;
                 b[i] = MODE && a.b ? a.b[c + i] : 0.f;
             }
-#pragma unroll 4
-            for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
-                float x[VEC];
-                load<T, VEC>(X + (size_t)s * a.Ch + c, x);
+            rows.each([&](long long, float (&x)[VEC], float (&dy)[VEC]) {
                 if (MODE == 0) {
                     vadd(x, x, p);
                     vadd(s1, s1, x);
                     vfma(s2, x, x, s2);
                 } else {
-                    float dy[VEC], z[VEC];
-                    load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
+                    float z[VEC];
                     vadd(x, x, Same{-mu});
                     vmul(x, x, Same{rs});
                     vfma(z, x, w, b);
@@ -387,7 +424,7 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
                     vfma(s1, dy, x, s1);
                     vadd(s2, s2, dy);
                 }
-            }
+            });
         }
         if (v0) __syncthreads();
 #pragma unroll
@@ -444,6 +481,10 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
     const long long n = sl.n;
     extern __shared__ float stat[];                // [G][2]: mean, rstd; backward: m1, m2
     pdl_wait();
+    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
+    const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
+    T* Y = static_cast<T*>(BWD ? a.dx : a.y) + (size_t)n * a.S * a.Ch;
+    Rows<T, VEC, BWD, rows_ahead<VEC>(false)> rows(X + tc * VEC, D + tc * VEC, sl, tr < TR ? tr : 0, TR, a.Ch);
     {   // the sample's slices, a warp per group; means about the first slice's
         const float2* groups = reinterpret_cast<const float2*>(group_part(a)) + (size_t)n * a.slices * a.G;  // [G][slices]
         const int lane = threadIdx.x & 31;
@@ -487,10 +528,6 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
         __syncthreads();
     }
     if (tr >= TR) return;
-    constexpr int UNROLL = BWD ? 2 : 4;
-    const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
-    const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
-    T* Y = static_cast<T*>(BWD ? a.dx : a.y) + (size_t)n * a.S * a.Ch;
     const bool silu = a.act;
     for (int v = tc; v < cols; v += TC) {
         const int c = v * VEC;
@@ -504,11 +541,9 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
             w[i] = rs * (a.w ? a.w[c + i] : 1.f);
             b[i] = a.b ? a.b[c + i] : 0.f;
         }
-#pragma unroll UNROLL
-        for (long long s = sl.s0 + tr; s < sl.s1; s += TR) {
-            float x[VEC], dy[VEC], y[VEC];
-            load<T, VEC>(X + (size_t)s * a.Ch + c, x);
-            if (BWD) load<T, VEC>(D + (size_t)s * a.Ch + c, dy);
+        if (v != tc) rows = Rows<T, VEC, BWD, rows_ahead<VEC>(false)>(X + c, D + c, sl, tr, TR, a.Ch);
+        rows.each([&](long long s, float (&x)[VEC], float (&dy)[VEC]) {
+            float y[VEC];
             float d[VEC], z[VEC];
             vadd(d, x, Same{-mu});
             vfma(z, d, w, b);
@@ -520,7 +555,7 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
                 act<T>(y, z, silu);
             }
             store<T, VEC>(Y + (size_t)s * a.Ch + c, y);
-        }
+        });
     }
 }
 
