@@ -43,8 +43,8 @@ inline int longest(const KdaGdrParams& p) {  // chunks of the longest sequence, 
 // Segments of the longest sequence in the walks on tcgen05 (gdr_tc.cu).  A walk is a chain of chunks; where walks are few, or one is
 // much longer than its share, sequences are cut into segments of equal length that are walked twice: from zero (and from the identity,
 // for what a segment does to the state that it is entered with), and again from the states that follow.  Estimated with what a chunk
-// costs (3.2 us without outputs, 3.7 us with), a border (3.3 us) and the launches (12 us): equal sequences go in waves, packed ones
-// fill the SMs up to half a segment.  8 walks of 512 chunks, forward: 2312 -> 494 us.
+// costs (3.2 us without outputs, 3.7 us with), a border (2.6 us) and the launches (12 us): equal sequences go in waves, packed ones
+// fill the SMs up to half a segment.  8 walks of 512 chunks, forward: 2312 -> 485 us.
 inline int segment_count(const KdaGdrParams& p) {
     if (!on_tc(p)) return 1;
     const int nc = longest(p), sms = sm_count();
@@ -57,7 +57,7 @@ inline int segment_count(const KdaGdrParams& p) {
     for (int s = 2; s <= nc / 2 && s <= 64; ++s) {
         const int len = (nc + s - 1) / s;
         const double t1 = p.cu_seqlens ? fill(2 * (all - 0.75 * walks * len), len) : waves(walks * (2 * s - 3), len),
-                     t2 = p.cu_seqlens ? fill(all, len) : waves(walks * s, len), t = 3.2 * t1 + 3.7 * t2 + 3.3 * (s - 2) + 12.0;
+                     t2 = p.cu_seqlens ? fill(all, len) : waves(walks * s, len), t = 3.2 * t1 + 3.7 * t2 + 2.6 * (s - 2) + 12.0;
         if (t < best) best = t, n = s;
     }
     // (segment buffers of 64 KB a segment and head)

@@ -10,7 +10,7 @@
 // Bound by the chain of a chunk: split S - S k - R - R T - V' - W k - S.  Everything else is off it: two producer warps bring the next
 // chunk's rows (core-matrix order) and records, one warp issues all products, four warps turn finished outputs into rows.  A chunk of
 // 64 tokens takes 4.5 us with few CTAs, 5.9 forward and 6.5 backward with 96 that save their records (16 x 2048 tokens of 6 heads: 189
-// and 208 us, 3.4 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.
+// and 208 us, 3 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.
 #include "gdr.cuh"
 
 namespace kda {
@@ -753,12 +753,13 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
 }
 
 // States at the segments' borders, 8 columns of one (sequence, head) per CTA: forward, E_j <- X_j E_{j-1} + E_j for j = 1, 2, ..; backward
-// (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  FP32 multiply-adds; the next segment's X arrives meanwhile.
-constexpr int LDX = 132;  // floats per row of X
+// (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  2.6 us a border (8 heads); FP32 multiply-adds; the X
+// of the next two segments arrive meanwhile.  2.6 us a border (8 heads); with 512 threads, two to a sum, 3.5.
+constexpr int LDX = 132, XBUF = 3;  // floats per row of X, its copies
 template <bool TR>
 __global__ void __launch_bounds__(256) gdr_borders_kernel(const KdaGdrParams p, const Layout lay, float* M, const float* X) {
-    extern __shared__ __align__(16) float sm[];  // X twice, then the columns [128][8]
-    float* cols = sm + 2 * 128 * LDX;
+    extern __shared__ __align__(16) float sm[];  // X three times, then the columns [128][8]
+    float* cols = sm + XBUF * 128 * LDX;
     const int tid = threadIdx.x, d = tid >> 1, c4 = (tid & 1) * 4, c0 = (blockIdx.x & 15) * 8;
     const size_t base = (size_t)(blockIdx.x >> 4) * lay.segs * 16384;
     pdl_wait();
@@ -769,19 +770,21 @@ __global__ void __launch_bounds__(256) gdr_borders_kernel(const KdaGdrParams p, 
     auto seg = [&](int i) { return TR ? last - 1 - i : 1 + i; };
     auto request = [&](int i) {
         const float* x = X + base + (size_t)seg(i) * 16384;
-        for (int q = tid; q < 4096; q += 256) cp_async16_z(sm + (i & 1) * 128 * LDX + (q >> 5) * LDX + (q & 31) * 4, x + 4 * q, true);
+        if (i < steps)
+            for (int q = tid; q < 4096; q += 256) cp_async16_z(sm + i % XBUF * 128 * LDX + (q >> 5) * LDX + (q & 31) * 4, x + 4 * q, true);
         cp_async_commit();
     };
     auto at = [&](int s) { return reinterpret_cast<float4*>(M + base + (size_t)s * 16384 + d * 128 + c0 + c4); };
-    request(0);
+    for (int i = 0; i < XBUF - 1; ++i) request(i);
+    float4 next = *at(seg(0));
     *reinterpret_cast<float4*>(cols + d * 8 + c4) = *at(TR ? last : 0);
     for (int i = 0; i < steps; ++i) {
-        if (i + 1 < steps) request(i + 1);
-        else cp_async_commit();
-        float4 acc = *at(seg(i));
-        cp_async_wait<1>();
+        float4 acc = next;
+        cp_async_wait<XBUF - 2>();
         __syncthreads();
-        const float* x = sm + (i & 1) * 128 * LDX;
+        request(i + XBUF - 1);  // (into what the step before read)
+        if (i + 1 < steps) next = *at(seg(i + 1));
+        const float* x = sm + i % XBUF * 128 * LDX;
 #pragma unroll 8
         for (int k = 0; k < 128; k += 4) {
             float w[4];
@@ -811,7 +814,7 @@ static cudaError_t walk(Kernel* k, dim3 grid, int bytes, const KdaGdrParams& p, 
 }
 template <bool TR>
 static cudaError_t borders(const KdaGdrParams& p, const Layout& l, float* m, cudaStream_t s) {
-    constexpr int bytes = (2 * 128 * LDX + 128 * 8) * 4;
+    constexpr int bytes = (XBUF * 128 * LDX + 128 * 8) * 4;
     if (l.segs < 3) return cudaSuccess;
     const cudaError_t e = allow_smem(gdr_borders_kernel<TR>, bytes);
     const float* x = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + l.segX);
