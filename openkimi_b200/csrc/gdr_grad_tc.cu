@@ -8,7 +8,7 @@
 //
 // One CTA per SM walks the (chunk, value head) units.  A warp copies the records' K-steps into shared memory, eight warps take <S0, dS>
 // and leave three BF16 parts in a ring of two K-steps; one issues the products; one brings the next unit's rows; sixteen do the rest
-// of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  3072 units take 365 us (732 on mma.sync):
+// of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  16 x 2048 tokens of 6 heads take 365 us (732 on mma.sync):
 // 375 KB of records, rows and gradients per unit, 3.1 TB/s, half of the copy's rate.  What bounds it is shared memory's pipe: the copy
 // of the records in, their conversion (read once, written in 1.5 times the bytes), the MMAs' operands and the exchange of rows and
 // columns; twice the warps for either part gained nothing.  An MMA whose A operand lies in shared memory takes N / 2 + 43 cycles here
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 leave(b + S0 + 16 * t, SPART, x[0]);
                 leave(b + DS + 16 * t, SPART, x[1]);
                 if (first) {
-                    leave(b + V + (t >> 6) * 3072 + 16 * (t & 63), 1024, x[2]);
+                    leave(b + V + (t >> 6) * (3 * 1024) + 16 * (t & 63), 1024, x[2]);
                 } else {
                     unsigned char* rows = b + gt::B + (row >> 3) * 256 + (t & 1) * 128 + (row & 7) * 16;
                     *reinterpret_cast<uint4*>(rows) = od;
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                     for (int i = 0; i < 3; ++i) {
                         S[i] = make_desc(b + S0 + i * SPART, 2048, 128);
                         D[i] = make_desc(b + DS + i * SPART, 2048, 128);
-                        W[i] = make_desc(b + V + i * 1024, 3072, 128);
+                        W[i] = make_desc(b + V + i * 1024, 3 * 1024, 128);
                     }
                     const uint64_t dO = make_desc(b + gt::B, 128, 256), Y0 = make_desc(b + gt::B + YPART, 128, 256),
                                    Y1 = make_desc(b + gt::B + 2 * YPART, 128, 256), Y2 = make_desc(b + gt::B + 3 * YPART, 128, 256);

@@ -8,7 +8,7 @@
 // inverse goes by blocks: the four 16 x 16 diagonal blocks by substitution (a lane per column), then neighbours joined twice,
 // T_21 = -T_22 (L_21 T_11), in FP32 multiply-adds.
 //
-// Bound by latency between its barriers and by issue slots: 3072 units (BF16, 128 channels) take 90 us, 64 KB of HBM traffic a unit
+// Bound by latency between its barriers and by issue slots: 16 x 2048 tokens of 6 heads (BF16, 128 channels) take 90 us, 64 KB of HBM traffic a unit
 // at 2.1 TB/s.  The matrices take the place of the rows in shared memory, so that five CTAs fit an SM instead of three, the
 // gates of up to four heads are summed while the rows are on their way, and most decays are products of a row's and a column's
 // exponential: 116 us without the three.
