@@ -24,8 +24,8 @@ namespace gdr {
 namespace gt {
 constexpr int MAIN = 512, CONV = 256, NTHR = 896, RING = 2, K = 128;
 constexpr int W_CONV = MAIN / 32, W_MMA = W_CONV + CONV / 32, W_ROWS = W_MMA + 1, W_COPY = W_ROWS + 1;  // the other warps; the last is the gate's
-// registers of the main, converting and other warps; 16 x 80 + 8 x 56 + 4 x 72 = 28 x 72 a lane
-constexpr int REG_MAIN = 80, REG_CONV = 56;  // the rest keep the 72 of the launch
+// registers of the main, converting and other warps; 16 x 88 + 8 x 56 + 4 x 40 = 28 x 72 a lane
+constexpr int REG_MAIN = 88, REG_CONV = 56, REG_REST = 40;
 constexpr uint32_t MAT = SQ * 2;
 // the rows of a unit: q, k as two halves of 64 columns with 128-byte swizzle
 constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;
@@ -144,6 +144,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
     bool ok = true;
     if (warp < W_CONV) registers_up<REG_MAIN>();  // (one instruction for the four warps of a group)
     else if (warp < W_MMA) registers_down<REG_CONV>();
+    else registers_down<REG_REST>();
 
     if (warp < MAIN / 32) {
         const int rb = warp & 3, ib = warp >> 2, g = lane >> 2, t = lane & 3, d = tid & 127, t0 = 16 * ib;
@@ -184,16 +185,16 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             // ---- everything out of the accumulators
             float fq[16], fk[16], hh[16], dA[2][4], dL[2][4];
             {
-                float e1[16];
-                tmem_row16(tm + T_F + t0, fq);
                 tmem_row16(tm + T_E + t0, fk);
-                tmem_row16(tm + T_E + 64 + t0, e1);
+                tmem_row16(tm + T_E + 64 + t0, hh);
+                tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) fk[j] += hh[j];
+                tmem_row16(tm + T_F + t0, fq);
                 tmem_row16(tm + T_H + t0, hh);
                 tmem_frag2(tm + T_DA + t0, dA);
                 tmem_frag2(tm + T_DL + t0, dL);
                 tmem_wait_ld();
-#pragma unroll
-                for (int j = 0; j < 16; ++j) fk[j] += e1[j];
             }
             tc_fence_before();
             __syncwarp();
@@ -270,36 +271,36 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 const int at = swz_bf16(t0 + j, d);
                 qk_d[j] = reinterpret_cast<const uint16_t*>(sq)[at] | (uint32_t)reinterpret_cast<const uint16_t*>(sk)[at] << 16;
             }
-            {
-                float s[16];
+            {   // one sum after the other: what is live is F, E, H, the rows and one sum's terms
+                float s[16], *to = dots + rb * C + t0 + (lane >> 1);
+                auto scaled = [&](float (&x)[16], int factor) {
+#pragma unroll
+                    for (int j = 0; j < 16; j += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(aux + factor * C + t0 + j);
+                        x[j] *= f.x; x[j + 1] *= f.y; x[j + 2] *= f.z; x[j + 3] *= f.w;
+                    }
+                };
+                auto total = [&](int which) {
+                    lanes_total(s, lane);
+                    if (!(lane & 1)) to[which * 4 * C] = s[0];
+                };
+                scaled(fq, A_OQ);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[j] = fq[j] * __uint_as_float(qk_d[j] << 16);
+                total(0);
+                scaled(fk, A_GK);  // k.E
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[j] = fk[j] * __uint_as_float(qk_d[j] & 0xffff0000u);
+                total(1);
+                scaled(hh, A_FK);  // k.H
+#pragma unroll
+                for (int j = 0; j < 16; ++j) s[j] = hh[j] * __uint_as_float(qk_d[j] & 0xffff0000u);
+                total(2);
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const float4 oq = *reinterpret_cast<const float4*>(aux + A_OQ * C + t0 + j), gk = *reinterpret_cast<const float4*>(aux + A_GK * C + t0 + j),
-                                 fl = *reinterpret_cast<const float4*>(aux + A_FK * C + t0 + j), bb = *reinterpret_cast<const float4*>(be + t0 + j);
-                    const float *o = &oq.x, *e = &gk.x, *f = &fl.x, *b4 = &bb.x;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        fq[j + x] *= o[x];
-                        s[j + x] = fk[j + x] * e[x];  // k.E
-                        hh[j + x] *= f[x];            // k.H
-                        fk[j + x] = hh[j + x] - b4[x] * s[j + x];
-                        const float k = __uint_as_float(qk_d[j + x] & 0xffff0000u);
-                        s[j + x] *= k;
-                        hh[j + x] *= k;
-                    }
-                }
-                lanes_total(s, lane);
-                lanes_total(hh, lane);
-#pragma unroll
-                for (int j = 15; j > 0; --j) hh[j] = fq[j] * __uint_as_float(qk_d[j] << 16);
-                const float kh = hh[0];
-                hh[0] = fq[0] * __uint_as_float(qk_d[0] << 16);
-                lanes_total(hh, lane);
-                if (!(lane & 1)) {
-                    float* to = dots + rb * C + t0 + (lane >> 1);
-                    to[0] = hh[0];
-                    to[4 * C] = s[0];
-                    to[8 * C] = kh;
+                    const float4 f = *reinterpret_cast<const float4*>(be + t0 + j);
+                    fk[j] = hh[j] - f.x * fk[j]; fk[j + 1] = hh[j + 1] - f.y * fk[j + 1];
+                    fk[j + 2] = hh[j + 2] - f.z * fk[j + 2]; fk[j + 3] = hh[j + 3] - f.w * fk[j + 3];
                 }
             }
             __syncwarp();
