@@ -429,43 +429,74 @@ __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, con
 
 // dq and dk of shared key heads: the shares of a group's value heads in their order, then the gradient of the L2 norm.  A warp per
 // (row, key head).
+// two or four consecutive values
+template <int N>
+__device__ __forceinline__ void load_row(const float* p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 v = load2(p + i);
+        x[i] = v.x; x[i + 1] = v.y;
+    }
+}
+template <>
+__device__ __forceinline__ void load_row<4>(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
+}
+template <int N>
+__device__ __forceinline__ void load_row(const bf16* p, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        const float2 v = load2(p + i);
+        x[i] = v.x; x[i + 1] = v.y;
+    }
+}
 template <typename T, int K>
 __global__ void __launch_bounds__(256) gdr_heads_kernel(const KdaGdrParams p, const Layout lay) {
-    constexpr int N = K / 32;
+    constexpr int N = K / 32, R = 4;
     const int lane = threadIdx.x & 31, grp = p.HV / p.H;
-    const int c = blockIdx.x / p.H, kh = blockIdx.x % p.H;
+    const int b = gridDim.x - 1 - blockIdx.x, c = b / p.H, kh = b % p.H;  // what was written last is still in L2
     pdl_wait();
     const ChunkInfo ci = chunk_info(p, c);
     const float* aux = reinterpret_cast<const float*>(static_cast<const char*>(p.workspace) + lay.aux) + ((size_t)c * p.HV + kh * grp) * AUX;
     const float* in = reinterpret_cast<const float*>(static_cast<const char*>(p.bwd_scratch) + lay.dqk) + ((size_t)c * p.HV + kh * grp) * 2 * C * K;
-    for (int x = threadIdx.x >> 5; x < 2 * ci.len; x += 8) {
-        const int r = x >> 1, which = x & 1;  // q, k
-        float s[N];
+    // a warp has R rows at a time, q's and k's in turn, all of their loads on the way before the first is used
+    for (int x0 = (threadIdx.x >> 5) * R; x0 < 2 * ci.len; x0 += 8 * R) {
+        float s[R][N], xv[R][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = 0.f;
-        for (int hg = 0; hg < grp; ++hg)
+        for (int y = 0; y < R; ++y) {
+            const int x = min(x0 + y, 2 * ci.len - 1), r = x >> 1, which = x & 1;
+            load_row(in + (size_t)which * C * K + r * K + N * lane, s[y]);
+            load_row(static_cast<const T*>(which ? p.k : p.q) + (((size_t)ci.tok0 + r) * p.H + kh) * K + N * lane, xv[y]);
+        }
+        for (int hg = 1; hg < grp; ++hg) {
+            float v[R][N];
 #pragma unroll
-            for (int i = 0; i < N; i += 2) {
-                const float2 v = load2(in + ((size_t)hg * 2 + which) * C * K + r * K + N * lane + i);
-                s[i] += v.x; s[i + 1] += v.y;
+            for (int y = 0; y < R; ++y) {
+                const int x = min(x0 + y, 2 * ci.len - 1);
+                load_row(in + ((size_t)hg * 2 + (x & 1)) * C * K + (x >> 1) * K + N * lane, v[y]);
             }
-        const size_t at = (((size_t)ci.tok0 + r) * p.H + kh) * K + N * lane;
-        const T* row = static_cast<const T*>(which ? p.k : p.q) + at;
-        T* out = static_cast<T*>(which ? p.grad_k : p.grad_q) + at;
-        float xv[N], dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float2 v = load2(row + i);
-            xv[i] = v.x; xv[i + 1] = v.y;
-            dot += v.x * s[i] + v.y * s[i + 1];
-        }
-        float f = 0.f;
-        if (p.flags & KDA_FLAG_QK_L2NORM) {
-            const float inv = aux[(which ? A_RK : A_RQ) * C + r];
-            f = inv < 1e6f ? inv * inv * warp_sum(dot) : 0.f;
+            for (int y = 0; y < R; ++y)
+#pragma unroll
+                for (int i = 0; i < N; ++i) s[y][i] += v[y][i];
         }
 #pragma unroll
-        for (int i = 0; i < N; i += 2) store2(out + i, s[i] - xv[i] * f, s[i + 1] - xv[i + 1] * f);
+        for (int y = 0; y < R; ++y) {
+            const int x = x0 + y, r = x >> 1, which = x & 1;
+            if (x >= 2 * ci.len) break;
+            float f = 0.f;
+            if (p.flags & KDA_FLAG_QK_L2NORM) {
+                float dot = 0.f;
+#pragma unroll
+                for (int i = 0; i < N; ++i) dot = fmaf(xv[y][i], s[y][i], dot);
+                const float inv = aux[(which ? A_RK : A_RQ) * C + r];
+                f = inv < 1e6f ? inv * inv * warp_sum(dot) : 0.f;
+            }
+            T* out = static_cast<T*>(which ? p.grad_k : p.grad_q) + (((size_t)ci.tok0 + r) * p.H + kh) * K + N * lane;
+#pragma unroll
+            for (int i = 0; i < N; i += 2) store2(out + i, s[y][i] - xv[y][i] * f, s[y][i + 1] - xv[y][i + 1] * f);
+        }
     }
 }
 
