@@ -159,7 +159,7 @@ __device__ __forceinline__ void split(float x0, float x1, uint32_t (&w)[P]) {
         const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
         w[i] = *reinterpret_cast<const uint32_t*>(&h);
         if (i + 1 < P) {  // (packed: x - p)
-const float2 r = __ffma2_rn(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), make_float2(-1.f, -1.f), make_float2(x0, x1));
+            const float2 r = __ffma2_rn(make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u)), make_float2(-1.f, -1.f), make_float2(x0, x1));
             x0 = r.x;
             x1 = r.y;
         }

@@ -6,15 +6,16 @@
 // with the key channels as the 128 lanes, so that products with the states run at M = 128.  What L2 norm's gradient needs of q . dq and
 // k . dk comes from the same sums as dG: q . F, k . E, k . H, and rows and columns of Z (q k^T) and X (k k^T).
 //
-// One CTA per SM walks the (chunk, value head) units.  A warp copies the records' K-steps into shared memory, eight warps take <S0, dS>
-// and leave three BF16 parts in a ring of two K-steps; one issues the products; one brings the next unit's rows; sixteen do the rest
-// of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  16 x 2048 tokens of 6 heads take 365 us (732 on mma.sync):
-// 375 KB of records, rows and gradients per unit, 3.1 TB/s, half of the copy's rate.  What bounds it is shared memory's pipe: the copy
-// of the records in, their conversion (read once, written in 1.5 times the bytes), the MMAs' operands and the exchange of rows and
-// columns; twice the warps for either part gained nothing.  An MMA whose A operand lies in shared memory takes N / 2 + 43 cycles here
-// (M = 128; M = 64: N / 2 + 27), so do and the parts of Y lie side by side and go through as one operand of up to 192 columns.  Loads
-// from tensor memory wait for the MMAs issued before them, so a unit's accumulators are read at once, before the next unit's first
-// K-step, and the last products of a unit slip in between two K-steps of the next.
+// One CTA per SM walks the (chunk, value head) units.  Eight warps read the records, take <S0, dS> and leave three BF16 parts in a ring
+// of two K-steps (a warp asks L2 for the next unit's meanwhile); one issues the products; one brings the next unit's rows; sixteen do
+// the rest of a unit while the next unit's accumulators fill; one the gradients of gate and beta.  16 x 2048 tokens of 6 heads take
+// 350 us (732 on mma.sync): 375 KB of records, rows and gradients per unit, 3.3 TB/s, half of the copy's rate.  What bounds it is the
+// pipe of shared memory and L1: the records in, their parts out (1.5 times the bytes), the MMAs' operands, the exchange of rows and
+// columns and the main warps' spills; twice the warps for either part gained nothing, 88 registers instead of 80 for the main ones 5 %.
+// An MMA whose A operand lies in shared memory takes N / 2 + 43 cycles here (M = 128; M = 64: N / 2 + 27), so do and the parts of Y lie
+// side by side and go through as one operand of up to 192 columns.  Loads from tensor memory wait for the MMAs issued before them, so a
+// unit's accumulators are read at once, before the next unit's first K-step, and the last products of a unit slip in between two
+// K-steps of the next.
 // Records of two BF16 parts take the same bytes and no conversion, but dg is a difference of larger sums: 2e-5 off for 15 tokens.
 #include "gdr.cuh"
 

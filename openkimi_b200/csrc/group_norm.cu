@@ -12,7 +12,7 @@
 //     second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which give dw, db and, weighted with w,
 //     m1 and m2; then dx.  The second pass reads from L2 what fits there.
 // Bound by issue slots (70 % of them used in the first form) and by the latency of small slices: [32768, 768] in groups of 128, BF16
-// with SiLU, takes 29 us forward (3.5 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups 47 and 64 (3.2 and 4.3 TB/s of
+// with SiLU, takes 26 us forward (3.8 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups 47 and 64 (3.2 and 4.3 TB/s of
 // what its passes read and write).  In the first form the two took 172 and 291 us; what made them faster is two values an instruction, a
 // thread's channels all of one group, rows kept as they lie in memory until they are used, and a grid of what is resident.
 // Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
@@ -212,27 +212,24 @@ __global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? (BWD ? 3 : 4) : NV * VEC
             b[j][i] = in && a.b ? a.b[c0 + c] : 0.f;
             dw[j][i] = db[j][i] = 0.f;
         }
-    const long long turns = (a.N + step - 1) / step;
     Raw<T, VEC> nx[NV], ndy[NV];                   // the next row
-    auto request = [&](long long k) {
-        const long long n = slot / a.G + k * step;
-        const bool on = !idle && n < a.N;
-        const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
+    const long long row0 = slot / a.G, turns = (a.N + step - 1) / step, rows = idle || row0 >= a.N ? 0 : (a.N - row0 + step - 1) / step;
+    const size_t first = (size_t)(rows ? row0 : 0) * a.Ch + c0 + lane * VEC, ahead = (size_t)step * a.Ch;
+    const int own = Cg - lane * VEC;               // channels of the group from this lane's first on
+    auto request = [&](size_t at, bool on) {
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-            const int c = (j * L + lane) * VEC;
             nx[j] = ndy[j] = Raw<T, VEC>{};
-            if (on && c < Cg) {
-                nx[j] = load_raw<T, VEC>(X + base + c);
-                if (BWD) ndy[j] = load_raw<T, VEC>(static_cast<const T*>(a.dy) + base + c);
+            if (on && j * L * VEC < own) {
+                nx[j] = load_raw<T, VEC>(X + at + j * L * VEC);
+                if (BWD) ndy[j] = load_raw<T, VEC>(static_cast<const T*>(a.dy) + at + j * L * VEC);
             }
         }
     };
-    request(0);
-    for (long long k = 0; k < turns; ++k) {
-        const long long n = slot / a.G + k * step;
-        const bool on = !idle && n < a.N;
-        const size_t base = (size_t)(on ? n : 0) * a.Ch + c0;
+    request(first, rows > 0);
+    size_t at = first;
+    for (long long k = 0; k < turns; ++k, at += ahead) {
+        const bool on = k < rows;
         float x[NV][VEC], dy[NV][VEC];
         float2 s = make_float2(0.f, 0.f), q = s;
 #pragma unroll
@@ -241,23 +238,22 @@ __global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? (BWD ? 3 : 4) : NV * VEC
             if (BWD) unpack(ndy[j], dy[j]);
             s = sum2(s, x[j]);
         }
-        if (k + 1 < turns) request(k + 1);
+        request(at + ahead, k + 1 < rows);
         const float mean = lanes_sum(s.x + s.y, L) * inv;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             vadd(x[j], x[j], Same{-mean});
-            if ((j * L + lane) * VEC < Cg) q = dot2(q, x[j], x[j]);
+            if (j * L * VEC < own) q = dot2(q, x[j], x[j]);
         }
         const float var = lanes_sum(q.x + q.y, L) * inv, rstd = on ? inv_sqrt<T>(var + a.eps) : 0.f;  // (no row: no infinity into dw, db)
         if (!BWD) {
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = (j * L + lane) * VEC;
                 float y[VEC];
                 vmul(x[j], x[j], Same{rstd});
                 vfma(x[j], x[j], w[j], b[j]);
                 act<T>(y, x[j], silu);
-                if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.y) + base + c, y);
+                if (on && j * L * VEC < own) store<T, VEC>(static_cast<T*>(a.y) + at + j * L * VEC, y);
             }
         } else {
             float2 t1 = make_float2(0.f, 0.f), t2 = t1;
@@ -276,12 +272,11 @@ __global__ void __launch_bounds__(NTHR, NV * VEC <= 8 ? (BWD ? 3 : 4) : NV * VEC
             const float m1 = -lanes_sum(t1.x + t1.y, L) * inv, m2 = -lanes_sum(t2.x + t2.y, L) * inv;
 #pragma unroll
             for (int j = 0; j < NV; ++j) {
-                const int c = (j * L + lane) * VEC;
                 float dx[VEC];
                 vadd(dx, dy[j], Same{m1});  // (before rstd: a group of one channel has exactly 0)
                 vfma(dx, x[j], Same{m2}, dx);
                 vmul(dx, dx, Same{rstd});
-                if (on && c < Cg) store<T, VEC>(static_cast<T*>(a.dx) + base + c, dx);
+                if (on && j * L * VEC < own) store<T, VEC>(static_cast<T*>(a.dx) + at + j * L * VEC, dx);
             }
         }
     }
