@@ -4,7 +4,7 @@
 // rows as they arrive, and decay, beta and the rows' 1 / norm multiply the results in FP32.  So in BF16 mode every product has
 // an operand that BF16 holds exactly (q, k, do) or two computed ones (T, V', S, ...).  Computed operands are BF16 in up to three
 // parts, x = p0 + p1 + p2 to 2^-24, and a product of parts i and j is taken where i + j < 3: FP32-class results (measured against
-// 64 bits: 2e-7 to 1e-6) from tensor cores with FP32 accumulators.  Where only a BF16 output can see the difference two parts do
+// 64 bits: 1e-7 to 3e-7 on mma.sync, 2e-7 to 1.7e-6 on tcgen05, whose accumulators truncate) from tensor cores with FP32 accumulators.  Where only a BF16 output can see the difference two parts do
 // (2^-17).  FP32 tensors go the same way with three parts for q, k, v, do as well.
 #pragma once
 
@@ -139,17 +139,30 @@ __device__ __forceinline__ void tri_frag_t(uint32_t (&f)[4], uint32_t x, int b, 
     ldsm_t(f, x + 2 * (b * BLK + tri_idx((lane & 7) + (lane >> 4) * 8, ((lane >> 3) & 1) * 8)));
 }
 
-// products of the parts of one A block and two column tiles of B
+// Products of the parts of one A block and two column tiles of B.  The tensor core truncates at every accumulation: several products
+// are summed from zero, the smallest first, and added in FP32, so that one truncation of a K-step's own size is left of each
+// (FP32 tensors: dk 1.8e-6 -> 1.8e-7 of its norm from 64 bits).
 template <int PA, int PB, int ORD, int NT>
 __device__ __forceinline__ void mma_parts(float (&acc)[NT][4], int pair, const uint32_t (&a)[PA][4], const uint32_t (&b)[PB][4]) {
+    if constexpr (PA * PB == 1) {
+        mma(acc[2 * pair], a[0], b[0][0], b[0][1]);
+        mma(acc[2 * pair + 1], a[0], b[0][2], b[0][3]);
+    } else {
+        float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
-    for (int j = PB - 1; j >= 0; --j)
+        for (int o = ORD - 1; o >= 0; --o)
 #pragma unroll
-        for (int i = PA - 1; i >= 0; --i)
-            if (i + j < ORD) {
-                mma(acc[2 * pair], a[i], b[j][0], b[j][1]);
-                mma(acc[2 * pair + 1], a[i], b[j][2], b[j][3]);
-            }
+            for (int j = PB - 1; j >= 0; --j)
+                if (o - j >= 0 && o - j < PA) {
+                    mma(s[0], a[o - j], b[j][0], b[j][1]);
+                    mma(s[1], a[o - j], b[j][2], b[j][3]);
+                }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            acc[2 * pair][i] += s[0][i];
+            acc[2 * pair + 1][i] += s[1][i];
+        }
+    }
 }
 
 template <int P>

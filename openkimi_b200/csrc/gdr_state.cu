@@ -8,8 +8,8 @@
 // of a chunk gets shorter with VP and there are dv / VP times as many CTAs.  The panel of the state stays in registers, in the
 // accumulators of its update (warp w: key channels w dk/4 ..), and goes to shared memory in three BF16 parts as the operand of the
 // next chunk.  The next chunk's q, k, T, A (and do) are requested as soon as their other copy is free.
-// Bound by the chain of a chunk: 6.2 us forward and 9.3 backward in FP32 (8 chunks of 64 key channels, 64 CTAs of 16 columns: 50 and
-// 75 us).  BF16 with 128 channels and columns goes on tcgen05 (gdr_tc.cu).
+// Bound by the chain of a chunk: 6.3 us forward and 7.6 backward in FP32 (8 chunks of 64 key channels, 64 CTAs of 16 columns: 51 and
+// 61 us).  BF16 with 128 channels and columns goes on tcgen05 (gdr_tc.cu).
 #include "gdr.cuh"
 
 namespace kda {
