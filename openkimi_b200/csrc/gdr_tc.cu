@@ -240,12 +240,16 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
                     f[j] *= x[g][j];
                 }
                 st_parts<3>(tm + M::R + half * 16 + 8 * g, 32, f);
-                if (OUT) st_parts<2>(tm + M::VA + half * 32 + 8 * g, 16, x[g]);
             }
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&wready);
+            if (OUT) {  // for V' A^T, which waits for siread
+#pragma unroll
+                for (int g = 0; g < 2; ++g) st_parts<2>(tm + M::VA + half * 32 + 8 * g, 16, x[g]);
+                tmem_wait_st();
+            }
             if (SAVE) {
                 float* V = reinterpret_cast<float*>(static_cast<char*>(p.workspace) + lay.Vn) + unit * C * 128;
 #pragma unroll
