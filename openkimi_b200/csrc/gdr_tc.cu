@@ -9,8 +9,8 @@
 // added to the decayed state in FP32.
 // Bound by the chain of a chunk: split S - S k - R - R T - V' - W k - S.  Everything else is off it: two producer warps bring the next
 // chunk's rows (core-matrix order) and records, one warp issues all products, four warps turn finished outputs into rows.  A chunk of
-// 64 tokens takes 4.5 us with few CTAs, 5.9 forward and 6.5 backward with 96 that save their records (16 x 2048 tokens of 6 heads: 189
-// and 208 us, 3 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.
+// 64 tokens takes 4.5 us with few CTAs, 5.8 forward and 6.5 backward with 96 that save their records (16 x 2048 tokens of 6 heads: 185
+// and 207 us, 3 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.
 #include "gdr.cuh"
 
 namespace kda {
