@@ -13,7 +13,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .ops import _chunk_tables
+from .ops import _cached_tables, _chunk_tables
 
 
 def _flags(l2norm, gate, sigmoid, v_first):
@@ -24,9 +24,6 @@ def _flags(l2norm, gate, sigmoid, v_first):
 @lru_cache(maxsize=64)
 def _offsets(cu: tuple, device_index: int):
     return torch.tensor(cu, dtype=torch.int64, device=torch.device("cuda", device_index))
-
-
-_in_graphs: dict = {}  # tables that captured graphs read: a graph outlives what the caches above keep
 
 
 @torch.compiler.disable
@@ -64,9 +61,7 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
         tokens = q.shape[0] * q.shape[1]
         seq, off, nt, tab, longest = _chunk_tables(None, host, q.device, tokens)
         cu = tuple(int(x) for x in host.tolist())
-        tables = (_offsets(cu, q.device.index or 0), seq, off, tab, nt, longest, cu[0] == 0 and cu[-1] == tokens)
-        if torch.cuda.is_current_stream_capturing():
-            _in_graphs.setdefault((cu, q.device.index or 0), tables)
+        tables = (_cached_tables(_offsets, cu, q.device), seq, off, tab, nt, longest, cu[0] == 0 and cu[-1] == tokens)
     return _lib.host().chunk_gdr(q, k, v, g, beta, A_log, dt_bias, initial_state, scale,
                                  _flags(use_qk_l2norm_in_kernel, use_gate_in_kernel, use_beta_sigmoid_in_kernel, state_v_first),
                                  bool(output_final_state), *tables)

@@ -38,6 +38,24 @@ def _chunk_tables_cached(cu: tuple, device_index: int):
             torch.tensor(tab if tab else [(0, 0, 0, 0)], dtype=torch.int32, device=dev), max(counts, default=0))
 
 
+_in_graphs: dict = {}  # (builder, offsets, device) -> tables whose addresses captured graphs hold
+
+
+def _cached_tables(build, cu, device):
+    """``build(cu, device index)`` from its cache, which drops what was used longest ago.  A captured graph reads its tables by their
+    addresses, and nothing says when it is gone: the tables of a call that is captured are kept for good, and are those of every later
+    call with the same offsets, captured or not."""
+    key = (build, cu, device.index or 0)
+    tables = _in_graphs.get(key)
+    if tables is None:
+        tables = build(cu, key[2])
+        with torch.cuda.device(device):
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
+            tables = _in_graphs.setdefault(key, tables)
+    return tables
+
+
 def _chunk_tables(cu_seqlens, cu_seqlens_cpu, device, tokens):
     """Per-chunk sequence index and per-sequence first chunk.  Chunks never straddle a
     document boundary, so the table depends on the lengths; it is built on the host
@@ -46,7 +64,7 @@ def _chunk_tables(cu_seqlens, cu_seqlens_cpu, device, tokens):
     cu = tuple(int(x) for x in host.tolist())
     if cu and (cu[0] < 0 or cu[-1] > tokens):
         raise ValueError(f"cu_seqlens must stay within the {tokens} tokens of the batch, got {cu[0]} to {cu[-1]}")
-    return _chunk_tables_cached(cu, device.index or 0)
+    return _cached_tables(_chunk_tables_cached, cu, device)
 
 
 def _packed_tables(cu_seqlens, cu_seqlens_cpu, x):
