@@ -295,7 +295,7 @@ void take_tables(Inputs& tables, const OptTensor& cu, const OptTensor& chunk_seq
     if (batch != 1)
         value_error("The batch size is expected to be 1 rather than " + std::to_string(batch) +
                     " when using `cu_seqlens`.Please flatten variable-length inputs before processing.");
-    tables.cu = *cu; tables.chunk_seq = *chunk_seq; tables.seq_off = *seq_off; tables.chunk_tab = *chunk_tab;
+    tables.cu = *cu; tables.chunk_seq = read_here(*chunk_seq); tables.seq_off = read_here(*seq_off); tables.chunk_tab = read_here(*chunk_tab);
 }
 
 std::tuple<Tensor, OptTensor> chunk_kda(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,

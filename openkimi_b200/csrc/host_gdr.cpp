@@ -232,7 +232,7 @@ std::tuple<Tensor, OptTensor> chunk_gdr(const Tensor& q, const Tensor& k, const 
     sp.NT = B * ((T + CHUNK - 1) / CHUNK);
     if (cu) {
         if (B != 1) value_error("The batch size is expected to be 1 rather than " + std::to_string(B) + " when using `cu_seqlens`.");
-        tables.cu = *cu; tables.chunk_seq = *chunk_seq; tables.seq_off = *seq_off; tables.chunk_tab = *chunk_tab;
+        tables.cu = read_here(*cu); tables.chunk_seq = read_here(*chunk_seq); tables.seq_off = read_here(*seq_off); tables.chunk_tab = read_here(*chunk_tab);
         sp.N = cu->numel() - 1;
         sp.NT = NT;
         sp.longest = longest;

@@ -4,6 +4,7 @@
 #include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/extension.h>
@@ -143,6 +144,12 @@ template <class T>
 T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
 inline void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+
+// A cached table belongs to the stream that made it: the current one reads it too, so that its memory waits for both when the cache drops it.
+inline const Tensor& read_here(const Tensor& t) {
+    c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), at::cuda::getCurrentCUDAStream(t.device().index()));
+    return t;
+}
 
 inline Tensor bytes(size_t n, const Tensor& like) { return fresh({(int64_t)n}, at::kByte, like); }
 inline Tensor fresh_like(const Tensor& t) { return fresh(t.sizes(), t.scalar_type(), t); }
