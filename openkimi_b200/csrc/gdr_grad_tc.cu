@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             mbar_init(&tfull[i], 1);
-            mbar_init(&tempty[i], 2 + MAIN / 32);
+            mbar_init(&tempty[i], 3 + MAIN / 32);  // the last products, the gate's warp, the one that asks L2, the main ones
         }
         mbar_init(&accbar, 1 + CONV / 32);
         mbar_init(&accfree, MAIN / 32);
@@ -523,10 +523,12 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             __syncwarp();
             if (lane == 0) mbar_arrive(&tfull[tb]);
         }
-    } else if (warp == W_COPY) {  // (nothing waits for it: hints only, a unit ahead of the converters)
+    } else if (warp == W_COPY) {  // hints only, a unit ahead of the converters; counted in tempty, or it might miss a phase of tfull
         if (lane == 0)
-            for (int u = blockIdx.x, it = 0; u + stride < units && ok; u += stride, ++it) {
+            for (int u = blockIdx.x, it = 0; u + stride < units; u += stride, ++it) {
                 ok = mbar_wait(&tfull[it & 1], (it >> 1) & 1, p, 1 << 9);
+                if (!ok) break;
+                mbar_arrive(&tempty[it & 1]);
                 const size_t n = (size_t)u + stride;
                 l2_prefetch_bulk(ws + lay.S0 + n * K * 512, K * 512);
                 l2_prefetch_bulk(sc + lay.dS + n * K * 512, K * 512);
