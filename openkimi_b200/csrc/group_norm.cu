@@ -7,15 +7,15 @@
 //   * S = 1 (every token by itself, groups of up to 1024 channels): L lanes hold a group of one row in registers, so that one pass
 //     does it all, the next row on its way meanwhile; the lanes keep their group over the rows they walk and with it w, b and their
 //     shares of dw, db.
-//   * else: a thread keeps VEC channels and walks rows of a slice of a sample.  Forward: sums of x and x^2 about the slice's first
-//     row, joined over the slice's channels to (mean, sum of squared deviations) of a group, and over the slices at the start of the
-//     second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which give dw, db and, weighted with w,
-//     m1 and m2; then dx.  The second pass reads from L2 what fits there.
+//   * else: a thread keeps VEC channels and walks rows of a slice of a sample.  Forward: sums of x and x^2 about a row of its own, then
+//     about the mean of its first rows, joined over the slice's channels to (mean, sum of squared deviations) of a group, and over
+//     the slices at the start of the second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which
+//     give dw, db and, weighted with w, m1 and m2; then dx.  The second pass reads from L2 what fits there.
 // Bound by issue slots (70 % of them used in the first form) and by the latency of small slices: [32768, 768] in groups of 128, BF16
 // with SiLU, takes 26 us forward (3.8 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups 47 and 64 (3.2 and 4.3 TB/s of
 // what its passes read and write).  In the first form the two took 172 and 291 us; what made them faster is two values an instruction, a
 // thread's channels all of one group, rows kept as they lie in memory until they are used, and a grid of what is resident.
-// Sums are in FP32 over at most a few thousand values, then in 64 bits in a fixed order: no atomics.
+// Sums are in FP32 over at most 1024 rows, then in 64 bits in a fixed order: no atomics.
 #include "kda_common.cuh"
 
 namespace kda {
@@ -25,7 +25,8 @@ using bf16 = __nv_bfloat16;
 constexpr int NTHR = 256;
 constexpr int SLICE_THR = 384;    // at most, in the kernels over slices
 constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
-constexpr int MAX_SLICES = 256;
+constexpr int MAX_SLICES = 256;   // of a sample in the second pass
+constexpr int SUM_ROWS = 1024;    // that one FP32 sum adds up
 constexpr int GROUPS_MAX = 24576; // groups whose numbers fit shared memory where they are not taken row by row
 
 struct Args {
@@ -35,9 +36,11 @@ struct Args {
     float *mean, *rstd;           // [N, G]
     float *dw, *db;               // [Ch], may be NULL
     float* part;                  // scratch
-    long long N, S, len;          // len: rows of a slice
-    int Ch, G, act, slices;
+    long long N, S;
+    long long len, span;          // rows of a slice of the first pass, of the second
+    int Ch, G, act, slices, cuts; // slices of a sample in either
     float eps;
+    double inv_S, inv_Cg;         // 1 / S, 1 / (Ch / G)
 };
 
 // VEC elements as they lie in memory: 16 bytes, two elements or one
@@ -185,6 +188,22 @@ __device__ __forceinline__ float lanes_sum(float v, int L) {
         if (o < L) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+// three sums at once
+__device__ __forceinline__ void lanes_sum(double& a, double& b, double& c, int L) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+        if (o < L) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            b += __shfl_xor_sync(0xffffffffu, b, o);
+            c += __shfl_xor_sync(0xffffffffu, c, o);
+        }
+}
+// Sums u of w d and q of w d^2, d differences from some number: the sum of w (d - mean)^2, w adding up to 1 / inv.  (In 64 bits the
+// difference loses nothing that FP32 d have; rounding leaves it no less than 0, and a NaN stays one.)
+__device__ __forceinline__ double deviations(double u, double q, double inv) {
+    const double d = q - u * u * inv;
+    return d < 0.0 ? 0.0 : d;
+}
 template <typename T>
 __device__ __forceinline__ float inv_sqrt(float v) { return sizeof(T) == 4 ? 1.f / sqrtf(v) : rsqrtf(v); }
 
@@ -318,12 +337,12 @@ __global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* pa
 // CTAs per SM that registers allow without spilling
 __host__ __device__ constexpr int slice_ctas(bool bwd) { return bwd ? 2 : 3; }
 struct Slice {
-    long long n, s0, s1;
-    __device__ __forceinline__ Slice(const Args& a) {
-        n = blockIdx.x / a.slices;
-        const long long i = blockIdx.x % a.slices;
-        s0 = i * a.len;
-        s1 = min(a.S, s0 + a.len);
+    long long n, i, s0, s1;
+    __device__ __forceinline__ Slice(long long S, int slices, long long len) {
+        n = blockIdx.x / slices;
+        i = blockIdx.x % slices;
+        s0 = i * len;
+        s1 = min(S, s0 + len);
     }
 };
 // A thread's rows of a slice, every TR-th, VEC channels each: f(row, x, dy).  The next U rows are on their way while U are used (a load
@@ -367,18 +386,34 @@ struct Rows {
 // rows in flight, what registers allow: [4, 8191, 768] BF16 in 32 groups, sums of the backward 29 us with one and 37 with two; its second
 // pass 31 with two and 33 with one
 template <int VEC> constexpr int rows_ahead(bool two) { return VEC <= 2 ? 4 : VEC == 4 || !two ? 2 : 1; }
-// scratch: [N * slices][2][Ch] sums of the channels, then [N][G][slices][2] numbers of the groups
+// scratch: [N * slices][2][Ch] numbers of the channels, then [N][G][slices][2] numbers of the groups
 __device__ __forceinline__ float* group_part(const Args& a) { return a.part + (size_t)a.N * a.slices * 2 * a.Ch; }
 
-// MODE 0: sums of x - x0 and (x - x0)^2 about the slice's first row x0, and from them a group's mean and sum of squared deviations;
-// 1: sums of dz x^ and dz, and over a group's channels w times those
+// Sums s1 of x - b and s2 of (x - b)^2 over k rows, p = -b, become those about the rows' mean: however far the first row lies from
+// the others, what follows is added about their middle.
+template <int VEC>
+__device__ __forceinline__ void about_mean(float (&p)[VEC], float (&s1)[VEC], float (&s2)[VEC], float k) {
+    const float inv = 1.f / k;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const float to = fmaf(-inv, s1[i], p[i]), e = p[i] - to;
+        s2[i] = fmaf(-e, fmaf(-k, e, 2.f * s1[i]), s2[i]);
+        s1[i] = fmaf(-k, e, s1[i]);
+        p[i] = to;
+    }
+}
+
+// MODE 0: per thread and channel the mean less the slice's first row x0 and the sum of squared deviations, joined over the threads, and
+// from them a group's; 1: sums of dz x^ and dz, and over a group's channels w times those
 template <typename T, int VEC, int MODE>
 __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_kernel(const Args a) {
     extern __shared__ float sm[];                  // [2][TR][TC * VEC]
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
-    const Slice sl(a);
+    const Slice sl(a.S, a.slices, a.len);
     const long long n = sl.n;
+    const int m = (int)(sl.s1 - sl.s0);            // (at most SUM_ROWS * SLICE_THR)
+    const double inv_m = 1.0 / m;
     pdl_wait();
     const T* X = static_cast<const T*>(a.x) + (size_t)n * a.S * a.Ch;
     const T* D = static_cast<const T*>(a.dy) + (size_t)n * a.S * a.Ch;
@@ -393,7 +428,7 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
         if (on) {
             Rows<T, VEC, MODE, rows_ahead<VEC>(MODE)> rows(X + c, D + c, sl, tr, TR, a.Ch);
             if (MODE == 0) {
-                load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, p);
+                load<T, VEC>(X + (size_t)(sl.s0 + (tr < m ? tr : 0)) * a.Ch + c, p);
                 vmul(p, p, Same{-1.f});
             } else {
                 mu = a.mean[n * a.G + c / Cg];
@@ -405,11 +440,13 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
                 w[i] = MODE && a.w ? a.w[c + i] : 1.f;
                 b[i] = MODE && a.b ? a.b[c + i] : 0.f;
             }
+            int k = 0;
             rows.each([&](long long, float (&x)[VEC], float (&dy)[VEC]) {
                 if (MODE == 0) {
                     vadd(x, x, p);
                     vadd(s1, s1, x);
                     vfma(s2, x, x, s2);
+                    if (++k >= 8 && (k & (k - 1)) == 0) about_mean(p, s1, s2, (float)k);
                 } else {
                     float z[VEC];
                     vadd(x, x, Same{-mu});
@@ -420,6 +457,16 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
                     vadd(s2, s2, dy);
                 }
             });
+            if (MODE == 0 && k > 0) {
+                about_mean(p, s1, s2, (float)k);
+                float x0[VEC];
+                load<T, VEC>(X + (size_t)sl.s0 * a.Ch + c, x0);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    s1[i] = fmaf(1.f / k, s1[i], -p[i] - x0[i]);
+                    s2[i] = s2[i] < 0.f ? 0.f : s2[i];  // (a NaN stays one)
+                }
+            }
         }
         if (v0) __syncthreads();
 #pragma unroll
@@ -429,42 +476,62 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(MODE)) group_norm_sums_k
                 sm[(TR + tr) * TC * VEC + tc * VEC + i] = s2[i];
             }
         __syncthreads();
-        for (int i = threadIdx.x; i < 2 * TC * VEC; i += blockDim.x) {
-            const int which = i / (TC * VEC), cc = i % (TC * VEC);
+        // over the TR threads of a channel: a thread does that, or a warp where they are many
+        const int L = TR > 32 ? 32 : 1, on_lane = threadIdx.x & (L - 1);
+        for (int cc = threadIdx.x / L; cc < TC * VEC; cc += blockDim.x / L) {
             if (v0 * VEC + cc >= a.Ch) continue;
-            float s = 0.f;
-            for (int r = 0; r < TR; ++r) s += sm[(which * TR + r) * TC * VEC + cc];
-            out[(size_t)which * a.Ch + v0 * VEC + cc] = s;
-            sm[which * TR * TC * VEC + cc] = s;
+            double u = 0.0, q = 0.0, v = 0.0;
+            for (int r = on_lane; r < TR; r += L) {
+                const double x = sm[r * TC * VEC + cc], y = sm[(TR + r) * TC * VEC + cc];
+                if (MODE == 0) {
+                    const double w = x * ((m - r + TR - 1) / TR);  // (r < m, or the thread has had no row)
+                    u += r < m ? w : 0.0;
+                    q += r < m ? w * x : 0.0;
+                } else {
+                    u += x;
+                }
+                v += y;
+            }
+            lanes_sum(u, q, v, L);
+            if (MODE == 0) {
+                v += deviations(u, q, inv_m);
+                u *= inv_m;
+            }
+            if (on_lane == 0) {
+                out[v0 * VEC + cc] = sm[cc] = (float)u;
+                out[(size_t)a.Ch + v0 * VEC + cc] = sm[TR * TC * VEC + cc] = (float)v;
+            }
         }
     }
     __syncthreads();
     // a row as wide as one block of channels is still in shared memory; else the CTA reads back what it wrote
     const float *sum1 = cols <= TC ? sm : out, *sum2 = cols <= TC ? sm + TR * TC * VEC : out + a.Ch;
-    float* groups = group_part(a) + ((size_t)n * a.G * a.slices + blockIdx.x % a.slices) * 2;
+    float* groups = group_part(a) + ((size_t)n * a.G * a.slices + sl.i) * 2;
     const int lane = threadIdx.x & 31;
-    const float m = (float)(sl.s1 - sl.s0);
     for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
-        float u = 0.f, v = 0.f;
-        if (MODE == 0) {
-            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) u += fmaf(m, ldf(X + (size_t)sl.s0 * a.Ch + c), sum1[c]);
-            u = warp_sum(u) / (m * Cg);
-            // sum (x - mean)^2 = sum (x - x0)^2 + 2 (x0 - mean) sum (x - x0) + m (x0 - mean)^2
-            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
-                const float d = ldf(X + (size_t)sl.s0 * a.Ch + c) - u;
-                v += fmaf(d, fmaf(m, d, 2.f * sum1[c]), sum2[c]);
+        double u = 0.0, q = 0.0, v = 0.0;
+        const float *s1 = sum1 + g * Cg, *s2 = sum2 + g * Cg;
+        if (MODE == 0) {  // about the first channel's mean
+            const T* x0 = X + (size_t)sl.s0 * a.Ch + g * Cg;
+            const double about = (double)ldf(x0) + s1[0];
+            for (int c = lane; c < Cg; c += 32) {
+                const double d = (double)ldf(x0 + c) + s1[c] - about;
+                u += d;
+                q += d * d;
+                v += s2[c];
             }
-            v = warp_sum(v);
+            lanes_sum(u, q, v, 32);
+            v += m * deviations(u, q, a.inv_Cg);
+            u = about + u * a.inv_Cg;
         } else {
-            for (int c = g * Cg + lane; c < (g + 1) * Cg; c += 32) {
-                const float w = a.w ? a.w[c] : 1.f;
-                v = fmaf(w, sum1[c], v);
-                u = fmaf(w, sum2[c], u);
+            for (int c = lane; c < Cg; c += 32) {
+                const double w = a.w ? a.w[g * Cg + c] : 1.f;
+                v += w * s1[c];
+                u += w * s2[c];
             }
-            u = warp_sum(u);
-            v = warp_sum(v);
+            lanes_sum(u, q, v, 32);
         }
-        if (lane == 0) *reinterpret_cast<float2*>(groups + (size_t)g * a.slices * 2) = make_float2(u, v);
+        if (lane == 0) *reinterpret_cast<float2*>(groups + (size_t)g * a.slices * 2) = make_float2((float)u, (float)v);
     }
 }
 
@@ -472,7 +539,7 @@ template <typename T, int VEC, bool BWD>
 __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_kernel(const Args a) {
     const int cols = a.Ch / VEC, TC = min(cols, SLICE_THR), TR = SLICE_THR / TC;
     const int tc = threadIdx.x % TC, tr = threadIdx.x / TC, Cg = a.Ch / a.G;
-    const Slice sl(a);
+    const Slice sl(a.S, a.cuts, a.span);
     const long long n = sl.n;
     extern __shared__ float stat[];                // [G][2]: mean, rstd; backward: m1, m2
     pdl_wait();
@@ -483,37 +550,31 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
     {   // the sample's slices, a warp per group; means about the first slice's
         const float2* groups = reinterpret_cast<const float2*>(group_part(a)) + (size_t)n * a.slices * a.G;  // [G][slices]
         const int lane = threadIdx.x & 31;
-        const float rows = (float)a.len, tail = (float)(a.S - (a.slices - 1) * a.len), count = (float)a.S * Cg;
+        const double rows = (double)a.len, tail = (double)(a.S - (long long)(a.slices - 1) * a.len), inv = a.inv_S * a.inv_Cg;
         for (int g = threadIdx.x >> 5; g < a.G; g += blockDim.x >> 5) {
-            float2 p[MAX_SLICES / 32];
             const float2* of = groups + (size_t)g * a.slices;
-            const float u0 = BWD ? 0.f : of[0].x;
-            float u = 0.f, v = 0.f;
-#pragma unroll
-            for (int j = 0; j < MAX_SLICES / 32; ++j)
-                if (j * 32 < a.slices) {
-                    const int i = j * 32 + lane;
-                    p[j] = i < a.slices ? of[i] : make_float2(u0, 0.f);
-                    p[j].x -= u0;
-                    u += BWD ? p[j].x : p[j].x * (i == a.slices - 1 ? tail : rows);
-                    v += p[j].y;
+            const double u0 = BWD ? 0.0 : of[0].x;
+            double u = 0.0, q = 0.0, v = 0.0;
+#pragma unroll 4
+            for (int i = lane; i < a.slices; i += 32) {
+                const float2 p = of[i];
+                if (BWD) {
+                    u += p.x;
+                } else {
+                    const double d = p.x - u0, w = d * (i == a.slices - 1 ? tail : rows);
+                    u += w;
+                    q += w * d;
                 }
-            u = warp_sum(u);
-            if (!BWD) {
-                u /= (float)a.S;
-#pragma unroll
-                for (int j = 0; j < MAX_SLICES / 32; ++j)
-                    if (j * 32 + lane < a.slices) {
-                        const float d = p[j].x - u;
-                        v = fmaf(d * d, (j * 32 + lane == a.slices - 1 ? tail : rows) * Cg, v);
-                    }
+                v += p.y;
             }
-            v = warp_sum(v);
-            const float s0 = BWD ? u / count : u0 + u, s1 = BWD ? v / count : 1.f / sqrtf(fmaxf(v, 0.f) / count + a.eps);
+            lanes_sum(u, q, v, 32);
+            if (!BWD) {
+                v += Cg * deviations(u, q, a.inv_S);
+                u = u0 + u * a.inv_S;
+            }
             if (lane == 0) {
-                // (fmaxf drops a NaN: one among the values is one in their mean)
-                stat[2 * g] = s0;
-                stat[2 * g + 1] = !BWD && s0 != s0 ? s0 : s1;
+                stat[2 * g] = (float)(BWD ? u * inv : u);
+                stat[2 * g + 1] = BWD ? (float)(v * inv) : 1.f / sqrtf((float)(v * inv) + a.eps);
                 if (!BWD && sl.s0 == 0) {
                     a.mean[n * a.G + g] = stat[2 * g];
                     a.rstd[n * a.G + g] = stat[2 * g + 1];
@@ -557,14 +618,21 @@ __global__ void __launch_bounds__(SLICE_THR, slice_ctas(BWD)) group_norm_apply_k
 // ---- launches -----------------------------------------------------------------------------------------------------------
 static bool by_rows(long long S, int Ch, int G) { return S == 1 && Ch / G <= ROWS_MAX; }
 
-// slices of a sample: as many as are resident over all samples, of at least 8 rows, all but the last of the same length
+// Slices of a sample in the second pass: as many as are resident over all samples, of at least 8 rows, all but the last of the same
+// length.  In the first pass the same ones, or shorter where a thread would add up more than SUM_ROWS rows (with one channel an access).
 static void cut(Args& a, bool bwd) {
+    a.inv_S = 1.0 / a.S;
+    a.inv_Cg = (double)a.G / a.Ch;
     long long want = (long long)slice_ctas(bwd) * sm_count() / a.N, most = (a.S + 7) / 8;
     if (want > most) want = most;
     if (want > MAX_SLICES) want = MAX_SLICES;
     if (want < 1) want = 1;
-    a.len = (a.S + want - 1) / want;
-    a.slices = (int)((a.S + a.len - 1) / a.len);
+    a.span = (a.S + want - 1) / want;
+    a.cuts = (int)((a.S + a.span - 1) / a.span);
+    const long long most_rows = (long long)SUM_ROWS * (SLICE_THR / (a.Ch < SLICE_THR ? a.Ch : SLICE_THR));
+    a.len = a.span < most_rows ? a.span : most_rows;
+    const long long slices = (a.S + a.len - 1) / a.len;
+    a.slices = slices < 0x7fffffffLL ? (int)slices : 0x7fffffff;  // (refused)
 }
 
 struct RowsGrid { int L; long long ctas, step; };
@@ -575,7 +643,8 @@ static RowsGrid rows_grid(long long N, int Ch, int G, int vec, bool bwd) {
     while (r.L < 32 && r.L * vec < Cg) r.L *= 2;
     const long long per = NTHR / r.L, need = (N * G + per - 1) / per;
     long long most = (bwd ? 3 : 4) * (long long)sm_count();
-    const long long least = (G + per - 1) / per;   // every group has a slot
+    const long long steps = bwd ? (N + SUM_ROWS - 1) / SUM_ROWS : 1;  // a slot adds at most SUM_ROWS rows to its dw, db
+    const long long least = (steps * G + per - 1) / per;              // and every group has a slot
     if (most < least) most = least;
     r.ctas = need < least ? least : need < most ? need : most;
     r.step = r.ctas * per / G;
@@ -604,12 +673,12 @@ static cudaError_t rows_launch(const Args& a, cudaStream_t s) {
 
 template <typename T, int VEC, bool BWD>
 static cudaError_t slices_launch(const Args& a, cudaStream_t s) {
-    const dim3 grid((unsigned)(a.N * a.slices));
+    const dim3 grid((unsigned)(a.N * a.slices)), grid2((unsigned)(a.N * a.cuts));
     const int cols = a.Ch / VEC, TC = cols < SLICE_THR ? cols : SLICE_THR, TR = SLICE_THR / TC, threads = (TC * TR + 31) / 32 * 32;
     const size_t smem = (size_t)2 * TR * TC * VEC * sizeof(float), stat = (size_t)2 * a.G * sizeof(float);
     cudaError_t e = stat > 48 * 1024 ? allow_smem(group_norm_apply_kernel<T, VEC, BWD>, GROUPS_MAX * 8) : cudaSuccess;
     if (e == cudaSuccess) e = launch_dependent(group_norm_sums_kernel<T, VEC, BWD ? 1 : 0>, grid, threads, smem, s, a);
-    if (e == cudaSuccess) e = launch_dependent(group_norm_apply_kernel<T, VEC, BWD>, grid, threads, stat, s, a);
+    if (e == cudaSuccess) e = launch_dependent(group_norm_apply_kernel<T, VEC, BWD>, grid2, threads, stat, s, a);
     if (e == cudaSuccess && BWD && a.dw)
         e = launch_dependent(group_norm_params_kernel, dim3((a.Ch + 31) / 32, 2), dim3(32, 32), 0, s, (const float*)a.part, a.N * a.slices, a.Ch, a.dw, a.db);
     return e;
@@ -628,7 +697,12 @@ static int check(const Args& a, int dtype) {
     if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
     if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.G <= 0 || a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
     // a grid of samples x slices, and the groups' numbers in shared memory
-    if (!by_rows(a.S, a.Ch, a.G) && (a.N > 0x7fffffffLL / MAX_SLICES || a.G > GROUPS_MAX)) return KDA_ERR_SHAPE;
+    if (!by_rows(a.S, a.Ch, a.G)) {
+        if (a.N > 0x7fffffffLL / MAX_SLICES || a.G > GROUPS_MAX) return KDA_ERR_SHAPE;
+        Args b = a;
+        cut(b, false);
+        if (b.slices == 0x7fffffff || b.slices > 0x7fffffffLL / a.N) return KDA_ERR_SHAPE;
+    }
     if (by_rows(a.S, a.Ch, a.G) && a.N > (1LL << 40) / a.G) return KDA_ERR_SHAPE;
     return KDA_OK;
 }
@@ -644,7 +718,7 @@ static size_t scratch(long long N, long long S, int Ch, int G, int es, bool bwd)
         return (size_t)step * 2 * Ch * sizeof(float);
     }
     Args a = {};
-    a.N = N; a.S = S;
+    a.N = N; a.S = S; a.Ch = Ch; a.G = G;
     cut(a, bwd);
     return (size_t)N * a.slices * 2 * (Ch + G) * sizeof(float);
 }
