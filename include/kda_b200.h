@@ -324,11 +324,13 @@ int kda_gdr_recurrent_fwd(const void *q, const void *k, const void *v, const voi
                           int32_t HV, int32_t dk, int32_t dv, int32_t dtype, int32_t g_dtype, int32_t flags, float scale,
                           void *cuda_stream);
 
+#define KDA_GROUP_NORM_MAX_GROUPS 24576 /* where S > 1 or a group has more than 1024 channels; else any number */
 /* Group normalisation with an activation, channels last: x, y [N, S, channels], statistics over the S positions and
  * channels / groups channels of every (sample, group); y = act((x - mean) / sqrt(var + eps) * weight + bias), act SiLU or none.
  * weight, bias [channels] may be NULL (1, 0).  mean, rstd [N, groups] are written by the forward and read by the backward unless
  * S == 1 with groups of at most 1024 channels, where they and the forward's scratch may be NULL.  dweight and dbias: both or
- * neither. */
+ * neither.  Elsewhere the scratch has 8 (channels + groups) bytes per slice of a sample (at least one; about 440 over all samples, more
+ * where a sample has over 1024 rows per slice): with few rows a sample that is a multiple of x. */
 int kda_group_norm_scratch_bytes(int64_t N, int64_t S, int32_t channels, int32_t groups, int32_t dtype, size_t *fwd_bytes,
                                  size_t *bwd_bytes);
 int kda_group_norm_fwd(const void *x, const float *weight, const float *bias, void *y, float *mean, float *rstd, float *scratch,

@@ -27,7 +27,7 @@ constexpr int SLICE_THR = 384;    // at most, in the kernels over slices
 constexpr int ROWS_MAX = 1024;    // channels of a group that 32 lanes hold in registers
 constexpr int MAX_SLICES = 256;   // of a sample in the second pass
 constexpr int SUM_ROWS = 1024;    // that one FP32 sum adds up
-constexpr int GROUPS_MAX = 24576; // groups whose numbers fit shared memory where they are not taken row by row
+constexpr int GROUPS_MAX = KDA_GROUP_NORM_MAX_GROUPS; // whose numbers fit shared memory where they are not taken row by row
 
 struct Args {
     const void *x, *dy;
@@ -696,12 +696,12 @@ static cudaError_t dispatch(const Args& a, cudaStream_t s) {
 static int check(const Args& a, int dtype) {
     if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
     if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.G <= 0 || a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
-    // a grid of samples x slices, and the groups' numbers in shared memory
+    // the groups' numbers in shared memory, and grids of samples x slices
     if (!by_rows(a.S, a.Ch, a.G)) {
-        if (a.N > 0x7fffffffLL / MAX_SLICES || a.G > GROUPS_MAX) return KDA_ERR_SHAPE;
+        if (a.G > GROUPS_MAX) return KDA_ERR_SHAPE;
         Args b = a;
-        cut(b, false);
-        if (b.slices == 0x7fffffff || b.slices > 0x7fffffffLL / a.N) return KDA_ERR_SHAPE;
+        cut(b, false);  // (no fewer slices than in the backward)
+        if (b.slices == 0x7fffffff || (b.slices > b.cuts ? b.slices : b.cuts) > 0x7fffffffLL / a.N) return KDA_ERR_SHAPE;
     }
     if (by_rows(a.S, a.Ch, a.G) && a.N > (1LL << 40) / a.G) return KDA_ERR_SHAPE;
     return KDA_OK;

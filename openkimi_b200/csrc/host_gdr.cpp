@@ -387,12 +387,16 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
     if (groups < 1 || sp.Ch < 1 || sp.Ch % groups || sp.Ch > 0x7fffffff)
         value_error("the channels must divide into the groups, got " + std::to_string(sp.Ch) + " channels and " + std::to_string(groups) + " groups");
     if (!(eps >= 0.0)) value_error("eps must not be negative");
+    int64_t positions = 1;
+    for (int64_t i = 1; i + 1 < x.dim(); ++i) positions *= x.size(i);
+    if (groups > KDA_GROUP_NORM_MAX_GROUPS && (positions > 1 || sp.Ch / groups > 1024))
+        value_error("over several positions, or with more than 1024 channels a group, there may be at most " +
+                    std::to_string(KDA_GROUP_NORM_MAX_GROUPS) + " groups, got " + std::to_string(groups));
     for (const OptTensor* t : {&weight, &bias})
         if (*t && ((*t)->dim() != 1 || (*t)->numel() != sp.Ch))
             value_error("weight and bias must have one entry per channel, got " + shape_of(**t));
     same_device(x, "x", "weight", val(weight)); same_device(x, "x", "bias", val(bias));
-    sp.S = 1;
-    for (int64_t i = 1; i + 1 < x.dim(); ++i) sp.S *= x.size(i);
+    sp.S = positions;
     const std::array<const Tensor*, 3> inputs = {&x, &val(weight), &val(bias)};
     refuse_tangents(inputs);
     bool grad = false;

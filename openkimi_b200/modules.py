@@ -207,7 +207,9 @@ def _plain(m, cls):
 def group_norm(x, num_groups, weight=None, bias=None, eps=1e-5, activation=None):
     """Group normalisation of channels-last x [N, ..., channels] with an activation: mean and variance over everything between the
     first and the last axis and over the channels of a group, then ``weight``, ``bias`` (each [channels] or None) and ``activation``
-    (None or "silu").  x of shape [tokens, channels] normalises every token by itself (the heads of a layer's output, say).
+    (None or "silu").  x of shape [tokens, channels] normalises every token by itself (the heads of a layer's output, say); over
+    several positions, or with groups of more than 1024 channels, there may be at most 24576 groups, and the backward of samples of a
+    few rows takes scratch memory of up to 8 bytes an element.
     BF16 or FP32; statistics and parameter gradients in FP32 or more."""
     if activation not in (None, "silu", "swish"):
         raise ValueError(f"group_norm supports activation None or 'silu', got {activation!r}")
