@@ -89,7 +89,8 @@ __device__ __forceinline__ int last_segment(int nc, const Layout& l) { return l.
 // What a CTA walks: chunks cb..ce of a sequence for one value head.
 //   pass 0  whole sequences
 //   pass 1  segments of sequences, for the state they end in: blockIdx.y 0, from zero (the first: from the sequence's own start),
-//           1: from the identity and without values, what the segment makes of the state that it is entered with
+//           1: from the identity and without values, what the segment makes of the state that it is entered with; the last
+//           segment is walked neither way: nothing follows it, and the backward starts behind it
 //   pass 2  segments from the states that gdr_borders_kernel has made of that
 // The backward's segments run from their ends to their starts; its pass 1 takes the transitions of the forward.
 struct Walk {
@@ -131,8 +132,7 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_fwd_tc_kernel(const KdaGdrPar
     wk.init(p, lay, pass == 1 && blockIdx.y, pass == 1 ? lay.segs - 1 : lay.segs);
     const int nc = wk.ce - wk.cb;
     const bool values = pass != 1 || blockIdx.y == 0;
-    // segments that the sequence does not reach; the last one ends in pass 2, and its transition is for the backward
-    if (wk.seg > wk.last || (pass == 1 && wk.seg == wk.last && (values || (p.flags & KDA_FLAG_NO_SAVE)))) return;
+    if (wk.seg > wk.last || (pass == 1 && wk.seg == wk.last)) return;  // (segments that the sequence does not reach)
     wk.c0 += wk.cb;
     wk.tok_begin += (long long)wk.cb * C;
     if (warp == 0) {
@@ -830,8 +830,8 @@ cudaError_t fwd_tc(const KdaGdrParams& p, const Layout& l, cudaStream_t s) {
     const bool save = !(p.flags & KDA_FLAG_NO_SAVE);
     cudaError_t e = cudaSuccess;
     if (l.segs > 1) {
-        // (two segments need no transition in the forward)
-        e = walk(gdr_fwd_tc_kernel<false, false>, dim3(walks * (l.segs - 1), save || l.segs > 2 ? 2 : 1), ft::Map::TOTAL, p, l, 1, s);
+        // (two segments need no transition: the first starts from the sequence's own state, the last's nobody needs)
+        e = walk(gdr_fwd_tc_kernel<false, false>, dim3(walks * (l.segs - 1), l.segs > 2 ? 2 : 1), ft::Map::TOTAL, p, l, 1, s);
         if (e == cudaSuccess) e = borders<false>(p, l, reinterpret_cast<float*>(static_cast<char*>(p.workspace) + l.segE), s);
     }
     if (e != cudaSuccess) return e;
