@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 // four warps of a block of rows write the same
                 const int r = t0 + (lane & 15);
                 float cq = 0.f, ck = 0.f;
-                if (p.flags & KDA_FLAG_QK_L2NORM) {
+                if (grp == 1 && (p.flags & KDA_FLAG_QK_L2NORM)) {
                     const float z = rows(R_ZQ, r), dz = red[R_DZ * C + r];
                     if (rq[r] < 1e6f) cq = rq[r] * rq[r] * (dot(0, r) + z);
                     if (rk[r] < 1e6f) ck = rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + (rows(R_N, r) - (z - dz)) + cols(r) + dz);
