@@ -27,6 +27,7 @@ enum { A_GAM, A_FALL, A_BETA, A_RQ, A_RK, A_GHI, A_GLO, A_LAST, A_BGK, A_FK, A_O
 constexpr int SQ = C * C;          // elements of one part of a 64 x 64 matrix in core-matrix order (cm_idx)
 // BF16 with 128 key channels and value columns goes on tcgen05; T and A are then whole matrices in core-matrix order
 __host__ __device__ __forceinline__ bool on_tc(const KdaGdrParams& p) { return p.dtype == KDA_DTYPE_BF16 && p.dk == 128 && p.dv == 128; }
+constexpr float G_ZERO = -104.f;   // e^g is 0 in FP32 below
 constexpr float G_MIN = -1000.f;   // log decays below count as this: e^-1000 is 0 in FP32, and sums of 64 stay finite
 
 __host__ __device__ __forceinline__ constexpr int blk(int I, int J) { return I * (I + 1) / 2 + J; }
@@ -299,9 +300,11 @@ __device__ __forceinline__ void gate_gradients(const KdaGdrParams& p, const Layo
         const size_t at = (size_t)(ci.tok0 + r) * p.HV + h;
         float d = i ? dg1 : dg0, b = i ? db1 : db0;
         const float be = i ? be1 : be0;
-        if (gate) {
-            const float a = load_g(p, p.g, at) + bias;
-            dA += d * fmaxf(-eA * softplus_f(a), G_MIN);
+        const float a = load_g(p, p.g, at) + bias, decay = gate ? -eA * softplus_f(a) : a;
+        // nothing passes through a token whose decay is 0: what d has there is the rounding of sums that cancel (a NaN is left)
+        if (decay < G_ZERO && d == d) d = 0.f;
+        if (gate && d != 0.f) {  // (e^A_log may be infinite where d is 0)
+            dA += d * fmaxf(decay, G_MIN);
             d *= -eA * (a > 20.f ? 1.f : sigmoid_f(a));
             dbias += d;
         }
