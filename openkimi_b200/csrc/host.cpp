@@ -71,6 +71,7 @@ std::tuple<Tensor, OptTensor> recurrent(const Tensor& q, const Tensor& k, const 
                                ptr<float>(s_in), ptr<float>(s_out), o.data_ptr(), (int)N, (int)T, (int)H, (int)K, (int)K, dtype, flags,
                                (float)scale.value_or(1.0 / std::sqrt((double)K)), stream_of(q)),
              "kda_recurrent_fwd");
+    if (s_out.defined() && inplace && !s_back.defined()) written(s_out);
     if (s_back.defined()) s_out = s_back.copy_(s_out);
     return {o, want_state ? OptTensor(s_out) : OptTensor()};
 }

@@ -306,6 +306,7 @@ std::tuple<Tensor, OptTensor> recurrent_gdr(const Tensor& q, const Tensor& k, co
                                        ptr<float>(s_in), ptr<float>(s_out), o.data_ptr(), (int)N, (int)T, (int)H, (int)HV, (int)K, (int)V,
                                        code(dt), code(gt), (int)flags, (float)scale.value_or(1.0 / std::sqrt((double)K)), stream_of(q)),
                  "kda_gdr_recurrent_fwd");
+        if (inplace && !s_back.defined()) written(s_out);
     }
     if (s_back.defined()) s_out = s_back.copy_(s_out);
     return {o, want_state ? OptTensor(s_out) : OptTensor()};

@@ -145,6 +145,11 @@ T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : n
 
 inline void* stream_of(const Tensor& t) { return at::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
 
+// A kernel has written t: what autograd has saved of it is no longer what it was.  (A tensor made in inference mode has no version.)
+inline void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A cached table belongs to the stream that made it: the current one reads it too, so that its memory waits for both when the cache drops it.
 inline const Tensor& read_here(const Tensor& t) {
     c10::cuda::CUDACachingAllocator::recordStream(t.storage().data_ptr(), at::cuda::getCurrentCUDAStream(t.device().index()));
