@@ -276,6 +276,7 @@ std::tuple<Tensor, OptTensor> recurrent_gdr(const Tensor& q, const Tensor& k, co
     const bool gate = flags & KDA_FLAG_GATE;
     const Tensor &a0 = gate ? val(A_log) : val(std::nullopt), &b0 = gate ? val(dt_bias) : val(std::nullopt), &s0 = val(state);
     same_device(q, "q", "state", s0); same_device(q, "q", "A_log", a0); same_device(q, "q", "dt_bias", b0);
+    refuse_tangents(std::array<const Tensor*, 8>{&q, &k, &v, &g, &beta, &s0, &a0, &b0});
     at::NoGradGuard no_grad;
     c10::cuda::CUDAGuard guard(q.device());
     const auto dt = q.scalar_type(), gt = gate_type(g, beta);
