@@ -297,6 +297,7 @@ std::tuple<Tensor, OptTensor> recurrent_gdr(const Tensor& q, const Tensor& k, co
         }
     }
     Tensor o = fresh(v.sizes(), dt, q);
+    status_word(q.device().index());  // (a wait that gave up in the call that made the state surfaces here)
     if (N * T == 0) {
         if (s_out.defined() && !(s_in.defined() && s_out.data_ptr() == s_in.data_ptr())) {
             if (s_in.defined()) s_out.copy_(s_in);

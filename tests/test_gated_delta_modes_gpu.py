@@ -30,3 +30,19 @@ def test_tangents_are_refused(call, name):
         x[name] = fwd.make_dual(x[name], torch.ones_like(x[name]))
         with pytest.raises((RuntimeError, NotImplementedError)):
             _calls()[call](**x)
+
+
+@pytest.mark.parametrize("call", range(3))
+def test_a_failure_on_the_device_surfaces_in_the_next_call(call):
+    """What a kernel's given-up wait leaves in the words of status: the next call raises, the one after it answers."""
+    from openkimi_b200.ops import _DeviceStatus
+
+    x = _inputs()
+    want = _calls()[call](**x)
+    torch.cuda.synchronize()
+    words = _DeviceStatus.get(torch.device("cuda", torch.cuda.current_device()))
+    words.dev.fill_(32)
+    words.host.fill_(32)
+    with pytest.raises(RuntimeError, match="bounded device-side wait gave up"):
+        _calls()[call](**x)
+    assert torch.equal(_calls()[call](**x)[0], want[0])
