@@ -325,8 +325,8 @@ int kda_gdr_recurrent_fwd(const void *q, const void *k, const void *v, const voi
                           void *cuda_stream);
 
 #define KDA_GROUP_NORM_MAX_GROUPS 24576 /* where S > 1 or a group has more than 1024 channels; else any number */
-/* Group normalisation with an activation, channels last: x, y [N, S, channels], statistics over the S positions and
- * channels / groups channels of every (sample, group); y = act((x - mean) / sqrt(var + eps) * weight + bias), act SiLU or none.
+/* Group normalisation with an activation, channels last: x, y [N, S, channels] of at most 2^30 channels, statistics over the S
+ * positions and channels / groups channels of every (sample, group); y = act((x - mean) / sqrt(var + eps) * weight + bias), act SiLU or none.
  * weight, bias [channels] may be NULL (1, 0).  mean, rstd [N, groups] are written by the forward and read by the backward unless
  * S == 1 with groups of at most 1024 channels, where they and the forward's scratch may be NULL.  dweight and dbias: both or
  * neither.  Elsewhere the scratch has 8 (channels + groups) bytes per slice of a sample (at least one; about 440 over all samples, more

@@ -695,7 +695,8 @@ static cudaError_t dispatch(const Args& a, cudaStream_t s) {
 
 static int check(const Args& a, int dtype) {
     if (dtype != KDA_DTYPE_F32 && dtype != KDA_DTYPE_BF16) return KDA_ERR_DTYPE;
-    if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.G <= 0 || a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
+    if (a.N <= 0 || a.S <= 0 || a.Ch <= 0 || a.Ch > 1 << 30 || a.G <= 0 ||  // (two rows of channels are counted in 32 bits)
+         a.Ch % a.G || !(a.eps >= 0.f)) return KDA_ERR_SHAPE;
     // the groups' numbers in shared memory, and grids of samples x slices
     if (!by_rows(a.S, a.Ch, a.G)) {
         if (a.G > GROUPS_MAX) return KDA_ERR_SHAPE;

@@ -387,8 +387,8 @@ Tensor group_norm(const Tensor& x, int64_t groups, const OptTensor& weight, cons
         type_error(std::string("x must be float32 or bfloat16, got ") + c10::toString(x.scalar_type()));
     NormSpec sp;
     sp.N = x.size(0); sp.Ch = x.size(-1); sp.G = groups; sp.eps = eps; sp.silu = silu;
-    if (groups < 1 || sp.Ch < 1 || sp.Ch % groups || sp.Ch > 0x7fffffff)
-        value_error("the channels must divide into the groups, got " + std::to_string(sp.Ch) + " channels and " + std::to_string(groups) + " groups");
+    if (groups < 1 || sp.Ch < 1 || sp.Ch % groups || sp.Ch > 1 << 30)
+        value_error("the channels, at most 2^30, must divide into the groups, got " + std::to_string(sp.Ch) + " channels and " + std::to_string(groups) + " groups");
     if (!(eps >= 0.0)) value_error("eps must not be negative");
     int64_t positions = 1;
     for (int64_t i = 1; i + 1 < x.dim(); ++i) positions *= x.size(i);

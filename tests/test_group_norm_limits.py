@@ -41,3 +41,8 @@ def test_samples_and_groups():
         group_norm(z, 24577)
     assert group_norm(z[:, 0], 24577).shape == (1, 24577)
     assert torch.equal(group_norm(z[..., :24576] + 3, 24576), torch.zeros_like(z[..., :24576]))
+
+
+def test_channels_that_32_bits_count_twice():
+    assert _scratch(1, 1, 2 ** 30, 2 ** 20)[0] == 0
+    assert _scratch(1, 1, 2 ** 31 - 1024, 2 ** 21 - 1)[0] == 2 and _scratch(1, 3, 2 ** 31 - 1, 1)[0] == 2
