@@ -3,9 +3,10 @@
 // With one decay per head the pairwise decays of a chunk are numbers, not vectors: q k^T and k k^T are plain products of the
 // rows as they arrive, and decay, beta and the rows' 1 / norm multiply the results in FP32.  So in BF16 mode every product has
 // an operand that BF16 holds exactly (q, k, do) or two computed ones (T, V', S, ...).  Computed operands are BF16 in up to three
-// parts, x = p0 + p1 + p2 to 2^-24, and a product of parts i and j is taken where i + j < 3: FP32-class results (measured against
-// 64 bits: 1e-7 to 3e-7 on mma.sync, 2e-7 to 1.7e-6 on tcgen05, whose accumulators truncate) from tensor cores with FP32 accumulators.  Where only a BF16 output can see the difference two parts do
-// (2^-17).  FP32 tensors go the same way with three parts for q, k, v, do as well.
+// parts, x = p0 + p1 + p2 to 2^-24, and a product of parts i and j is taken where i + j < 3: from tensor cores with FP32 accumulators
+// results that are 1e-7 to 4e-7 of their norm from 64 bits on mma.sync, and on tcgen05, whose accumulators truncate, 2e-7 to 6e-7 for
+// states and up to 1.7e-6 for dg and dbeta.  Where only a BF16 output can see the difference two parts do (2^-17: three outputs in a
+// thousand are rounded to the neighbour of the nearest BF16 number).  FP32 tensors go the same way with three parts for q, k, v, do as well.
 #pragma once
 
 #include "kda_common.cuh"
@@ -43,9 +44,12 @@ inline int longest(const KdaGdrParams& p) {  // chunks of the longest sequence, 
 }
 // Segments of the longest sequence in the walks on tcgen05 (gdr_tc.cu).  A walk is a chain of chunks; where walks are few, or one is
 // much longer than its share, sequences are cut into segments of equal length that are walked twice: from zero (and from the identity,
-// for what a segment does to the state that it is entered with), and again from the states that follow.  Estimated with what a chunk
-// costs (3.2 us without outputs, 3.7 us with), a border (2.6 us) and the launches (12 us): equal sequences go in waves, packed ones
-// fill the SMs up to half a segment.  8 walks of 512 chunks, forward: 2312 -> 485 us.
+// for what a segment does to the state that it is entered with), and again from the states that follow.  Estimated with 3.2 us for a
+// chunk without outputs and 3.7 with, 2.6 us for a border and 12 us for the launches: equal sequences go in waves, packed ones fill the
+// SMs up to half a segment.  8 walks of 512 chunks, forward: 2312 -> 485 us.  The estimate is rough: a chunk takes 3.8 us without
+// outputs and 4.5 to 6.5 with (gdr_tc.cu), the backward is not estimated by itself, and of packed documents it takes the first pass for
+// free where most of them end in their first segment (24 571 tokens of 12 documents, 8 heads: two segments, a first pass of 165 us).
+// It tends to too few segments.
 inline int segment_count(const KdaGdrParams& p) {
     if (!on_tc(p)) return 1;
     const int nc = longest(p), sms = sm_count();

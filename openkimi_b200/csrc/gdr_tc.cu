@@ -10,7 +10,8 @@
 // Bound by the chain of a chunk: split S - S k - R - R T - V' - W k - S.  Everything else is off it: two producer warps bring the next
 // chunk's rows (core-matrix order) and records, one warp issues all products, four warps turn finished outputs into rows.  A chunk of
 // 64 tokens takes 4.5 us with few CTAs, 5.8 forward and 6.5 backward with 96 that save their records (16 x 2048 tokens of 6 heads: 185
-// and 207 us, 3 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.
+// and 207 us, 3 TB/s of records and rows); on mma.sync, in panels of 32 columns on 384 CTAs, 479 and 494.  At 128 registers a thread the
+// forward spills 52 bytes and the backward 212.
 #include "gdr.cuh"
 
 namespace kda {
@@ -757,8 +758,8 @@ __global__ void __launch_bounds__(ft::NTHR, 1) gdr_bwd_tc_kernel(const KdaGdrPar
 }
 
 // States at the segments' borders, 8 columns of one (sequence, head) per CTA: forward, E_j <- X_j E_{j-1} + E_j for j = 1, 2, ..; backward
-// (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  2.6 us a border (8 heads); FP32 multiply-adds; the X
-// of the next two segments arrive meanwhile.  2.6 us a border (8 heads); with 512 threads, two to a sum, 3.5.
+// (TR), F_j <- X_j^T F_{j+1} + F_j for j = segs - 2 downwards.  FP32 multiply-adds; the X of the next two segments arrive meanwhile.
+// 2.6 us a border (8 heads); with 512 threads, two to a sum, 3.5.
 constexpr int LDX = 132, XBUF = 3;  // floats per row of X, its copies
 template <bool TR>
 __global__ void __launch_bounds__(256) gdr_borders_kernel(const KdaGdrParams p, const Layout lay, float* M, const float* X) {

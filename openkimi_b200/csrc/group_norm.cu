@@ -12,8 +12,8 @@
 //     the slices at the start of the second pass, which applies.  Backward: per slice and channel the sums of dz and dz x^, which
 //     give dw, db and, weighted with w, m1 and m2; then dx.  The second pass reads from L2 what fits there.
 // Bound by issue slots (70 % of them used in the first form) and by the latency of small slices: [32768, 768] in groups of 128, BF16
-// with SiLU, takes 26 us forward (3.8 TB/s) and 49 backward (3.1 TB/s); [4, 8191, 768] in 32 groups 47 and 64 (3.2 and 4.3 TB/s of
-// what its passes read and write).  In the first form the two took 172 and 291 us; what made them faster is two values an instruction, a
+// with SiLU, takes 26 us forward (3.8 TB/s) and 49 backward (3.1 TB/s, 72 bytes of spills); [4, 8191, 768] in 32 groups 49 and 64
+// (3.1 and 4.3 TB/s of what its passes read and write).  In the first form the two took 172 and 291 us; what made them faster is two values an instruction, a
 // thread's channels all of one group, rows kept as they lie in memory until they are used, and a grid of what is resident.
 // Sums are in FP32 over at most 1024 rows, then in 64 bits in a fixed order: no atomics.
 #include "kda_common.cuh"
@@ -334,7 +334,8 @@ __global__ void __launch_bounds__(1024) group_norm_params_kernel(const float* pa
 // ---- samples of several positions -------------------------------------------------------------------------------------
 // A CTA has one slice of one sample; thread = (row of TR, VEC channels), channels in blocks of SLICE_THR * VEC where a row is wider than
 // the CTA.
-// CTAs per SM that registers allow without spilling
+// CTAs per SM.  With the 56 and 80 registers a thread that leaves, the second pass spills 72 bytes forward and 156 backward in its
+// 16-byte BF16 form, the first pass next to nothing
 __host__ __device__ constexpr int slice_ctas(bool bwd) { return bwd ? 2 : 3; }
 struct Slice {
     long long n, i, s0, s1;
