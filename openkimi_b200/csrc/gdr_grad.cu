@@ -23,7 +23,10 @@ namespace gdr {
 // half = warp / 4 of the columns.
 namespace gr {
 constexpr int NTHR = 256, EP = 32, LDE = EP + 8, PAN = C * LDE, LDZ = C + 8;
-enum { R_N = 0, R_B = 2, R_F = 4, R_E = 6, R_H = 8, R_Y = 10, R_COL = 11, RED = 15 };  // rows of `red`: sums of N (2 halves), dL KKD (2), q.F (2), k.E (2), k.H (2), Y.v, columns of N (4)
+enum { R_B = 0, R_F = 2, R_E = 4, R_H = 6, R_Y = 8, RED = 9 };  // rows of `red`: sums of dL KKD (2 halves), q.F (2), k.E (2), k.H (2), Y.v
+// rows of `sumN`, in 64 bits: sums over rows of N (2 halves) and over its columns (4 blocks of rows).  In dG's running sum a pair of rows
+// cancels between its row and its column: with sums in FP32 their rounding was left, 4e-6 of dA_log's terms at decays of e^-0.3 to e^-32.
+enum { N_ROW = 0, N_COL = 2, SUMN = 6 };
 }
 
 // the chunk's rows and where its 64 x 64 matrices go
@@ -36,6 +39,7 @@ struct GradRows {
     uint32_t za, xa;
     const float *gam, *fall, *be, *rq, *rk, *ghi, *glo;
     float* red;
+    double* sumN;
     float last;
 };
 
@@ -75,11 +79,12 @@ __device__ __forceinline__ void grad_pairs(const GradRows<T, K>& m, float scale,
     constexpr int PO = In<T>::PO;
     const int g = lane >> 2, t = lane & 3;
     const int r0 = 16 * rb + g;
-    float rn[2] = {0.f, 0.f}, rbeta[2] = {0.f, 0.f};
+    double rn[2] = {0.0, 0.0};
+    float rbeta[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         if (2 * half + j / 2 > rb) break;
-        float col[2] = {0.f, 0.f};
+        double col[2] = {0.0, 0.0};
         const int j0 = 32 * half + 8 * j + 2 * t;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -106,7 +111,7 @@ __device__ __forceinline__ void grad_pairs(const GradRows<T, K>& m, float scale,
         for (int y = 0; y < 2; ++y) {
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) col[y] += __shfl_xor_sync(0xffffffffu, col[y], o);
-            if (g == 0) m.red[(R_COL + rb) * C + j0 + y] = col[y];
+            if (g == 0) m.sumN[(N_COL + rb) * C + j0 + y] = col[y];
         }
     }
 #pragma unroll
@@ -117,7 +122,7 @@ __device__ __forceinline__ void grad_pairs(const GradRows<T, K>& m, float scale,
             rbeta[i] += __shfl_xor_sync(0xffffffffu, rbeta[i], o);
         }
         if (t == 0) {
-            m.red[(R_N + half) * C + r0 + 8 * i] = rn[i];
+            m.sumN[(N_ROW + half) * C + r0 + 8 * i] = rn[i];
             m.red[(R_B + half) * C + r0 + 8 * i] = rbeta[i];
         }
     }
@@ -213,12 +218,12 @@ __device__ __forceinline__ void grad_finish(const KdaGdrParams& p, const Layout&
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = 2 * lane + i, I = r >> 4;
-            float colsum = 0.f;
-            for (int x = I; x < 4; ++x) colsum += m.red[(R_COL + x) * C + r];
-            const float n = m.red[R_N * C + r] + m.red[(R_N + 1) * C + r], bb = m.red[R_B * C + r] + m.red[(R_B + 1) * C + r];
+            double n = m.sumN[N_ROW * C + r] + m.sumN[(N_ROW + 1) * C + r];
+            for (int x = I; x < 4; ++x) n -= m.sumN[(N_COL + x) * C + r];
+            const float bb = m.red[R_B * C + r] + m.red[(R_B + 1) * C + r];
             const float f = m.red[R_F * C + r] + m.red[(R_F + 1) * C + r], e = m.red[R_E * C + r] + m.red[(R_E + 1) * C + r],
                         hh = m.red[R_H * C + r] + m.red[(R_H + 1) * C + r];
-            dG[i] = (double)n - colsum + f - (double)m.be[r] * e - hh;
+            dG[i] = n + f - (double)m.be[r] * e - hh;
             hsum += hh;
             db[i] = m.red[R_Y * C + r] - e + bb;
         }
@@ -297,8 +302,9 @@ struct GradMap {
                          DS = S0 + 3 * K * gr::LDE, END = DS + 3 * K * gr::LDE;
     static constexpr int Z = DO, X = Z + PO * C * gr::LDZ;  // over the panels, once they have been used
     static_assert(X + PO * C * gr::LDZ <= END, "Z and X fit");
-    static constexpr int FLOATS = 7 * C + 16 * C;            // rows' numbers; sums over rows and columns
-    static constexpr int BYTES = 2 * END + FLOATS * 4;
+    static constexpr int FLOATS = 7 * C + (gr::RED + 1) * C; // rows' numbers; sums over rows
+    static constexpr int BYTES = 2 * END + FLOATS * 4 + gr::SUMN * C * 8;
+    static_assert((2 * END + FLOATS * 4) % 8 == 0, "sums in 64 bits");
 };
 
 template <typename T, int K>
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(256) gdr_grad_kernel(const KdaGdrParams p, con
     const float* aux = reinterpret_cast<const float*>(ws + lay.aux) + unit * AUX;
     for (int i = tid; i < 7 * C; i += NTHR) sx[i] = aux[i];
     const GradRows<T, K> m = {sm + M::Q, sm + M::KK, sa + 2 * M::Q, sa + 2 * M::KK, sm + M::Z, sm + M::X, sa + 2 * M::Z, sa + 2 * M::X,
-                              sx, sx + C, sx + 2 * C, sx + 3 * C, sx + 4 * C, sx + 5 * C, sx + 6 * C, red, aux[A_LAST * C]};
+                              sx, sx + C, sx + 2 * C, sx + 3 * C, sx + 4 * C, sx + 5 * C, sx + 6 * C, red, reinterpret_cast<double*>(sx + M::FLOATS), aux[A_LAST * C]};
 
     float F[NK][4], E[NK][4], H[NK][4], dA[4][4], dL[4][4];
 #pragma unroll

@@ -34,14 +34,17 @@ constexpr uint32_t Q = 0, KK = 16384, AU = 32768, TILE = AU + AUX * 4;
 // [4 x 64][16], all in core-matrix order
 constexpr uint32_t SPART = 4096, YPART = 2048, S0 = 0, DS = 3 * SPART, V = 6 * SPART, B = V + 6144, STAGE = B + 4 * YPART;
 // Z^T, X^T: two parts each in core-matrix order, then dq and dk as rows
-constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 20 * C * 4,
-                   TOTAL = DOTS + 12 * C * 4;
+constexpr uint32_t R0 = 2 * TILE, Z = R0 + RING * STAGE, X = Z + 2 * MAT, RED = X + 2 * MAT, DOTS = RED + 12 * C * 4,
+                   SUMN = DOTS + 12 * C * 4, TOTAL = SUMN + 8 * C * 8;
 static_assert(TOTAL <= 232448 - 1024 && TILE % 1024 == 0, "fits");
 // tensor memory columns; E^T in two halves that are added up (products with the first and the second part of Y)
 constexpr uint32_t T_F = 0, T_E = 64, T_H = 192, T_DA = 256, T_DL = 320, T_DQ = 384, T_DK = 448;
-// sums over 64 x 64 matrices with rows i, columns j: of N over columns j by block of i (4); over rows i by block of j: N (4), Z qk^T (4),
-// dL KKD (4); diagonals of Z qk^T and of Y V'^T; the factors of q and k in the gradient of the L2 norm
-enum { R_COL = 0, R_N = 4, R_ZQ = 8, R_B = 12, R_DZ = 16, R_DY = 17, R_CQ = 18, R_CK = 19 };
+// sums over 64 x 64 matrices with rows i, columns j: over rows i by block of j: Z qk^T (4), dL KKD (4); diagonals of Z qk^T and of
+// Y V'^T; the factors of q and k in the gradient of the L2 norm
+enum { R_ZQ = 0, R_B = 4, R_DZ = 8, R_DY = 9, R_CQ = 10, R_CK = 11 };
+// the same in 64 bits: of N over columns j by block of i (4), over rows i by block of j (4).  In dG's running sum a pair of rows cancels
+// between its row and its column: with sums in FP32 their rounding was left, 4e-6 of dA_log's terms at decays of e^-0.3 to e^-32.
+enum { N_COL = 0, N_ROW = 4 };
 }  // namespace gt
 
 // 16 lanes x 16 consecutive columns as fragments: f[i] is (row g, columns 8 i + 2 t, + 1), (row g + 8, the same)
@@ -130,16 +133,19 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
         const float* x = dots + which * 4 * C + r;
         return (x[0] + x[C]) + (x[2 * C] + x[3 * C]);
     };
-    auto rows = [&](int which, int r) {  // sum over row r, the blocks of columns up to its own
-        float s = 0.f;
+    double* sumN = reinterpret_cast<double*>(dyn + SUMN);
+    auto rows = [&](const auto* of, int r) {  // sum over row r, the blocks of columns up to its own
+        auto s = of[r];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s += j <= r >> 4 ? red[(which + j) * C + r] : 0.f;
+        for (int j = 1; j < 4; ++j)
+            if (j <= r >> 4) s += of[j * C + r];
         return s;
     };
-    auto cols = [&](int r) {  // sum over column r, the blocks of rows from its own on
-        float s = 0.f;
+    auto cols = [&](int r) {  // sum of N over column r, the blocks of rows from its own on
+        double s = sumN[(N_COL + 3) * C + r];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s += i >= r >> 4 ? red[(R_COL + i) * C + r] : 0.f;
+        for (int i = 0; i < 3; ++i)
+            if (i >= r >> 4) s += sumN[(N_COL + i) * C + r];
         return s;
     };
     bool ok = true;
@@ -204,10 +210,11 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             if (any) {  // ---- pairs of rows: 16 rows j x 16 columns i
                 const int r0 = 16 * rb + g;
                 const float gj[2] = {ghi[r0], ghi[r0 + 8]}, lj[2] = {glo[r0], glo[r0 + 8]}, kj[2] = {rk[r0], rk[r0 + 8]};
-                float cn[2] = {0.f, 0.f};
+                double cn[2] = {0.0, 0.0};
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    float rn[2] = {0.f, 0.f}, rz[2] = {0.f, 0.f}, rl[2] = {0.f, 0.f};
+                    double rn[2] = {0.0, 0.0};
+                    float rz[2] = {0.f, 0.f}, rl[2] = {0.f, 0.f};
                     const int i0 = t0 + 8 * j + 2 * t;
                     const float2 gi = load2(ghi + i0), li = load2(glo + i0), qi = load2(rq + i0), ki = load2(rk + i0), bi = load2(be + i0);
 #pragma unroll
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                             rz[y] += __shfl_xor_sync(0xffffffffu, rz[y], o);
                         }
                         if (g == 0) {
-                            red[(R_N + rb) * C + i0 + y] = rn[y];
+                            sumN[(N_ROW + rb) * C + i0 + y] = rn[y];
                             red[(R_ZQ + rb) * C + i0 + y] = rz[y];
                         }
                         if (tiny) {
@@ -259,7 +266,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int o = 1; o < 4; o <<= 1) cn[i] += __shfl_xor_sync(0xffffffffu, cn[i], o);
-                    if (t == 0) red[(R_COL + ib) * C + r0 + 8 * i] = cn[i];
+                    if (t == 0) sumN[(N_COL + ib) * C + r0 + 8 * i] = cn[i];
                 }
                 fence_async_smem();
             }
@@ -312,9 +319,9 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                 const int r = t0 + (lane & 15);
                 float cq = 0.f, ck = 0.f;
                 if (grp == 1 && (p.flags & KDA_FLAG_QK_L2NORM)) {
-                    const float z = rows(R_ZQ, r), dz = red[R_DZ * C + r];
+                    const float z = rows(red + R_ZQ * C, r), dz = red[R_DZ * C + r];
                     if (rq[r] < 1e6f) cq = rq[r] * rq[r] * (dot(0, r) + z);
-                    if (rk[r] < 1e6f) ck = rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + (rows(R_N, r) - (z - dz)) + cols(r) + dz);
+                    if (rk[r] < 1e6f) ck = rk[r] * rk[r] * (dot(2, r) - be[r] * dot(1, r) + ((float)rows(sumN + N_ROW * C, r) - (z - dz)) + (float)cols(r) + dz);
                 }
                 red[R_CQ * C + r] = cq;
                 red[R_CK * C + r] = ck;
@@ -549,7 +556,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             for (int i = 0; i < 2; ++i) {
                 const int r = 2 * lane + i;
                 const float e = dot(1, r), h1 = dot(2, r);
-                dG[i] = (double)rows(R_N, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
+                dG[i] = rows(sumN + N_ROW * C, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
                 hsum += h1;
                 // Y_i . V'_i / beta_i; where beta_i is 0, or so small that the quotient means nothing, Y_i . v_i less what the chunk
                 // predicts for v_i
@@ -560,7 +567,7 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                     float yv = 0.f;
                     if (r < ci.len) {
                         for (int x = 0; x < 128; ++x) yv = fmaf(y[x], ldf(static_cast<const bf16*>(p.v) + (((size_t)ci.tok0 + r) * p.HV + h) * 128 + x), yv);
-                        yv += rows(R_B, r) - e;
+                        yv += rows(red + R_B * C, r) - e;
                     }
                     db[i] = yv;
                 }
