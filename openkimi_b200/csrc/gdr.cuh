@@ -291,6 +291,24 @@ __device__ __forceinline__ size_t state_at(const KdaGdrParams& p, int d, int e) 
     return (p.flags & KDA_FLAG_STATE_V_FIRST) ? (size_t)e * p.dk + d : (size_t)d * p.dv + e;
 }
 
+// Gradients of the log decays from those of their running sums, a lane has two neighbouring rows: d the rows' gradients but for what the
+// end of the chunk adds, to the last row h_j of every row j with -h_j at row j itself, and end = e^G_last <S0, dS>.  The sum over rows from
+// t on then has the h_j of the rows before t: summed up as those, not as what is left of -h_j + h_j.
+__device__ __forceinline__ float2 decay_gradients(const double (&d)[2], const double (&h)[2], double end, int lane) {
+    double after = d[0] + d[1], before = h[0] + h[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const double a = __shfl_down_sync(0xffffffffu, after, o), b = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane + o < 32) after += a;
+        if (lane >= o) before += b;
+    }
+    after = __shfl_down_sync(0xffffffffu, after, 1);
+    before = __shfl_up_sync(0xffffffffu, before, 1);
+    if (lane == 31) after = 0.0;
+    if (lane == 0) before = 0.0;
+    const double r1 = after + d[1], r0 = r1 + d[0];
+    return make_float2((float)(r0 + (before + end)), (float)(r1 + (before + h[0] + end)));
+}
 // the gradients of g, beta and a unit's share of those of A_log, dt_bias from those of log decay and beta; a lane has two neighbouring rows
 __device__ __forceinline__ void gate_gradients(const KdaGdrParams& p, const Layout& lay, const ChunkInfo& ci, size_t unit, int h, float dg0, float dg1,
                                                float db0, float db1, float be0, float be1, int lane) {

@@ -213,7 +213,7 @@ __device__ __forceinline__ void grad_finish(const KdaGdrParams& p, const Layout&
         }
     }
     if (w == 0) {  // the gate's and beta's gradients, two neighbouring rows per lane
-        double dG[2], hsum = 0.0;
+        double dG[2], h1[2];
         float db[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -223,21 +223,12 @@ __device__ __forceinline__ void grad_finish(const KdaGdrParams& p, const Layout&
             const float bb = m.red[R_B * C + r] + m.red[(R_B + 1) * C + r];
             const float f = m.red[R_F * C + r] + m.red[(R_F + 1) * C + r], e = m.red[R_E * C + r] + m.red[(R_E + 1) * C + r],
                         hh = m.red[R_H * C + r] + m.red[(R_H + 1) * C + r];
-            dG[i] = n + f - (double)m.be[r] * e - hh;
-            hsum += hh;
+            dG[i] = n + f - (double)m.be[r] * e;
+            h1[i] = hh;
             db[i] = m.red[R_Y * C + r] - e + bb;
         }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
-        double run = dG[0] + dG[1];
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const double dn = __shfl_down_sync(0xffffffffu, run, o);
-            if (lane + o < 32) run += dn;
-        }
-        run += (double)m.last * total + hsum;
-        const double dg[2] = {run, run - dG[0]};
-        gate_gradients(p, lay, ci, unit, h, (float)dg[0], (float)dg[1], db[0], db[1], m.be[2 * lane], m.be[2 * lane + 1], lane);
+        const float2 dg = decay_gradients(dG, h1, (double)m.last * total, lane);
+        gate_gradients(p, lay, ci, unit, h, dg.x, dg.y, db[0], db[1], m.be[2 * lane], m.be[2 * lane + 1], lane);
     }
     if (grp > 1) {  // the group's value heads are added up by gdr_heads_kernel
         float* out = reinterpret_cast<float*>(static_cast<char*>(p.bwd_scratch) + lay.dqk) + unit * 2 * C * K;

@@ -550,14 +550,14 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
             ok = __all_sync(0xffffffffu, mbar_wait(&sums, it & 1, p, 1 << 8));
             if (!ok) break;
             const float last = aux[A_LAST * C], total = ((ss[tb][0] + ss[tb][1]) + (ss[tb][2] + ss[tb][3])) + ((ss[tb][4] + ss[tb][5]) + (ss[tb][6] + ss[tb][7]));
-            double dG[2], hsum = 0.0;
+            double dG[2], h1[2];
             float db[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int r = 2 * lane + i;
-                const float e = dot(1, r), h1 = dot(2, r);
-                dG[i] = rows(sumN + N_ROW * C, r) - cols(r) + dot(0, r) - (double)be[r] * e - h1;
-                hsum += h1;
+                const float e = dot(1, r);
+                dG[i] = rows(sumN + N_ROW * C, r) - cols(r) + dot(0, r) - (double)be[r] * e;
+                h1[i] = dot(2, r);
                 // Y_i . V'_i / beta_i; where beta_i is 0, or so small that the quotient means nothing, Y_i . v_i less what the chunk
                 // predicts for v_i
                 if (fabsf(be[r]) > 1e-18f) {
@@ -572,16 +572,8 @@ __global__ void __launch_bounds__(gt::NTHR, 1) gdr_grad_tc_kernel(const KdaGdrPa
                     db[i] = yv;
                 }
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) hsum += __shfl_xor_sync(0xffffffffu, hsum, o);
-            double run = dG[0] + dG[1];
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double dn = __shfl_down_sync(0xffffffffu, run, o);
-                if (lane + o < 32) run += dn;
-            }
-            run += (double)last * total + hsum;
-            gate_gradients(p, lay, ci, (size_t)u, h, (float)run, (float)(run - dG[0]), db[0], db[1], be[2 * lane], be[2 * lane + 1], lane);
+            const float2 dg = decay_gradients(dG, h1, (double)last * total, lane);
+            gate_gradients(p, lay, ci, (size_t)u, h, dg.x, dg.y, db[0], db[1], be[2 * lane], be[2 * lane + 1], lane);
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&gatefree);

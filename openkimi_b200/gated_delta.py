@@ -44,9 +44,8 @@ def chunk_gated_delta_rule(q, k, v, g, beta, scale=None, initial_state=None, out
 
     Sums, states and pairwise decays are in FP32; BF16 inputs are multiplied exactly and computed operands in 24 bits.  Of its norm a
     result in FP32 is about 4e-7 from 64 bits, and with BF16 inputs and K = V = 128 up to 6e-7 for states and 1.7e-6 for the gradients
-    of g, beta, A_log and dt_bias.  The gradient of g is a running sum of differences: of tokens that hardly reach back (decays of
-    e^-15 and less all over a chunk) it is as good as the chunk's largest allows; at a decay below e^-104, 0 in FP32, it is 0.  k and v
-    are cast to the type of q, and g and beta to FP32 unless both are BF16.
+    of g, beta, A_log and dt_bias.  At a decay below e^-104, 0 in FP32, the gradient of g is 0.  k and v are cast to the type of q, and
+    g and beta to FP32 unless both are BF16.
 
     Differentiated calls keep about (4 K V + 256 V + 34000) bytes per 64 tokens and value head for the backward (BF16 with K = V =
     128: 173 KB).  Where long sequences are cut into segments (BF16, K = V = 128), every sequence and head has room for as many as the
