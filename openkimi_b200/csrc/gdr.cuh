@@ -291,9 +291,9 @@ __device__ __forceinline__ size_t state_at(const KdaGdrParams& p, int d, int e) 
     return (p.flags & KDA_FLAG_STATE_V_FIRST) ? (size_t)e * p.dk + d : (size_t)d * p.dv + e;
 }
 
-// Gradients of the log decays from those of their running sums, a lane has two neighbouring rows: d the rows' gradients but for what the
-// end of the chunk adds, to the last row h_j of every row j with -h_j at row j itself, and end = e^G_last <S0, dS>.  The sum over rows from
-// t on then has the h_j of the rows before t: summed up as those, not as what is left of -h_j + h_j.
+// Gradients of the log decays from those of their running sums G; a lane has two neighbouring rows.  d: the rows' gradients without the
+// share of the chunk's end, which is h_j at the last row and -h_j at row j itself for every row j.  Summed from row t on, the h_j of the
+// rows before t remain: they are added up as such, not as what is left of -h_j + h_j.  end = e^G_last <S0, dS>.
 __device__ __forceinline__ float2 decay_gradients(const double (&d)[2], const double (&h)[2], double end, int lane) {
     double after = d[0] + d[1], before = h[0] + h[1];
 #pragma unroll
